@@ -383,6 +383,48 @@ int rh3_vae_gemm_swiglu(const void* xq, int64_t lda, const void* wq, const float
                         const void* bias_f16, int64_t M, int64_t N, int64_t K, void* out_f16, int64_t ldo,
                         cudaStream_t stream);
 
+/* ---- quantized key/value cache (a language model's attention: the text encoder's) -----------------------------
+ * No reference counterpart: the reference quantizes K and V anew for every call (attn_int8.cu). The row arithmetic is that of the
+ * row quantizers (custom_nodes/rapid_h3/kernels.py:75-82).
+ *
+ * Cache: codes kc, vc [pages][heads][page][D] bytes (kind 0: int8, 1: e4m3), scales ks, vs fp32 [pages][heads][page]; page = 16, 32, 64 or
+ * 128 tokens, D = 64 or 128; all four 16-byte aligned.
+ * Batch: table int32 [B] rows of per_seq pages at table_stride, the pages of each sequence in order; lens int32 [B], the tokens each
+ * sequence holds, the call's own among them; starts int32 [B + 1], ascending: rows starts[b] .. starts[b + 1] - 1 of the call are the last
+ * tokens of sequence b. They are read on the device: a captured call follows them. Rows at or behind starts[B] (T may be larger: a padded
+ * batch) are left as they were. Tokens that lie nowhere (before position 0, beyond the table, in a page outside the cache)
+ * are not written, read as zeros and are masked; a page outside the cache also leaves status 120 (rh3_check_status).
+ * dtype: 0 = bf16, 1 = fp16, 2 = fp32 (write and read only). Every row must start on a 16-byte boundary.
+ *
+ * rh3_kv_write: s = max(amax / (127 | 448), 1e-12), codes round-to-nearest-even of x / s. A row with a NaN or an infinity keeps it in its
+ *   scale and reads back as NaN. Sequences that share pages write them in no particular order: they must not write the same token.
+ * rh3_kv_read: k, v [T][heads][D] contiguous = codes * scale in fp32, rounded once to dtype.
+ * rh3_kv_attn: out[t, head] = softmax(scale * q . k) v over the keys of the row's sequence, at most its own position if causal; heads * group
+ *   query heads, head h * group + i reads KV head h. A row without a key gives 0. With prefix > 0 every row sees the first
+ *   `prefix` tokens of prefix_table's pages as well, before its own keys; lens, starts and positions then count the own part alone.
+ *   workspace: rh3_kv_attn_workspace_bytes() bytes, 256-byte aligned, in use until the call's kernels are done. */
+typedef struct rh3_kv_attn_args {
+  const void* q; int64_t q_st, q_sh;   /* [T][heads * group][D], token and head strides */
+  void* out; int64_t o_st, o_sh;
+  const void* k; const void* v; const float* ks; const float* vs;
+  int64_t pages, heads, page, D;
+  const int32_t* table; int64_t table_stride, per_seq;
+  const int32_t* lens; const int32_t* starts; int64_t B, T;
+  int64_t group;
+  const int32_t* prefix_table; int64_t prefix_pages, prefix;
+  float scale; int32_t kind, dtype, causal;
+} rh3_kv_attn_args;
+int rh3_kv_write(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, int dtype, void* kc,
+                 void* vc, float* ks, float* vs, int64_t pages, int64_t heads, int64_t page, int64_t D, int kind,
+                 const int32_t* table, int64_t table_stride, int64_t per_seq, const int32_t* lens, const int32_t* starts,
+                 int64_t B, int64_t T, cudaStream_t stream);
+int rh3_kv_read(const void* kc, const void* vc, const float* ks, const float* vs, int64_t pages, int64_t heads, int64_t page,
+                int64_t D, int kind, const int32_t* table, int64_t table_stride, int64_t per_seq, const int32_t* lens,
+                const int32_t* starts, int64_t B, int64_t T, void* k, void* v, int dtype, cudaStream_t stream);
+int64_t rh3_kv_attn_workspace_bytes(int64_t heads, int64_t group, int64_t page, int64_t D, int64_t per_seq, int64_t B, int64_t T,
+                                    int64_t prefix);
+int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t workspace_bytes, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

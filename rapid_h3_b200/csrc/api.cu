@@ -427,7 +427,8 @@ extern "C" int rh3_check_status(cudaStream_t stream, int* status_out) {
   if (int e = rh3::check_cuda(cudaStreamSynchronize(stream), "status sync")) return e;
   if (v != 0) {
     if (int e = rh3::check_cuda(cudaMemsetAsync(w, 0, sizeof(int), stream), "status clear")) return e;
-    rh3::set_error(v, "a bounded device wait gave up (status %d)", v);
+    if (v == rh3::ST_KV_BAD_PAGE) rh3::set_error(v, "a page table named a page outside its cache (status %d)", v);
+    else rh3::set_error(v, "a bounded device wait gave up (status %d)", v);
   }
   if (status_out) *status_out = v;
   return 0;

@@ -1,0 +1,315 @@
+// Writing rows into the quantized key/value cache and reading them back.
+//
+// A row is one token's D channels of one head. Written: s = max(amax / 127, 1e-12), code = rint(x / s) (int8), or
+// s = max(amax / 448, 1e-12), code = e4m3(clamp(x / s)) -- the arithmetic of the row quantizers (quant.cu), codes and scales bit for bit.
+// A row with a NaN or an infinity keeps it in its scale, its codes are 0: it reads back as NaN, and a masked one cannot reach
+// a product through its codes. Read: code * s in fp32, rounded once to the asked type.
+//
+// HBM-bound copies: write takes in 2 * D * esize and puts out 2 * (D + 4) bytes per (token, head), read the reverse. A lane
+// holds 8 channels (16-byte accesses on the bf16 side, 8 bytes on the code side), D / 8 lanes a row, and a warp issues the
+// loads of KV_ITER groups of rows before it reduces the first: where they lie (sequence, page) is looked up once per token and warp.
+#include "kv_cache.cuh"
+#include "rapidh3_b200.h"
+
+namespace rh3 {
+namespace {
+
+constexpr int KV_THREADS = 256;
+constexpr int KV_ITER = 4;
+
+enum { KV_BF16 = 0, KV_F16 = 1, KV_F32 = 2 };
+
+template <int DT>
+struct KvRaw {  // eight elements of a row as loaded
+  uint4 a, b;
+};
+template <int DT>
+__device__ __forceinline__ void kv_load8(const void* base, int64_t at, KvRaw<DT>& r) {
+  if constexpr (DT == KV_F32) {
+    r.a = ld_global_16(static_cast<const float*>(base) + at);
+    r.b = ld_global_16(static_cast<const float*>(base) + at + 4);
+  } else {
+    r.a = ld_global_16(static_cast<const uint16_t*>(base) + at);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void kv_unpack8(const KvRaw<DT>& r, float* x) {
+  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+  if constexpr (DT == KV_F32) {
+    const uint32_t u[4] = {r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(w[j]), x[4 + j] = __uint_as_float(u[j]);
+  } else if constexpr (DT == KV_F16) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+      x[2 * j] = f.x, x[2 * j + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[2 * j] = bf16_lo(w[j]), x[2 * j + 1] = bf16_hi(w[j]);
+  }
+}
+// keeps a NaN, which fmaxf drops
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+struct KvWriteParams {
+  KvCache c;
+  KvRows r;
+  const void* k;
+  const void* v;
+  int64_t k_st, k_sh, v_st, v_sh;  // token and head strides in elements
+  int warps_per_token;
+  int* status;
+};
+
+template <int D, int FMT, int DT>
+__global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const KvWriteParams p) {
+  constexpr int LANES = D / 8, ROWS = 32 / LANES;  // lanes per row, rows per pass of a warp
+  grid_dependency_begin();
+  const int lane = threadIdx.x & 31;
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * (KV_THREADS / 32) + (threadIdx.x >> 5);
+  const int64_t t = w / p.warps_per_token;
+  if (t >= p.r.T) return;
+  const int part = static_cast<int>(w - t * p.warps_per_token);
+  const int heads2 = 2 * p.c.heads, sub = lane / LANES, ch = (lane % LANES) * 8;
+  KvRaw<DT> raw[KV_ITER];
+  const int first = part * (KV_ITER * ROWS) + sub;  // rows 0 .. heads-1 of a token are its K heads, then its V heads
+#pragma unroll
+  for (int i = 0; i < KV_ITER; ++i) {
+    const int row = first + i * ROWS;
+    raw[i].a = raw[i].b = make_uint4(0, 0, 0, 0);
+    if (row < heads2) {
+      const bool is_v = row >= p.c.heads;
+      const int h = is_v ? row - p.c.heads : row;
+      kv_load8<DT>(is_v ? p.v : p.k, t * (is_v ? p.v_st : p.k_st) + h * (is_v ? p.v_sh : p.k_sh) + ch, raw[i]);
+    }
+  }
+  bool known;
+  const int64_t place = kv_place(p.c, p.r, static_cast<int>(t), lane, p.status, &known);
+  if (place < 0) return;
+#pragma unroll
+  for (int i = 0; i < KV_ITER; ++i) {
+    const int row = first + i * ROWS;
+    float x[8];
+    kv_unpack8<DT>(raw[i], x);
+    float amax = fabsf(x[0]);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) amax = max_nan(amax, fabsf(x[j]));
+#pragma unroll
+    for (int o = LANES / 2; o; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    float s = __fdiv_rn(amax, FMT == RH3_KIND_I8 ? 127.f : 448.f);
+    if (s < 1e-12f) s = 1e-12f;
+    uint2 q = make_uint2(0, 0);
+    if (s < INFINITY) {
+      const float inv = __fdiv_rn(1.f, s);
+      q = FMT == RH3_KIND_I8 ? quant8_i8(x, s, inv) : quant8_e4m3(x, s, inv);
+    }
+    if (row < heads2) {
+      const bool is_v = row >= p.c.heads;
+      const int h = is_v ? row - p.c.heads : row;
+      const int64_t at = place + (static_cast<int64_t>(h) << p.c.page_log2);
+      *reinterpret_cast<uint2*>((is_v ? p.c.v : p.c.k) + at * D + ch) = q;
+      if (ch == 0) (is_v ? p.c.vs : p.c.ks)[at] = s;
+    }
+  }
+}
+
+struct KvReadParams {
+  KvCache c;
+  KvRows r;
+  void* k;
+  void* v;  // [T][heads][D], contiguous
+  int warps_per_token;
+  int* status;
+};
+
+template <int FMT>
+__device__ __forceinline__ void kv_decode8(uint2 q, float s, float* x) {
+  const uint32_t w[2] = {q.x, q.y};
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    if constexpr (FMT == RH3_KIND_I8) {
+      // the byte behind 2^23 is a float: 2^23 + (code + 128), exactly
+      const uint32_t u = w[j] ^ 0x80808080u;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        x[4 * j + b] = __fmul_rn(__fsub_rn(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 + b)), 8388736.f), s);
+    } else {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        uint32_t h2;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(w[j] >> (16 * b))));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+        x[4 * j + 2 * b] = __fmul_rn(f.x, s), x[4 * j + 2 * b + 1] = __fmul_rn(f.y, s);
+      }
+    }
+  }
+}
+
+template <int D, int FMT, int DT>
+__global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const KvReadParams p) {
+  constexpr int LANES = D / 8, ROWS = 32 / LANES;
+  grid_dependency_begin();
+  const int lane = threadIdx.x & 31;
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * (KV_THREADS / 32) + (threadIdx.x >> 5);
+  const int64_t t = w / p.warps_per_token;
+  if (t >= p.r.T) return;
+  const int part = static_cast<int>(w - t * p.warps_per_token);
+  const int heads2 = 2 * p.c.heads, sub = lane / LANES, ch = (lane % LANES) * 8;
+  bool known;
+  const int64_t place = kv_place(p.c, p.r, static_cast<int>(t), lane, p.status, &known);
+  if (!known) return;  // rows behind the last sequence stay as they are
+  const int first = part * (KV_ITER * ROWS) + sub;
+  uint2 q[KV_ITER];
+  float s[KV_ITER];
+#pragma unroll
+  for (int i = 0; i < KV_ITER; ++i) {
+    const int row = first + i * ROWS;
+    q[i] = make_uint2(0, 0);
+    s[i] = 0.f;
+    if (place >= 0 && row < heads2) {
+      const bool is_v = row >= p.c.heads;
+      const int64_t at = place + (static_cast<int64_t>(is_v ? row - p.c.heads : row) << p.c.page_log2);
+      q[i] = *reinterpret_cast<const uint2*>((is_v ? p.c.v : p.c.k) + at * D + ch);
+      s[i] = (is_v ? p.c.vs : p.c.ks)[at];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < KV_ITER; ++i) {
+    const int row = first + i * ROWS;
+    if (row >= heads2) continue;
+    float x[8];
+    kv_decode8<FMT>(q[i], s[i], x);
+    const bool is_v = row >= p.c.heads;
+    const int64_t at = (t * p.c.heads + (is_v ? row - p.c.heads : row)) * D + ch;
+    void* out = is_v ? p.v : p.k;
+    if constexpr (DT == KV_F32) {
+      float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
+      o[0] = make_float4(x[0], x[1], x[2], x[3]);
+      o[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+      uint32_t u[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (DT == KV_F16) {
+          const __half2 h = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
+          u[j] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          u[j] = pack_bf16x2(x[2 * j], x[2 * j + 1]);
+        }
+      }
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+  }
+}
+
+// calls fn(D, FMT, DT) as compile-time constants
+template <class F>
+int kv_dispatch(int64_t D, int fmt, int dt, F&& fn) {
+  auto by_type = [&](auto d, auto f) {
+    switch (dt) {
+      case KV_BF16: return fn(d, f, std::integral_constant<int, KV_BF16>());
+      case KV_F16: return fn(d, f, std::integral_constant<int, KV_F16>());
+      default: return fn(d, f, std::integral_constant<int, KV_F32>());
+    }
+  };
+  auto by_fmt = [&](auto d) {
+    return fmt == RH3_KIND_I8 ? by_type(d, std::integral_constant<int, RH3_KIND_I8>())
+                              : by_type(d, std::integral_constant<int, RH3_KIND_F8>());
+  };
+  return D == 64 ? by_fmt(std::integral_constant<int, 64>()) : by_fmt(std::integral_constant<int, 128>());
+}
+
+int kv_warps_per_token(int64_t heads, int64_t D) {
+  const int64_t rows = 32 / (D / 8) * KV_ITER;
+  return static_cast<int>((2 * heads + rows - 1) / rows);
+}
+
+}  // namespace
+
+int kv_fill_cache(KvCache* c, const char* what, const void* k, const void* v, const float* ks, const float* vs, int64_t pages,
+                  int64_t heads, int64_t page, int64_t D, int fmt) {
+  RH3_CHECK_ARG(fmt == RH3_KIND_I8 || fmt == RH3_KIND_F8, "%s: kind=%d must be 0 (int8) or 1 (e4m3)", what, fmt);
+  RH3_CHECK_ARG(D == 64 || D == 128, "%s: head size %lld must be 64 or 128", what, (long long)D);
+  RH3_CHECK_ARG(page == 16 || page == 32 || page == 64 || page == 128, "%s: pages of %lld tokens: must be 16, 32, 64 or 128", what,
+                (long long)page);
+  RH3_CHECK_ARG(heads > 0 && heads <= 1024 && pages > 0, "%s: bad cache shape: %lld pages, %lld heads", what, (long long)pages,
+                (long long)heads);
+  // TMA coordinates count rows of 128 bytes in 32 bits
+  RH3_CHECK_ARG(pages <= (1ll << 31) / (heads * page * D / 128) - 1, "%s: a cache of %lld pages is too large", what, (long long)pages);
+  RH3_CHECK_ARG(k && v && ks && vs && kv_a16(k) && kv_a16(v) && kv_a16(ks) && kv_a16(vs),
+                "%s: cache pointers must be set and 16-byte aligned", what);
+  c->k = static_cast<uint8_t*>(const_cast<void*>(k));
+  c->v = static_cast<uint8_t*>(const_cast<void*>(v));
+  c->ks = const_cast<float*>(ks);
+  c->vs = const_cast<float*>(vs);
+  c->pages = static_cast<int>(pages);
+  c->heads = static_cast<int>(heads);
+  c->page_log2 = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
+  return 0;
+}
+
+int kv_fill_rows(KvRows* r, const char* what, const int32_t* table, int64_t table_stride, int64_t per_seq, const int32_t* lens,
+                 const int32_t* starts, int64_t B, int64_t T) {
+  RH3_CHECK_ARG(B > 0 && B <= 65536 && per_seq >= 0 && per_seq < (1 << 24) && table_stride >= per_seq,
+                "%s: bad batch: %lld sequences, %lld pages each, stride %lld", what, (long long)B, (long long)per_seq,
+                (long long)table_stride);
+  RH3_CHECK_ARG(T >= 0 && T < (1 << 26), "%s: %lld rows: must be below 2^26", what, (long long)T);
+  RH3_CHECK_ARG((table || per_seq == 0) && lens && starts, "%s: null batch pointer", what);
+  *r = KvRows{table, lens, starts, table_stride, static_cast<int>(B), static_cast<int>(per_seq), static_cast<int>(T), 0};
+  return 0;
+}
+
+}  // namespace rh3
+
+using namespace rh3;
+
+extern "C" int rh3_kv_write(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, int dtype, void* kc,
+                            void* vc, float* ks, float* vs, int64_t pages, int64_t heads, int64_t page, int64_t D, int kind,
+                            const int32_t* table, int64_t table_stride, int64_t per_seq, const int32_t* lens, const int32_t* starts,
+                            int64_t B, int64_t T, cudaStream_t stream) {
+  KvWriteParams p{};
+  RH3_CHECK_ARG(dtype >= 0 && dtype <= 2, "kv_write: dtype=%d must be 0 (bf16), 1 (fp16) or 2 (fp32)", dtype);
+  if (int e = kv_fill_cache(&p.c, "kv_write", kc, vc, ks, vs, pages, heads, page, D, kind)) return e;
+  if (int e = kv_fill_rows(&p.r, "kv_write", table, table_stride, per_seq, lens, starts, B, T)) return e;
+  if (T == 0) return 0;
+  const int64_t per16 = dtype == KV_F32 ? 4 : 8;
+  RH3_CHECK_ARG(k && v && kv_a16(k) && kv_a16(v) && k_st % per16 == 0 && k_sh % per16 == 0 && v_st % per16 == 0 && v_sh % per16 == 0,
+                "kv_write: every row of k and v must start on a 16-byte boundary");
+  p.k = k, p.v = v, p.k_st = k_st, p.k_sh = k_sh, p.v_st = v_st, p.v_sh = v_sh;
+  p.warps_per_token = kv_warps_per_token(heads, D);
+  p.status = device_status_word();
+  const int64_t blocks = (T * p.warps_per_token + KV_THREADS / 32 - 1) / (KV_THREADS / 32);
+  RH3_CHECK_ARG(blocks < (1ll << 31), "kv_write: too many rows");
+  const bool chained = blocks <= 4 * device_sm_count() && !in_capture(stream);
+  return kv_dispatch(D, kind, dtype, [&](auto d, auto f, auto t) {
+    return check_cuda(launch_kernel(chained, kv_write_kernel<d(), f(), t()>, dim3(static_cast<unsigned>(blocks)), KV_THREADS, 0, stream, 1, p),
+                      "kv_write launch");
+  });
+}
+
+extern "C" int rh3_kv_read(const void* kc, const void* vc, const float* ks, const float* vs, int64_t pages, int64_t heads, int64_t page,
+                           int64_t D, int kind, const int32_t* table, int64_t table_stride, int64_t per_seq, const int32_t* lens,
+                           const int32_t* starts, int64_t B, int64_t T, void* k, void* v, int dtype, cudaStream_t stream) {
+  KvReadParams p{};
+  RH3_CHECK_ARG(dtype >= 0 && dtype <= 2, "kv_read: dtype=%d must be 0 (bf16), 1 (fp16) or 2 (fp32)", dtype);
+  if (int e = kv_fill_cache(&p.c, "kv_read", kc, vc, ks, vs, pages, heads, page, D, kind)) return e;
+  if (int e = kv_fill_rows(&p.r, "kv_read", table, table_stride, per_seq, lens, starts, B, T)) return e;
+  if (T == 0) return 0;
+  RH3_CHECK_ARG(k && v && kv_a16(k) && kv_a16(v), "kv_read: outputs must be set and 16-byte aligned");
+  p.k = k, p.v = v;
+  p.warps_per_token = kv_warps_per_token(heads, D);
+  p.status = device_status_word();
+  const int64_t blocks = (T * p.warps_per_token + KV_THREADS / 32 - 1) / (KV_THREADS / 32);
+  RH3_CHECK_ARG(blocks < (1ll << 31), "kv_read: too many rows");
+  const bool chained = blocks <= 4 * device_sm_count() && !in_capture(stream);
+  return kv_dispatch(D, kind, dtype, [&](auto d, auto f, auto t) {
+    return check_cuda(launch_kernel(chained, kv_read_kernel<d(), f(), t()>, dim3(static_cast<unsigned>(blocks)), KV_THREADS, 0, stream, 1, p),
+                      "kv_read launch");
+  });
+}

@@ -1,0 +1,207 @@
+// What the kernels of the quantized key/value cache share: the cache and batch descriptors, where a row of a call lies in
+// the cache, and how the work of a ragged batch is cut into equal pieces on the device.
+//
+// Cache: codes [pages][heads][page][D] (int8 or e4m3, one byte each), scales fp32 [pages][heads][page]; page is a power of
+// two of 16 .. 128 tokens, so a head's part of a page is one contiguous run that a single TMA box takes.
+// Batch: table int32 [B][table_stride] (the pages of each sequence in order), lens int32 [B] (cached tokens, the call's own
+// among them), starts int32 [B + 1]: rows starts[b] .. starts[b + 1] - 1 of the call are the last tokens of sequence b.
+// All three live on the device and are read there: a captured call follows them when it is replayed. Values that make no
+// sense (a page that does not exist, a length beyond the table, rows beyond the call's) are cut to what exists, never
+// followed; a missing page's tokens count as masked, and ST_KV_BAD_PAGE is left in the status word.
+#pragma once
+#include "common.cuh"
+
+namespace rh3 {
+
+struct KvCache {
+  uint8_t* k;
+  uint8_t* v;
+  float* ks;
+  float* vs;
+  int pages, heads, page_log2;
+};
+struct KvRows {
+  const int* table;
+  const int* lens;
+  const int* starts;
+  int64_t table_stride;
+  int B, per_seq;  // sequences; pages per row of the table
+  int T;           // rows of the call
+  int fixed_len;   // > 0: one sequence of this many tokens whose rows are all of the call's (a shared prefix; lens and starts are not read)
+};
+
+__device__ __forceinline__ void kv_report(int* status, int code) {
+  if (status) atomicCAS(status, 0, code);
+}
+
+// How many of ends[0 .. n) (ascending) are <= t: a 32-way search by a whole warp, one load per lane and round (one round
+// up to 32 sequences, two up to 1,024).
+__device__ __forceinline__ int kv_count_ends(const int* ends, int n, int t, int lane) {
+  int lo = 0;
+  while (n > 0) {
+    const int step = (n + 31) >> 5;
+    const int first = lane * step;
+    const bool have = first < n;
+    const int at = lo + min(n, first + step) - 1;
+    const bool below = have && ends[at] <= t;
+    const int c = __popc(__ballot_sync(0xffffffffu, below));   // chunks that lie wholly at or below t
+    const int skip = min(n, c * step);
+    const int left = min(step, n - skip);
+    lo += skip;
+    n = left > 0 ? left - 1 : 0;                               // the chunk's last element is known to be above t
+  }
+  return lo;
+}
+
+// Where row t of the call lies (whole warp, t uniform): pages of the cache are checked against its size.
+__device__ __forceinline__ int64_t kv_place(const KvCache& c, const KvRows& r, int t, int lane, int* status, bool* known) {
+  const int b = kv_count_ends(r.starts + 1, r.B, t, lane);
+  *known = b < r.B && t >= r.starts[b];
+  if (!*known) return -1;
+  const int64_t pos = static_cast<int64_t>(r.lens[b]) - (static_cast<int64_t>(r.starts[b + 1]) - t);
+  const int64_t pi = pos >> c.page_log2;
+  if (pos < 0 || pi >= r.per_seq) return -1;
+  const int id = r.table[b * r.table_stride + pi];
+  if (id < 0 || id >= c.pages) {
+    if (lane == 0) kv_report(status, ST_KV_BAD_PAGE);
+    return -1;
+  }
+  return ((static_cast<int64_t>(id) * c.heads) << c.page_log2) + (pos & ((1 << c.page_log2) - 1));
+}
+
+// ---------------------------------------------------------------------------------------------
+// cutting a ragged batch into equal pieces
+// ---------------------------------------------------------------------------------------------
+// The rows of a sequence are its new tokens x the query heads of one KV head ("group"): row = token * group + head. A unit is
+// BM such rows of one sequence and KV head against all of its keys, in tiles of TK keys; every unit has at least one tile, so that rows
+// without a key are written too. The tiles of all units, in the order (sequence, head, row tile, key tile), are dealt to the CTAs
+// in equal runs [W * c / G, W * (c + 1) / G): a CTA's run begins and ends anywhere inside a unit.
+struct KvSeq {
+  int first, n, len;  // first row token of the call, new tokens, cached tokens
+  int qt, kt;         // row tiles, key tiles of a unit
+  __device__ __forceinline__ long long tiles(int heads) const { return static_cast<long long>(heads) * qt * kt; }
+};
+template <int BM, int TK>
+__device__ __forceinline__ KvSeq kv_seq(const KvRows& r, int page_log2, int group, int b) {
+  KvSeq s;
+  const int lo = r.fixed_len ? 0 : min(max(r.starts[b], 0), r.T), hi = r.fixed_len ? r.T : min(max(r.starts[b + 1], lo), r.T);
+  s.first = lo;
+  s.n = hi - lo;
+  const long long room = static_cast<long long>(r.per_seq) << page_log2;
+  s.len = static_cast<int>(min(static_cast<long long>(r.fixed_len ? r.fixed_len : max(r.lens[b], 0)), room));
+  s.qt = static_cast<int>((static_cast<long long>(s.n) * group + BM - 1) / BM);
+  s.kt = max(1, (s.len - 1 + TK) / TK);
+  return s;
+}
+// What a CTA needs to begin: its run and the sequence it begins in. Filled by the whole block (a scan over the sequences).
+struct KvRun {
+  long long x0, x1;   // the CTA's tiles
+  long long xb;       // first tile of sequence b
+  long long W;
+  int b, G;           // sequence that x0 lies in; CTAs that have a run
+};
+template <int BM, int TK, int NT>
+__device__ __forceinline__ void kv_find_run(const KvRows& r, int page_log2, int heads, int group, long long* scan /* NT/32 */,
+                                            KvRun* run) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (r.B + NT - 1) / NT;
+  const int b0 = min(r.B, tid * per), b1 = min(r.B, b0 + per);
+  long long own = 0;
+  for (int b = b0; b < b1; ++b) own += kv_seq<BM, TK>(r, page_log2, group, b).tiles(heads);
+  long long incl = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 31) scan[warp] = incl;
+  __syncthreads();
+  long long before = 0, W = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 32; ++i) {
+    if (i < warp) before += scan[i];
+    W += scan[i];
+  }
+  incl += before;
+  const long long excl = incl - own;
+  const int G = static_cast<int>(min(static_cast<long long>(gridDim.x), W));
+  const long long c = blockIdx.x;
+  const long long x0 = c < G ? W * c / G : W, x1 = c < G ? W * (c + 1) / G : W;
+  if (tid == 0) {
+    run->x0 = x0, run->x1 = x1, run->W = W, run->G = G;
+    run->b = r.B, run->xb = W;
+  }
+  __syncthreads();
+  if (x0 < x1 && excl <= x0 && x0 < incl) {
+    long long xb = excl;
+    int b = b0;
+    for (; b < b1; ++b) {
+      const long long w = kv_seq<BM, TK>(r, page_log2, group, b).tiles(heads);
+      if (x0 < xb + w) break;
+      xb += w;
+    }
+    run->b = b, run->xb = xb;
+  }
+  __syncthreads();
+}
+// One unit's part of a CTA's run
+struct KvSegment {
+  KvSeq s;
+  int b, h, u;        // sequence, KV head, row tile
+  int k0, k1;         // key tiles [k0, k1) of the unit's s.kt
+};
+// Steps through a run; next() gives the segment at x and moves on.
+template <int BM, int TK>
+struct KvWalk {
+  long long x, x1, xb;
+  int b;
+  KvSeq s;
+  bool have;
+  __device__ __forceinline__ KvWalk(const KvRun& run) : x(run.x0), x1(run.x1), xb(run.xb), b(run.b), have(false) {}
+  __device__ __forceinline__ bool next(const KvRows& r, int page_log2, int heads, int group, KvSegment& g) {
+    if (x >= x1) return false;
+    if (!have) s = kv_seq<BM, TK>(r, page_log2, group, b), have = true;
+    while (x >= xb + s.tiles(heads)) {  // ends: the tiles of the sequences from b on reach beyond x < x1 <= W
+      if (b + 1 >= r.B) return false;
+      xb += s.tiles(heads);
+      s = kv_seq<BM, TK>(r, page_log2, group, ++b);
+    }
+    const long long rem = x - xb;
+    const long long unit = rem / s.kt;
+    g.s = s, g.b = b;
+    g.k0 = static_cast<int>(rem - unit * s.kt);
+    g.h = static_cast<int>(unit / s.qt);
+    g.u = static_cast<int>(unit - static_cast<long long>(g.h) * s.qt);
+    g.k1 = static_cast<int>(min(static_cast<long long>(s.kt), g.k0 + (x1 - x)));
+    x += g.k1 - g.k0;
+    return true;
+  }
+};
+// Keys that some row of row tile u sees: the last row's position + 1 (causal) or all of them.
+template <int BM>
+__device__ __forceinline__ int kv_visible(const KvSeq& s, int group, int u, bool causal) {
+  if (!causal) return s.len;
+  const int last = static_cast<int>((min(static_cast<long long>(u + 1) * BM, static_cast<long long>(s.n) * group) - 1) / group);
+  return max(0, min(s.len, s.len - s.n + last + 1));
+}
+
+// ---------------------------------------------------------------------------------------------
+// TMA without a tensor map: a contiguous run of 16-byte units
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem_dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// ---------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------
+inline bool kv_a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// the arguments every entry takes; 0 or an argument error. `what` names the entry.
+int kv_fill_cache(KvCache* c, const char* what, const void* k, const void* v, const float* ks, const float* vs, int64_t pages,
+                  int64_t heads, int64_t page, int64_t D, int fmt);
+int kv_fill_rows(KvRows* r, const char* what, const int32_t* table, int64_t table_stride, int64_t per_seq, const int32_t* lens,
+                 const int32_t* starts, int64_t B, int64_t T);
+
+}  // namespace rh3

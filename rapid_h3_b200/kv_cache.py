@@ -1,0 +1,209 @@
+"""Quantized key/value cache for the attention of a language model (the text encoder's: grouped heads), and attention to it.
+
+Keys and values are stored per token and KV head as 8-bit codes with one fp32 scale, in the arithmetic of the row quantizers
+(`quantizers.quant_rows_i8` / `quant_rows`), in pages that sequences of any length share out among themselves:
+
+    cache = kv_cache.alloc(pages=512, kv_heads=8, head_dim=128, page=64, kind="int8")
+    rows = kv_cache.Rows(table, lens, starts)             # which rows of a call belong to which sequence, see Rows
+    kv_cache.write(cache, k, v, rows)                     # quantize new tokens into their pages
+    out = kv_cache.attention(q, cache, rows)              # their attention to everything their sequences hold
+    out = kv_cache.attention_shared(q, cache, rows, prefix, n)   # behind one prefix that all sequences share
+    k, v = kv_cache.read(cache, rows, total)              # back as bf16 rows
+
+`lens`, `starts` and the page table stay on the device and are read there, so a captured call follows them. The tensors of a call are on
+the cache's device, and the work goes to that device's current stream. Everything is CUDA; there is no fallback.
+"""
+import struct
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+
+FP8 = torch.float8_e4m3fn
+PAGES = (16, 32, 64, 128)
+HEAD_DIMS = (64, 128)
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_KINDS = {"int8": (torch.int8, 0), "fp8": (FP8, 1)}
+
+# rh3_kv_attn_args: q, out, the cache and the batch (pointers, strides, sizes), then scale, kind, dtype, causal
+_ARGS = struct.Struct("@PqqPqqPPPPqqqqPqqPPqqqPqqfiii")
+
+
+class KVCache:
+    """Codes k, v [pages, kv_heads, page, head_dim] (int8, or float8_e4m3fn) and scales k_scale, v_scale fp32 [pages, kv_heads, page],
+    contiguous, on one CUDA device. page: 16, 32, 64 or 128 tokens; head_dim: 64 or 128."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page", "head_dim", "kind", "device", "_args")
+
+    def __init__(self, k, v, k_scale, v_scale):
+        _lib.require_cuda(k, v, k_scale, v_scale)
+        if k.ndim != 4 or k.dtype not in (torch.int8, FP8):
+            raise RuntimeError(f"k: expected int8 or e4m3 codes [pages, kv_heads, page, head_dim], got {tuple(k.shape)} {k.dtype}")
+        if v.shape != k.shape or v.dtype != k.dtype:
+            raise RuntimeError("v must have the shape and type of k")
+        self.pages, self.kv_heads, self.page, self.head_dim = k.shape
+        if self.page not in PAGES or self.head_dim not in HEAD_DIMS or self.pages < 1 or not 1 <= self.kv_heads <= 1024:
+            raise RuntimeError(f"page must be one of {PAGES}, head_dim one of {HEAD_DIMS}: got a cache of {tuple(k.shape)}")
+        for t in (k_scale, v_scale):
+            if t.dtype != torch.float32 or t.shape != k.shape[:3]:
+                raise RuntimeError("scales must be fp32 [pages, kv_heads, page]")
+        for t in (k, v, k_scale, v_scale):
+            if not t.is_contiguous() or t.data_ptr() % 16 or t.device != k.device:
+                raise RuntimeError("the cache's tensors must be contiguous, 16-byte aligned and on one device")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device = k.device
+        self.kind = 0 if k.dtype == torch.int8 else 1
+        self._args = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.pages, self.kv_heads, self.page, self.head_dim)
+
+
+def alloc(pages, kv_heads, head_dim=128, page=64, kind="int8", device="cuda"):
+    """An empty cache of `pages` pages of `page` tokens; kind "int8" or "fp8" (e4m3)."""
+    if kind not in _KINDS:
+        raise RuntimeError(f"kind must be one of {tuple(_KINDS)}, got {kind!r}")
+    shape = (pages, kv_heads, page, head_dim)
+    k, v = (torch.zeros(shape, device=device, dtype=_KINDS[kind][0]) for _ in range(2))
+    return KVCache(k, v, *(torch.zeros(shape[:3], device=device, dtype=torch.float32) for _ in range(2)))
+
+
+@dataclass(frozen=True)
+class Rows:
+    """Which rows of a call belong to which sequence, int32 on the cache's device:
+    table [B, P] the pages of each sequence in order (rows may be strided); lens [B] the tokens each sequence holds, the call's own
+    among them; starts [B + 1], ascending: rows starts[b] .. starts[b + 1] - 1 of the call are the last tokens of sequence b.
+
+    The values are not looked at on the host. Rows at or behind starts[B] (a padded batch) are left as they were; tokens that lie
+    nowhere (before position 0, beyond the table, in a page the cache does not have) are not written, read as zeros and are
+    masked, and a page the cache does not have is reported by `_lib.check_status()`."""
+    table: torch.Tensor
+    lens: torch.Tensor
+    starts: torch.Tensor
+
+    def __post_init__(self):
+        table, lens, starts = self.table, self.lens, self.starts
+        _lib.require_cuda(table, lens, starts)
+        if not table.dtype == lens.dtype == starts.dtype == torch.int32:
+            raise RuntimeError("table, lens and starts must be int32")
+        if table.ndim != 2 or lens.ndim != 1 or starts.ndim != 1 or len(lens) != len(table) or len(starts) != len(lens) + 1 or len(lens) == 0:
+            raise RuntimeError(f"expected table [B, P], lens [B], starts [B + 1] with B > 0, got {tuple(table.shape)}, {tuple(lens.shape)}, {tuple(starts.shape)}")
+        if not (lens.is_contiguous() and starts.is_contiguous()) or (table.shape[1] > 1 and table.stride(1) != 1):
+            raise RuntimeError("lens, starts and the rows of table must be contiguous")
+        if (table.shape[0] > 1 and table.stride(0) < table.shape[1]) or not table.device == lens.device == starts.device:
+            raise RuntimeError("the rows of table must not overlap, and all three must be on one device")
+        object.__setattr__(self, "_args", (table.data_ptr(), max(table.stride(0), table.shape[1]), table.shape[1], lens.data_ptr(),
+                                           starts.data_ptr(), len(lens)))
+
+
+class _on:
+    """The device a call's work goes to; entering it costs nothing where it is the current one."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, device):
+        self.guard = None if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _check_batch(cache, rows):
+    if rows.table.device != cache.device:
+        raise RuntimeError("the batch must be on the cache's device")
+
+
+def _check_rows(x, name, cache, heads, types):
+    if not x.is_cuda or x.device != cache.device:
+        raise RuntimeError(f"{name} must be a CUDA tensor on the cache's device; there is no CPU path")
+    if x.ndim != 3 or x.dtype not in types or x.shape[2] != cache.head_dim or (heads is not None and x.shape[1] != heads):
+        raise RuntimeError(f"{name}: expected [T, {heads or 'heads'}, {cache.head_dim}] of {', '.join(str(t) for t in types)}, got {tuple(x.shape)} {x.dtype}")
+    per16 = 16 // x.element_size()
+    if x.numel() and (x.stride(2) != 1 or x.stride(0) % per16 or x.stride(1) % per16 or x.data_ptr() % 16):
+        raise RuntimeError(f"{name}: the last dim must be contiguous and every row start on a 16-byte boundary")
+
+
+def write(cache, k, v, rows):
+    """Quantize k, v [T, kv_heads, head_dim] (bf16, fp16 or fp32, any token and head strides of whole 16 bytes) into the pages of
+    their sequences. A row with a NaN or an infinity reads back as NaN. Sequences that share a page must not write the same token."""
+    _check_batch(cache, rows)
+    _check_rows(k, "k", cache, cache.kv_heads, tuple(_DTYPES))
+    _check_rows(v, "v", cache, cache.kv_heads, (k.dtype,))
+    if v.shape != k.shape:
+        raise RuntimeError("k and v must have the same number of rows")
+    with _on(cache.device):
+        _lib.call("rh3_kv_write", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _DTYPES[k.dtype],
+                  *cache._args, cache.kind, *rows._args, k.shape[0], _lib.stream())
+
+
+def read(cache, rows, total, dtype=torch.bfloat16, out=None):
+    """(k, v) [total, kv_heads, head_dim] of `dtype`: codes x scales of the tokens `rows` names, rounded once. Rows that no sequence
+    has hold what `out` (a pair of contiguous tensors) held, or anything."""
+    _check_batch(cache, rows)
+    if dtype not in _DTYPES:
+        raise RuntimeError(f"dtype must be one of {tuple(_DTYPES)}, got {dtype}")
+    shape = (total, cache.kv_heads, cache.head_dim)
+    if out is None:
+        k, v = torch.empty((2, *shape), device=cache.device, dtype=dtype).unbind(0)
+    else:
+        k, v = out
+        for t in (k, v):
+            if t.shape != shape or t.dtype != dtype or t.device != cache.device or not t.is_contiguous() or t.data_ptr() % 16:
+                raise RuntimeError(f"out: expected two contiguous, 16-byte aligned {dtype} tensors {shape} on the cache's device")
+    with _on(cache.device):
+        _lib.call("rh3_kv_read", *cache._args, cache.kind, *rows._args, total, k.data_ptr(), v.data_ptr(), _DTYPES[dtype], _lib.stream())
+    return k, v
+
+
+def _attend(q, cache, rows, prefix, prefix_len, scale, causal, out):
+    _check_batch(cache, rows)
+    _check_rows(q, "q", cache, None, (torch.bfloat16, torch.float16))
+    t, heads, d = q.shape
+    if heads == 0 or heads % cache.kv_heads:
+        raise RuntimeError(f"{heads} query heads are not a multiple of the cache's {cache.kv_heads}")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0 < scale < float("inf"):
+        raise RuntimeError("the softmax scale must be positive and finite")
+    if out is None:
+        out = torch.empty((t, heads, d), device=q.device, dtype=q.dtype)
+    else:
+        _check_rows(out, "out", cache, heads, (q.dtype,))
+        if out.shape != q.shape:
+            raise RuntimeError("out must have the shape of q")
+    if t == 0:
+        return out
+    group = heads // cache.kv_heads
+    table, stride, per_seq, lens, starts, batch = rows._args
+    with _on(cache.device):
+        need = _lib.lib().rh3_kv_attn_workspace_bytes(cache.kv_heads, group, cache.page, d, per_seq, batch, t, prefix_len)
+        work = torch.empty(need, device=q.device, dtype=torch.uint8)
+        args = _ARGS.pack(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), *cache._args, table, stride,
+                          per_seq, lens, starts, batch, t, group, prefix.data_ptr() if prefix is not None else 0,
+                          prefix.numel() if prefix is not None else 0, prefix_len, scale, cache.kind, _DTYPES[q.dtype], bool(causal))
+        _lib.call("rh3_kv_attn", args, work.data_ptr(), need, _lib.stream())
+    return out
+
+
+def attention(q, cache, rows, scale=None, causal=True, out=None):
+    """softmax(scale * q . k) v of new tokens q [T, heads, head_dim] (bf16 or fp16) over what their sequences hold in the cache.
+
+    heads: a multiple of the cache's kv_heads (head h reads KV head h // group). causal: a token sees the tokens up to itself (the
+    last one of its sequence sees all), else every token sees all of its sequence. A token that sees nothing gives 0. The call's own
+    tokens are among what is seen: write them first. scale: 1 / sqrt(head_dim) unless given; out: a tensor like q to write to."""
+    return _attend(q, cache, rows, None, 0, scale, causal, out)
+
+
+def attention_shared(q, cache, rows, prefix, prefix_len, scale=None, causal=True, out=None):
+    """`attention` of a batch whose sequences all continue one cached prefix: its first `prefix_len` tokens lie in the pages `prefix`
+    (int32, on the cache's device) and are seen by every token. `rows` describes the own parts alone (a length of 0 is a sequence
+    that has nothing of its own). The prefix is read and multiplied once for the whole batch."""
+    _lib.require_cuda(prefix)
+    if prefix.dtype != torch.int32 or prefix.ndim != 1 or not prefix.is_contiguous() or prefix.device != cache.device:
+        raise RuntimeError("prefix must be contiguous int32 [pages] on the cache's device")
+    prefix_len = int(prefix_len)
+    if not 0 <= prefix_len <= prefix.numel() * cache.page:
+        raise RuntimeError(f"a prefix of {prefix_len} tokens does not fit {prefix.numel()} pages of {cache.page}")
+    return _attend(q, cache, rows, prefix, prefix_len, scale, causal, out)

@@ -1,0 +1,125 @@
+"""Refusals of the cache operators that need no GPU, the descriptors' checks, and the arithmetic that deals tiles to CTAs."""
+import bisect
+import random
+
+import pytest
+import torch
+
+from rapid_h3_b200 import _lib, kv_cache
+
+P = 4096  # an address that is never touched: the argument checks come first
+
+
+def write_args(**kw):
+    a = dict(k=P, k_st=1024, k_sh=128, v=P, v_st=1024, v_sh=128, dtype=0, kc=P, vc=P, ks=P, vs=P, pages=8, heads=8, page=64, D=128, kind=0, table=P,
+             table_stride=4, per_seq=4, lens=P, starts=P, B=2, T=3, stream=None)
+    a.update(kw)
+    return list(a.values())
+
+
+def read_args(**kw):
+    a = dict(kc=P, vc=P, ks=P, vs=P, pages=8, heads=8, page=64, D=128, kind=0, table=P, table_stride=4, per_seq=4, lens=P, starts=P, B=2, T=3,
+             k=P, v=P, dtype=0, stream=None)
+    a.update(kw)
+    return list(a.values())
+
+
+def attn_args(**kw):
+    a = dict(q=P, q_st=1024, q_sh=128, out=P, o_st=1024, o_sh=128, k=P, v=P, ks=P, vs=P, pages=8, heads=2, page=64, D=128, table=P, table_stride=4,
+             per_seq=4, lens=P, starts=P, B=2, T=3, group=4, prefix_table=0, prefix_pages=0, prefix=0, scale=0.1, kind=0, dtype=0, causal=1)
+    a.update(kw)
+    return kv_cache._ARGS.pack(*a.values())
+
+
+CACHE = [(dict(kind=2), b"kind"), (dict(kind=-1), b"kind"), (dict(D=96), b"head size"), (dict(page=8), b"16, 32, 64 or 128"), (dict(page=48), b"16, 32, 64 or 128"),
+         (dict(pages=0), b"bad cache shape"), (dict(heads=0), b"bad cache shape"), (dict(heads=2000), b"bad cache shape"), (dict(pages=1 << 40), b"too large"),
+         (dict(ks=P + 4), b"aligned"), (dict(vs=0), b"must be set")]
+BATCH = [(dict(B=0), b"bad batch"), (dict(B=1 << 20), b"bad batch"), (dict(per_seq=-1), b"bad batch"), (dict(table_stride=3), b"bad batch"),
+         (dict(T=-1), b"rows"), (dict(T=1 << 30), b"rows"), (dict(lens=0), b"null"), (dict(starts=0), b"null"), (dict(table=0), b"null")]
+
+
+@pytest.mark.parametrize("change,said", CACHE + BATCH + [(dict(dtype=3), b"dtype"), (dict(k=P + 2), b"16-byte"), (dict(v_sh=100), b"16-byte"), (dict(k_st=1), b"16-byte")])
+def test_write_refuses(change, said):
+    assert _lib.lib().rh3_kv_write(*write_args(**change)) < 0 and said in _lib.lib().rh3_last_error_string()
+
+
+@pytest.mark.parametrize("change,said", CACHE + BATCH + [(dict(dtype=-1), b"dtype"), (dict(k=P + 8), b"aligned"), (dict(v=0), b"must be set")])
+def test_read_refuses(change, said):
+    assert _lib.lib().rh3_kv_read(*read_args(**change)) < 0 and said in _lib.lib().rh3_last_error_string()
+
+
+@pytest.mark.parametrize("change,said", CACHE + BATCH + [
+    (dict(dtype=2), b"dtype"), (dict(group=0), b"per KV head"), (dict(group=1 << 20), b"per KV head"), (dict(scale=0.0), b"scale"), (dict(scale=float("nan")), b"scale"),
+    (dict(scale=float("inf")), b"scale"), (dict(prefix=1), b"prefix"), (dict(prefix=65, prefix_pages=1, prefix_table=P), b"prefix"), (dict(prefix=-1), b"prefix"),
+    (dict(q=0), b"16-byte"), (dict(q_st=4), b"16-byte"), (dict(o_sh=129), b"16-byte"), (dict(out=P + 2), b"16-byte"), (dict(), b"workspace")])
+def test_attention_refuses(change, said):
+    lib = _lib.lib()
+    assert lib.rh3_kv_attn(attn_args(**change), None, 0, None) < 0 and said in lib.rh3_last_error_string()
+    if not change:
+        need = lib.rh3_kv_attn_workspace_bytes(2, 4, 64, 128, 4, 2, 3, 0)
+        assert need > 0
+        assert lib.rh3_kv_attn(attn_args(), P, need - 1, None) < 0 and said in lib.rh3_last_error_string()
+        assert lib.rh3_kv_attn(attn_args(), P + 16, need, None) < 0 and said in lib.rh3_last_error_string()
+        assert lib.rh3_kv_attn(None, P, need, None) < 0
+
+
+def test_calls_without_rows_do_nothing():
+    lib = _lib.lib()
+    assert lib.rh3_kv_write(*write_args(T=0, k=0, v=0)) == 0 and lib.rh3_kv_read(*read_args(T=0, k=0, v=0)) == 0
+    assert lib.rh3_kv_attn(attn_args(T=0, q=0, out=0), None, 0, None) == 0
+
+
+def test_there_is_no_cpu_path():
+    codes, scales = torch.zeros(2, 1, 16, 64, dtype=torch.int8), torch.zeros(2, 1, 16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        kv_cache.KVCache(codes, codes, scales, scales)
+    i = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        kv_cache.Rows(i[None], i, torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="kind"):
+        kv_cache.alloc(1, 1, kind="int4", device="cpu")
+
+
+def owner(x, w, g):
+    return ((x + 1) * g - 1) // w
+
+
+def test_every_tile_has_one_owner_and_every_cut_unit_is_joined_once():
+    """The device's arithmetic (runs, slots, records, the join's walk), restated: units of any sizes dealt to any grid."""
+    rng = random.Random(1)
+    for _ in range(400):
+        units = [rng.choice([1, 1, 2, 5, rng.randint(1, 300)]) for _ in range(rng.randint(1, 60))]
+        grid = rng.choice([1, 2, 7, 296, rng.randint(1, 400)])
+        w = sum(units)
+        g = min(grid, w)
+        first = [sum(units[:i]) for i in range(len(units))]
+        slots, record, whole = {}, {}, set()
+        for c in range(g):
+            x, x1 = w * c // g, w * (c + 1) // g
+            assert x < x1
+            begins = True
+            while x < x1:
+                u = bisect.bisect_right(first, x) - 1
+                k0 = x - first[u]
+                k1 = min(units[u], k0 + x1 - x)
+                assert owner(x, w, g) == c
+                if begins:
+                    record[c], begins = (u if k0 else -1, k0), False
+                if k0 == 0 and k1 == units[u]:
+                    whole.add(u)
+                else:
+                    assert (c, k0 == 0) not in slots
+                    slots[c, k0 == 0] = u, k0, k1
+                x += k1 - k0
+        joined = set()
+        for c in range(1, g):
+            u, k0 = record[c]
+            xs = w * c // g - k0
+            if u < 0 or w * (c - 1) // g > xs:
+                continue
+            n = owner(xs + units[u] - 1, w, g) - c + 2
+            parts = [slots[c - 1, True]] + [slots[c + i, False] for i in range(n - 1)]
+            assert all(p[0] == u for p in parts) and parts[0][1] == 0 and parts[-1][2] == units[u]
+            assert all(a[2] == b[1] for a, b in zip(parts, parts[1:])) and u not in joined
+            joined.add(u)
+        assert joined | whole == set(range(len(units))) and not joined & whole
