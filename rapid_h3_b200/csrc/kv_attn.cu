@@ -1,15 +1,21 @@
 // Attention of few rows per sequence (decoding, short continuations) to the quantized paged cache.
 //
-// A unit is 16 rows (new tokens x query heads of one KV head) of one sequence against all of its keys. What bounds it is reading the
-// cache once: 2 * (D + 4) bytes per key and head. The key tiles of all units are dealt to the CTAs in equal runs (kv_cache.cuh), two CTAs per
-// SM, so ragged batches, single sequences and many heads all spread over the chip; a unit cut by a run's end leaves partial results
-// that a second small kernel joins in a fixed order.
+// A unit is BM = 8 or 16 rows (new tokens x query heads of one KV head) of one sequence against all of its keys. What bounds it is
+// reading the cache once: 2 * (D + 4) bytes per key and head. The key tiles of all units are dealt to the CTAs in equal runs
+// (kv_cache.cuh), so ragged batches, single sequences and many heads all spread over the chip; a unit cut by a run's end leaves
+// partial results that a second small kernel joins in a fixed order.
 //
 // One CTA = a producer warp and four warps that compute, each on 32 of a tile's 128 keys with its own running maximum, sums and
 // output, joined at the unit's end: no barrier among them per tile. The producer brings pages by TMA into a ring
-// (128-byte swizzle over the codes as they lie, so that the byte accesses below hit 32 banks), their scales by bulk copies.
-// Products are mma.sync m16n8k16 on fp16: 16 rows are all there is, a 128-row tensor-core tile would be seven-eighths empty,
-// and the conversion of the codes (5 instructions per 4 codes) costs more than the products.
+// (128-byte swizzle over the codes as they lie, so that the accesses below hit 32 banks), their scales by bulk copies.
+//
+// Products are mma.sync m16n8k16 on fp16 with the KEYS (and then the channels) as the 16 rows and the query rows as the 8 columns:
+//     S^T = K . Q^T,   O^T = V^T . W^T
+// so that 8 query rows fill an instruction (a 128-row tensor-core tile would be nearly empty), half of the softmax values, output registers and
+// products that 16 rows take. W^T comes from S^T by movmatrix. What is left is mostly the conversion of the codes, 3 to 6
+// instructions for four of them. K codes enter as code + 128 in the low bits of an fp16 (a subnormal number, (code + 128) * 2^-24,
+// exact): the accumulators begin at -128 * 2^-24 * sum q, the same for every key of a row. V codes are brought to fp16 proper: there the
+// offset would be summed over all keys.
 // The order of channels and keys inside an mma is free, so each lane takes the channels and keys whose bytes it can load
 // 16 at a time: channel order (K) 16c .. 16c+15 of lane c, key order n -> (n >> 1) | ((n & 1) << 2), output channels of
 // lane group g 16g' .. 16g'+15.
@@ -24,29 +30,49 @@ constexpr int KV_WARPS = 4;             // computing warps
 constexpr int KV_NT = KV_WARPS * 32 + 32;
 enum { MODE_PLAIN = 0, MODE_PREFIX = 1, MODE_OWN = 2 };
 
-template <int D>
+template <int D, int NT>
 struct KvNarrow {
-  static constexpr int STAGES = D == 128 ? 3 : 5;
+  static constexpr int BM = 8 * NT;
+  static constexpr int CTAS = NT == 1 ? 3 : 2;                    // per SM
+  static constexpr int STAGES = (D == 128 ? 1 : 2) * (NT == 1 ? 2 : 3);
   static constexpr int STAGE_BYTES = 2 * TK * D;
   static constexpr int SCALES = STAGES * STAGE_BYTES;             // [STAGES][2][TK] floats
-  static constexpr int MERGE = SCALES + STAGES * 2 * TK * 4;      // [D / 8][32] float4
-  static constexpr int TAIL = MERGE + KV_BM * D * 4;
+  static constexpr int MERGE = SCALES + STAGES * 2 * TK * 4;      // [NT][D / 16][32] float4
+  static constexpr int TAIL = MERGE + BM * D * 4;
+  static constexpr int PART = BM * D + 2 * BM;                    // floats of a partial result
 };
 struct __align__(8) KvTail {
-  uint64_t full[5], empty[5];
-  float ml[KV_WARPS][KV_BM][2];
+  uint64_t full[6], empty[6];
+  float ml[KV_WARPS][16][2];
   long long scan[KV_NT / 32];
   KvRun run;
-  uint32_t pages[5];   // which of a stage's pages were there
+  uint32_t pages[6];   // which of a stage's pages were there
   int abort_flag;
 };
-template <int D>
-constexpr int kv_narrow_smem() { return KvNarrow<D>::TAIL + static_cast<int>(sizeof(KvTail)) + 1024; }
+template <int D, int NT>
+constexpr int kv_narrow_smem() { return KvNarrow<D, NT>::TAIL + static_cast<int>(sizeof(KvTail)) + 1024; }
 
 __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// an 8 x 8 matrix of fp16, one row's pair per lane, transposed
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// Four K codes of a word as fp16 pairs: int8 as (code + 128) * 2^-24, e4m3 as they are.
+template <int FMT>
+__device__ __forceinline__ void k_codes_to_half(uint32_t w, uint32_t& a, uint32_t& b) {
+  if constexpr (FMT == RH3_KIND_I8) {
+    const uint32_t u = w ^ 0x80808080u;
+    a = __byte_perm(u, 0, 0x4140);
+    b = __byte_perm(u, 0, 0x4342);
+  } else {
+    kv_codes_to_half<FMT>(w, a, b);
+  }
 }
 
 // after an abandoned wait: copies that are still on their way land before the CTA gives its shared memory back
@@ -73,9 +99,10 @@ struct KvLaneRow {
   int pos;        // last key it sees
   long long flat; // row number in the prefix pass
 };
+template <int BM>
 __device__ __forceinline__ KvLaneRow kv_lane_row(const KvAttnParams& p, const KvSegment& g, int r) {
   KvLaneRow x;
-  const long long flat = static_cast<long long>(g.u) * KV_BM + r;
+  const long long flat = static_cast<long long>(g.u) * BM + r;
   const int i = static_cast<int>(flat / p.group), hh = static_cast<int>(flat - static_cast<long long>(i) * p.group);
   const bool there = i < g.s.n;
   const int64_t t = g.s.first + i, head = static_cast<int64_t>(g.h) * p.group + hh;
@@ -91,11 +118,11 @@ __device__ __forceinline__ float2 kv_unpack(uint32_t w, int is_f16) {
 }
 __device__ __forceinline__ uint32_t kv_pack(float a, float b, int is_f16) { return is_f16 ? pack_half2(a, b) : pack_bf16x2(a, b); }
 
-template <int D, int FMT, int MODE>
-__global__ void __launch_bounds__(KV_NT, 2)
+template <int D, int FMT, int MODE, int NT>
+__global__ void __launch_bounds__(KV_NT, KvNarrow<D, NT>::CTAS)
 kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const KvAttnParams p) {
-  using L = KvNarrow<D>;
-  constexpr int S = L::STAGES, NJ = D / 8, CH = D / 8, QW = D / 4;
+  using L = KvNarrow<D, NT>;
+  constexpr int S = L::STAGES, BM = L::BM, MT = D / 16, CH = D / 8, QW = D / 4;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* scales = reinterpret_cast<float*>(smem + L::SCALES);
@@ -114,8 +141,8 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   }
   __syncthreads();
   grid_dependency_begin();
-  kv_find_run<KV_BM, TK, KV_NT>(p.r, p.c.page_log2, p.c.heads, p.group, tail->scan, &tail->run);
-  KvWalk<KV_BM, TK> walk(tail->run);
+  kv_find_run<BM, TK, KV_NT>(p.r, p.c.page_log2, p.c.heads, p.group, tail->scan, &tail->run);
+  KvWalk<BM, TK> walk(tail->run);
   KvSegment g;
 
   if (warp == KV_WARPS) {
@@ -128,7 +155,7 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     int stage = 0;
     uint32_t ph = 1;
     while (walk.next(p.r, p.c.page_log2, p.c.heads, p.group, g)) {
-      const int kend = min(g.k1, (kv_visible<KV_BM>(g.s, p.group, g.u, p.causal) + TK - 1) / TK);
+      const int kend = min(g.k1, (kv_visible<BM>(g.s, p.group, g.u, p.causal) + TK - 1) / TK);
       for (int kt = g.k0; kt < kend; ++kt) {
         const int at = kt * tile_pages + lane;
         const bool need = lane < tile_pages && (static_cast<int64_t>(at) << p.c.page_log2) < g.s.len;
@@ -164,8 +191,10 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   }
 
   // ------------------------------ computing warps ------------------------------
-  const int gq = lane >> 2, c = lane & 3;   // row pair gq, gq + 8; quarter of the channels / keys
-  const int kc0 = col_perm<D>(2 * c), kc1 = col_perm<D>(2 * c + 1);
+  // lane = (gq, c). K and V side: key gq of an 8-key block, channels of quarter c; query rows 8 nt + 2c + e are the lane's columns
+  const int gq = lane >> 2, c = lane & 3;
+  const int kg = col_perm<D>(gq), kc0 = col_perm<D>(2 * c), kc1 = col_perm<D>(2 * c + 1);
+  const int ch0 = CH * col_perm<D>(gq);   // first of the lane's D / 8 output channels
   bool ok = true, first = true;
   int stage = 0;
   uint32_t ph = 0;
@@ -177,49 +206,58 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       p.record[2 * blockIdx.x + 1] = make_int4(g.k0, static_cast<int>(W & 0xffffffffu), static_cast<int>(W >> 32), tail->run.G);
     }
     first = false;
-    const KvLaneRow r0 = kv_lane_row(p, g, gq), r1 = kv_lane_row(p, g, gq + 8);
-    // q rows: channels 16c .. 16c+15 of each 64, as the A fragments of D / 16 products
-    uint32_t a[D / 16][4];
-    float c0, c1;
-    {
-      uint32_t x[2][QW / 2];
+    // query rows as B fragments of D / 16 products, row 8 nt + gq, channels 16c .. 16c+15 of each 64; per column: the factor from
+    // accumulator to base-2 exponent, and where the accumulator begins
+    uint32_t qb[NT][D / 16][2];
+    float cf[NT][2], base[NT][2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int64_t at = i ? r1.q : r0.q;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int64_t at = kv_lane_row<BM>(p, g, 8 * nt + gq).q;
+      uint32_t x[QW / 2];
 #pragma unroll
-        for (int j = 0; j < QW / 8; ++j) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (at >= 0) v = ld_global_16(p.q + at + (j >> 1) * 64 + c * 16 + (j & 1) * 8);
-          x[i][4 * j] = v.x, x[i][4 * j + 1] = v.y, x[i][4 * j + 2] = v.z, x[i][4 * j + 3] = v.w;
-        }
+      for (int j = 0; j < QW / 8; ++j) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (at >= 0) v = ld_global_16(p.q + at + (j >> 1) * 64 + c * 16 + (j & 1) * 8);
+        x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
       }
-      float up[2], down[2];
+      float amax = 0.f, up, down;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float amax = 0.f;
-#pragma unroll
-        for (int j = 0; j < QW / 2; ++j) {
-          const float2 f = kv_unpack(x[i][j], p.is_f16);
-          amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-        }
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        kv_row_factor(amax, up[i], down[i]);
-#pragma unroll
-        for (int j = 0; j < QW / 2; ++j) {
-          const float2 f = kv_unpack(x[i][j], p.is_f16);
-          a[j >> 1][i + 2 * (j & 1)] = pack_half2(f.x * up[i], f.y * up[i]);
-        }
+      for (int j = 0; j < QW / 2; ++j) {
+        const float2 f = kv_unpack(x[j], p.is_f16);
+        amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
       }
-      c0 = p.sl2 * down[0], c1 = p.sl2 * down[1];
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      kv_row_factor(amax, up, down);
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < QW / 2; ++j) {
+        const float2 f = kv_unpack(x[j], p.is_f16);
+        const __half2 h = __floats2half2_rn(f.x * up, f.y * up);
+        qb[nt][j >> 1][j & 1] = *reinterpret_cast<const uint32_t*>(&h);
+        const float2 r = __half22float2(h);
+        sum += r.x + r.y;
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      const float f = p.sl2 * down * (FMT == RH3_KIND_I8 ? 16777216.f : 1.f);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        cf[nt][e] = __shfl_sync(0xffffffffu, f, (2 * c + e) * 4);
+        base[nt][e] = FMT == RH3_KIND_I8 ? __shfl_sync(0xffffffffu, sum * -0x1p-17f, (2 * c + e) * 4) : 0.f;
+      }
     }
-    float o[NJ][4];
+    float o[NT][MT][4];
+    float m[NT][2], l[NT][2];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < MT; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
+    }
 
-    const int kend = min(g.k1, (kv_visible<KV_BM>(g.s, p.group, g.u, p.causal) + TK - 1) / TK);
-    const int pos_first = p.causal ? g.s.len - g.s.n + static_cast<int>(static_cast<long long>(g.u) * KV_BM / p.group) : g.s.len - 1;
+    const int kend = min(g.k1, (kv_visible<BM>(g.s, p.group, g.u, p.causal) + TK - 1) / TK);
+    const int pos_first = p.causal ? g.s.len - g.s.n + static_cast<int>(static_cast<long long>(g.u) * BM / p.group) : g.s.len - 1;
     for (int kt = g.k0; kt < kend; ++kt) {
       if (!__all_sync(0xffffffffu, mbar_wait(&tail->full[stage], ph, abort_flag, p.status, ST_TIMEOUT_TMA_FULL))) {
         ok = false;
@@ -245,88 +283,115 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
         }
         __syncwarp();
       }
-      // ---- scores: 4 blocks of 8 keys ----
-      float u[4][4];
+      // ---- scores: 2 blocks of 16 keys; u[nt][block][row of the block: gq, gq + 8][column] ----
+      float u[NT][2][2][2];
+      float iv[2][2];
 #pragma unroll
-      for (int nb = 0; nb < 4; ++nb) {
-        const int key = nb * 8 + col_perm<D>(gq);
-        uint32_t w[QW / 4];
+      for (int kb = 0; kb < 2; ++kb) {
+        uint32_t w[2][QW / 4];
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
-          const uint4 v = *reinterpret_cast<const uint4*>(sk + chunk_at<D>(key, 4 * i + c));
-          w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-        }
-        u[nb][0] = u[nb][1] = u[nb][2] = u[nb][3] = 0.f;
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4*>(sk + chunk_at<D>(kb * 16 + r * 8 + kg, 4 * i + c));
+            w[r][4 * i] = v.x, w[r][4 * i + 1] = v.y, w[r][4 * i + 2] = v.z, w[r][4 * i + 3] = v.w;
+          }
+        float acc[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][2] = base[nt][0], acc[nt][1] = acc[nt][3] = base[nt][1];
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
-          uint32_t b0, b1;
-          kv_codes_to_half<FMT>(w[j], b0, b1);
-          mma_f16(u[nb], a[j], b0, b1);
+          uint32_t a[4];
+          k_codes_to_half<FMT>(w[0][j], a[0], a[2]);
+          k_codes_to_half<FMT>(w[1][j], a[1], a[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt], a, qb[nt][j][0], qb[nt][j][1]);
         }
-      }
-      float iv[4][2];
 #pragma unroll
-      for (int nb = 0; nb < 4; ++nb) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = nb * 8 + (e ? kc1 : kc0);
-          const float ks = sks[key], vs = fmaxf(sks[TK + key], kVsMin);
+        for (int r = 0; r < 2; ++r) {
+          const float ks = sks[kb * 16 + r * 8 + kg], vs = fmaxf(sks[TK + kb * 16 + r * 8 + kg], kVsMin);
           const float lv = kv_lg2(vs);
-          iv[nb][e] = __frcp_rn(vs);
-          u[nb][e] = fmaf(u[nb][e] * ks, c0, lv);
-          u[nb][2 + e] = fmaf(u[nb][2 + e] * ks, c1, lv);
-          if (masked) {
-            const bool is = there(key);
-            if (!is || pos0 + key > r0.pos) u[nb][e] = -INFINITY;
-            if (!is || pos0 + key > r1.pos) u[nb][2 + e] = -INFINITY;
+          iv[kb][r] = kv_rcp(vs);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            u[nt][kb][r][0] = fmaf(acc[nt][2 * r] * ks, cf[nt][0], lv);
+            u[nt][kb][r][1] = fmaf(acc[nt][2 * r + 1] * ks, cf[nt][1], lv);
           }
         }
       }
+      if (masked) {
+        int pos[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) pos[nt][e] = kv_lane_row<BM>(p, g, 8 * nt + 2 * c + e).pos;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int key = kb * 16 + r * 8 + kg;
+            const bool is = there(key);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                if (!is || pos0 + key > pos[nt][e]) u[nt][kb][r][e] = -INFINITY;
+              }
+          }
+      }
       // ---- running maximum ----
-      float n0 = m0, n1 = m1;
+      float n[NT][2], z[NT][2];
+      bool grew = false;
 #pragma unroll
-      for (int nb = 0; nb < 4; ++nb) {
-        n0 = fmaxf(n0, fmaxf(u[nb][0], u[nb][1]));
-        n1 = fmaxf(n1, fmaxf(u[nb][2], u[nb][3]));
-      }
-      n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 1));
-      n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 1));
-      n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2));
-      n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2));
-      const float z0 = n0 == -INFINITY ? 0.f : n0, z1 = n1 == -INFINITY ? 0.f : n1;   // nothing seen yet: weights 2^-inf = 0
-      if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
-        const float f0 = kv_ex2(m0 - z0), f1 = kv_ex2(m1 - z1);
-        l0 *= f0, l1 *= f1;
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) o[j][0] *= f0, o[j][1] *= f0, o[j][2] *= f1, o[j][3] *= f1;
-        m0 = n0, m1 = n1;
-      }
-      // ---- weights ----
-      uint32_t pa[2][4];
-#pragma unroll
-      for (int nb = 0; nb < 4; ++nb) {
-        float w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[e] = kv_ex2(u[nb][e] - (e < 2 ? z0 : z1) + kWeightLog2);
-          // a masked key's 1 / vs may be anything
-          const float add = masked && w[e] == 0.f ? 0.f : w[e] * iv[nb][e & 1];
-          if (e < 2) l0 += add;
-          else l1 += add;
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(fmaxf(u[nt][0][0][e], u[nt][0][1][e]), fmaxf(u[nt][1][0][e], u[nt][1][1][e]));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          n[nt][e] = fmaxf(m[nt][e], x);
+          grew |= n[nt][e] > m[nt][e];
+          z[nt][e] = (n[nt][e] == -INFINITY ? 0.f : n[nt][e]) - kWeightLog2;   // nothing seen yet: weights 2^-inf = 0
         }
-        pa[nb >> 1][2 * (nb & 1)] = pack_half2(w[0], w[1]);
-        pa[nb >> 1][2 * (nb & 1) + 1] = pack_half2(w[2], w[3]);
-      }
-      // ---- O += w . V: 2 steps of 16 keys ----
+      if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
+        for (int nt = 0; nt < NT; ++nt) {
+          const float f0 = kv_ex2(m[nt][0] - (z[nt][0] + kWeightLog2)), f1 = kv_ex2(m[nt][1] - (z[nt][1] + kWeightLog2));
+          l[nt][0] *= f0, l[nt][1] *= f1;
+          m[nt][0] = n[nt][0], m[nt][1] = n[nt][1];
+#pragma unroll
+          for (int j = 0; j < MT; ++j) o[nt][j][0] *= f0, o[nt][j][1] *= f1, o[nt][j][2] *= f0, o[nt][j][3] *= f1;
+        }
+      }
+      // ---- weights, as B fragments (16 keys x 8 rows) ----
+      uint32_t wb[NT][2][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float w0 = kv_ex2(u[nt][kb][r][0] - z[nt][0]), w1 = kv_ex2(u[nt][kb][r][1] - z[nt][1]);
+            if (!masked) {
+              l[nt][0] = fmaf(w0, iv[kb][r], l[nt][0]);
+              l[nt][1] = fmaf(w1, iv[kb][r], l[nt][1]);
+            } else {   // a key that a row does not see may have any scale
+              if (w0 != 0.f) l[nt][0] = fmaf(w0, iv[kb][r], l[nt][0]);
+              if (w1 != 0.f) l[nt][1] = fmaf(w1, iv[kb][r], l[nt][1]);
+            }
+            wb[nt][kb][r] = transpose8(pack_half2(w0, w1));
+          }
+      // ---- O^T += V^T . W^T ----
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
         constexpr int VW = D / 32;   // words of D / 8 channels
         uint32_t v[4][VW];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int key = s * 16 + (i >> 1) * 8 + ((i & 1) ? kc1 : kc0);
+          const int key = kb * 16 + (i >> 1) * 8 + ((i & 1) ? kc1 : kc0);
           if constexpr (D == 128) {
-            const uint4 x = *reinterpret_cast<const uint4*>(sv + chunk_at<D>(key, col_perm<D>(gq)));
+            const uint4 x = *reinterpret_cast<const uint4*>(sv + chunk_at<D>(key, kg));
             v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
           } else {
             const uint2 x = *reinterpret_cast<const uint2*>(sv + chunk_at<D>(key, gq >> 1) + (gq & 1) * 8);
@@ -334,15 +399,16 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
           }
         }
 #pragma unroll
-        for (int w = 0; w < VW; ++w) {
-          uint32_t b0[4], b1[4];
-          kv_codes_to_half<FMT>(__byte_perm(v[0][w], v[1][w], 0x5140), b0[0], b0[1]);
-          kv_codes_to_half<FMT>(__byte_perm(v[0][w], v[1][w], 0x7362), b0[2], b0[3]);
-          kv_codes_to_half<FMT>(__byte_perm(v[2][w], v[3][w], 0x5140), b1[0], b1[1]);
-          kv_codes_to_half<FMT>(__byte_perm(v[2][w], v[3][w], 0x7362), b1[2], b1[3]);
+        for (int w = 0; w < VW; ++w)
 #pragma unroll
-          for (int b = 0; b < 4; ++b) mma_f16(o[4 * w + b], pa[s], b0[b], b1[b]);
-        }
+          for (int b = 0; b < 2; ++b) {   // bytes 2b and 2b + 1: rows gq and gq + 8 of output block 2w + b
+            const uint32_t sel = b ? 0x7362 : 0x5140;
+            uint32_t a[4];
+            kv_codes_to_half<FMT>(__byte_perm(v[0][w], v[1][w], sel), a[0], a[1]);
+            kv_codes_to_half<FMT>(__byte_perm(v[2][w], v[3][w], sel), a[2], a[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][2 * w + b], a, wb[nt][kb][0], wb[nt][kb][1]);
+          }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&tail->empty[stage]);
@@ -353,75 +419,81 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     if (MODE == MODE_OWN && g.k0 == 0) {
       const long long rows = static_cast<long long>(p.r.T) * p.group;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const KvLaneRow& r = i ? r1 : r0;
-        float& m = i ? m1 : m0;
-        float& l = i ? l1 : l0;
-        int n = 0;
-        if (r.q >= 0) {
-          const long long unit = static_cast<long long>(g.h) * ((rows + p.pre_bm - 1) / p.pre_bm) + r.flat / p.pre_bm;
-          n = kv_owner(unit * p.pre_kt + p.pre_kt - 1, p.pre_w, p.pre_g) - kv_owner(unit * p.pre_kt, p.pre_w, p.pre_g) + 1;
-        }
-        for (int s = warp; s < n; s += KV_WARPS) {
-          const long long at = (static_cast<long long>(s) * p.c.heads + g.h) * rows + r.flat;
-          const float pm = p.pre_ml[2 * at], pl = p.pre_ml[2 * at + 1];
-          const float nm = fmaxf(m, pm);
-          const float z = nm == -INFINITY ? 0.f : nm;
-          const float f = kv_ex2(m - z), fp = kv_ex2(pm - z);
-          m = nm;
-          l = l * f + (c == 0 ? pl * fp : 0.f);   // l is a sum over the row's four lanes
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float* src = p.pre_o + at * D + CH * (e ? kc1 : kc0);
+        for (int e = 0; e < 2; ++e) {
+          const KvLaneRow r = kv_lane_row<BM>(p, g, 8 * nt + 2 * c + e);
+          int parts = 0;
+          if (r.q >= 0) {
+            const long long unit = static_cast<long long>(g.h) * ((rows + p.pre_bm - 1) / p.pre_bm) + r.flat / p.pre_bm;
+            parts = kv_owner(unit * p.pre_kt + p.pre_kt - 1, p.pre_w, p.pre_g) - kv_owner(unit * p.pre_kt, p.pre_w, p.pre_g) + 1;
+          }
+          for (int s = warp; s < parts; s += KV_WARPS) {
+            const long long at = (static_cast<long long>(s) * p.c.heads + g.h) * rows + r.flat;
+            const float pm = p.pre_ml[2 * at], pl = p.pre_ml[2 * at + 1];
+            const float nm = fmaxf(m[nt][e], pm);
+            const float zz = nm == -INFINITY ? 0.f : nm;
+            const float f = kv_ex2(m[nt][e] - zz), fp = kv_ex2(pm - zz);
+            m[nt][e] = nm;
+            l[nt][e] = l[nt][e] * f + (gq == 0 ? pl * fp : 0.f);   // l is a sum over the column's eight lanes
+            const float* src = p.pre_o + at * D + ch0;
 #pragma unroll
-            for (int j = 0; j < CH; j += 4) {
-              const uint4 x = ld_global_16(src + j);
-              o[j][2 * i + e] = o[j][2 * i + e] * f + __uint_as_float(x.x) * fp;
-              o[j + 1][2 * i + e] = o[j + 1][2 * i + e] * f + __uint_as_float(x.y) * fp;
-              o[j + 2][2 * i + e] = o[j + 2][2 * i + e] * f + __uint_as_float(x.z) * fp;
-              o[j + 3][2 * i + e] = o[j + 3][2 * i + e] * f + __uint_as_float(x.w) * fp;
+            for (int j = 0; j < MT; j += 2) {
+              const uint4 x = ld_global_16(src + 2 * j);
+              o[nt][j][e] = o[nt][j][e] * f + __uint_as_float(x.x) * fp;
+              o[nt][j][2 + e] = o[nt][j][2 + e] * f + __uint_as_float(x.y) * fp;
+              o[nt][j + 1][e] = o[nt][j + 1][e] * f + __uint_as_float(x.z) * fp;
+              o[nt][j + 1][2 + e] = o[nt][j + 1][2 + e] * f + __uint_as_float(x.w) * fp;
             }
           }
         }
-      }
     }
 
     // ---- join the four warps ----
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    if (c == 0) {
-      tail->ml[warp][gq][0] = m0, tail->ml[warp][gq][1] = l0;
-      tail->ml[warp][gq + 8][0] = m1, tail->ml[warp][gq + 8][1] = l1;
-    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 4);
+        l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8);
+        l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
+        if (gq == 0) tail->ml[warp][8 * nt + 2 * c + e][0] = m[nt][e], tail->ml[warp][8 * nt + 2 * c + e][1] = l[nt][e];
+      }
     if (bar_sync_or(1, KV_WARPS * 32, !ok)) {
       kv_settle();
       return;
     }
-    float M0 = -INFINITY, M1 = -INFINITY, L0 = 0.f, L1 = 0.f;
 #pragma unroll
-    for (int w = 0; w < KV_WARPS; ++w) M0 = fmaxf(M0, tail->ml[w][gq][0]), M1 = fmaxf(M1, tail->ml[w][gq + 8][0]);
-    const float z0 = M0 == -INFINITY ? 0.f : M0, z1 = M1 == -INFINITY ? 0.f : M1;
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int w = 0; w < KV_WARPS; ++w) {
-      L0 += tail->ml[w][gq][1] * kv_ex2(tail->ml[w][gq][0] - z0);
-      L1 += tail->ml[w][gq + 8][1] * kv_ex2(tail->ml[w][gq + 8][0] - z1);
-    }
-    const float f0 = kv_ex2(m0 - z0), f1 = kv_ex2(m1 - z1);
+      for (int e = 0; e < 2; ++e) {
+        const int col = 8 * nt + 2 * c + e;
+        float M = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) o[j][0] *= f0, o[j][1] *= f0, o[j][2] *= f1, o[j][3] *= f1;
+        for (int w = 0; w < KV_WARPS; ++w) M = fmaxf(M, tail->ml[w][col][0]);
+        const float zz = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int w = 0; w < KV_WARPS; ++w) sum += tail->ml[w][col][1] * kv_ex2(tail->ml[w][col][0] - zz);
+        const float f = kv_ex2(m[nt][e] - zz);
+#pragma unroll
+        for (int j = 0; j < MT; ++j) o[nt][j][e] *= f, o[nt][j][2 + e] *= f;
+        m[nt][e] = M, l[nt][e] = sum;
+      }
 #pragma unroll
     for (int w = 1; w <= KV_WARPS; ++w) {   // warp 1 writes, 2 and 3 add in place, 0 takes the sum
       if (warp == (w & (KV_WARPS - 1))) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          if (w > 1) {
-            const float4 x = merge[j * 32 + lane];
-            o[j][0] += x.x, o[j][1] += x.y, o[j][2] += x.z, o[j][3] += x.w;
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < MT; ++j) {
+            float4& at = merge[(nt * MT + j) * 32 + lane];
+            float* v = o[nt][j];
+            if (w > 1) {
+              const float4 x = at;
+              v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+            }
+            if (w < KV_WARPS) at = make_float4(v[0], v[1], v[2], v[3]);
           }
-          if (w < KV_WARPS) merge[j * 32 + lane] = make_float4(o[j][0], o[j][1], o[j][2], o[j][3]);
-        }
       }
       if (w < KV_WARPS) asm volatile("bar.sync 2, %0;" ::"n"(KV_WARPS * 32) : "memory");
     }
@@ -432,46 +504,47 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       const long long unit = static_cast<long long>(g.h) * g.s.qt + g.u;
       const int s = blockIdx.x - kv_owner(unit * g.s.kt, tail->run.W, tail->run.G);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const KvLaneRow& r = i ? r1 : r0;
-        if (r.q < 0) continue;
-        const long long at = (static_cast<long long>(s) * p.c.heads + g.h) * rows + r.flat;
-        if (c == 0) p.pre_ml[2 * at] = i ? M1 : M0, p.pre_ml[2 * at + 1] = i ? L1 : L0;
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float4* dst = reinterpret_cast<float4*>(p.pre_o + at * D + CH * (e ? kc1 : kc0));
+          const KvLaneRow r = kv_lane_row<BM>(p, g, 8 * nt + 2 * c + e);
+          if (r.q < 0) continue;
+          const long long at = (static_cast<long long>(s) * p.c.heads + g.h) * rows + r.flat;
+          if (gq == 0) p.pre_ml[2 * at] = m[nt][e], p.pre_ml[2 * at + 1] = l[nt][e];
+          float4* dst = reinterpret_cast<float4*>(p.pre_o + at * D + ch0);
 #pragma unroll
-          for (int j = 0; j < CH; j += 4)
-            dst[j >> 2] = make_float4(o[j][2 * i + e], o[j + 1][2 * i + e], o[j + 2][2 * i + e], o[j + 3][2 * i + e]);
+          for (int j = 0; j < MT; j += 2)
+            dst[j >> 1] = make_float4(o[nt][j][e], o[nt][j][2 + e], o[nt][j + 1][e], o[nt][j + 1][2 + e]);
         }
-      }
     } else if (g.k0 == 0 && g.k1 == g.s.kt) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const KvLaneRow& r = i ? r1 : r0;
-        if (r.q < 0) continue;
-        const float l = i ? L1 : L0;
-        const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);   // no key: 0
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          uint16_t* dst = p.out + r.o + CH * (e ? kc1 : kc0);
+          const KvLaneRow r = kv_lane_row<BM>(p, g, 8 * nt + 2 * c + e);
+          if (r.q < 0) continue;
+          const float inv = l[nt][e] == 0.f ? 0.f : __fdiv_rn(1.f, l[nt][e]);   // no key: 0
+          uint16_t* dst = p.out + r.o + ch0;
 #pragma unroll
-          for (int j = 0; j < CH; j += 8) {
+          for (int j = 0; j < MT; j += 4) {
             uint32_t w[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = kv_pack(o[j + 2 * k][2 * i + e] * inv, o[j + 2 * k + 1][2 * i + e] * inv, p.is_f16);
-            *reinterpret_cast<uint4*>(dst + j) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int k = 0; k < 4; ++k) w[k] = kv_pack(o[nt][j + k][e] * inv, o[nt][j + k][2 + e] * inv, p.is_f16);
+            *reinterpret_cast<uint4*>(dst + 2 * j) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
-      }
     } else {
-      float* slot = p.part + (2ll * blockIdx.x + (g.k0 > 0 ? 0 : 1)) * kv_part_floats<D>();
+      float* slot = p.part + (2ll * blockIdx.x + (g.k0 > 0 ? 0 : 1)) * L::PART;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) reinterpret_cast<float4*>(slot)[j * 32 + lane] = make_float4(o[j][0], o[j][1], o[j][2], o[j][3]);
-      if (c == 0) {
-        float* ml = slot + KV_BM * D;
-        ml[gq] = M0, ml[gq + 8] = M1;
-        ml[KV_BM + gq] = L0, ml[KV_BM + gq + 8] = L1;
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+          reinterpret_cast<float4*>(slot)[(nt * MT + j) * 32 + lane] = make_float4(o[nt][j][0], o[nt][j][1], o[nt][j][2], o[nt][j][3]);
+        if (gq == 0) {
+          float* ml = slot + BM * D + 8 * nt + 2 * c;
+          ml[0] = m[nt][0], ml[1] = m[nt][1];
+          ml[BM] = l[nt][0], ml[BM + 1] = l[nt][1];
+        }
       }
     }
   }
@@ -479,9 +552,10 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
 
 // Joins the parts of the unit that CTA c = blockIdx.x + 1 of the pass before began inside of, if it was the first to do so:
 // slot 1 of CTA c - 1 and slot 0 of c, c + 1, ... while their runs begin inside the unit. Parts are taken in order.
-template <int D>
-__global__ void __launch_bounds__(4 * D) kv_join_kernel(const KvAttnParams p) {
-  __shared__ float rows[KV_BM][D + 4];
+template <int D, int NT>
+__global__ void __launch_bounds__(2 * D * NT) kv_join_kernel(const KvAttnParams p) {
+  constexpr int BM = 8 * NT, MT = D / 16, PART = KvNarrow<D, NT>::PART;
+  __shared__ float rows[BM][D + 4];
   grid_dependency_begin();
   const int c = blockIdx.x + 1;
   const int4 a = p.record[2 * c];
@@ -492,57 +566,58 @@ __global__ void __launch_bounds__(4 * D) kv_join_kernel(const KvAttnParams p) {
   const long long xs = W * c / G - r.x, xe = xs + a.w;
   if (W * (c - 1) / G > xs) return;
   const int n = kv_owner(xe - 1, W, G) - c + 2;
-  const int lane = threadIdx.x & 31, j = threadIdx.x >> 5, gq = lane >> 2, q = lane & 3;
+  // thread = (block of columns nt, output block j, lane): four values of a fragment
+  const int lane = threadIdx.x & 31, j = (threadIdx.x >> 5) % MT, nt = (threadIdx.x >> 5) / MT, gq = lane >> 2, col = 8 * nt + 2 * (lane & 3);
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   constexpr int STEP = 8;
   for (int i0 = 0; i0 < n; i0 += STEP) {
     float4 x[STEP];
-    float pm[STEP][2], pl[STEP][2];
+    float2 pm[STEP], pl[STEP];
 #pragma unroll
     for (int i = 0; i < STEP; ++i) {
       if (i0 + i < n) {
-        const float* slot = p.part + (i0 + i == 0 ? 2ll * (c - 1) + 1 : 2ll * (c - 1 + i0 + i)) * kv_part_floats<D>();
-        x[i] = reinterpret_cast<const float4*>(slot)[j * 32 + lane];
-        pm[i][0] = slot[KV_BM * D + gq], pm[i][1] = slot[KV_BM * D + gq + 8];
-        pl[i][0] = slot[KV_BM * D + KV_BM + gq], pl[i][1] = slot[KV_BM * D + KV_BM + gq + 8];
+        const float* slot = p.part + (i0 + i == 0 ? 2ll * (c - 1) + 1 : 2ll * (c - 1 + i0 + i)) * PART;
+        x[i] = reinterpret_cast<const float4*>(slot)[threadIdx.x];
+        pm[i] = *reinterpret_cast<const float2*>(slot + BM * D + col);
+        pl[i] = *reinterpret_cast<const float2*>(slot + BM * D + BM + col);
       } else {
         x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        pm[i][0] = pm[i][1] = -INFINITY, pl[i][0] = pl[i][1] = 0.f;
+        pm[i] = make_float2(-INFINITY, -INFINITY), pl[i] = make_float2(0.f, 0.f);
       }
     }
     float n0 = m0, n1 = m1;
 #pragma unroll
-    for (int i = 0; i < STEP; ++i) n0 = fmaxf(n0, pm[i][0]), n1 = fmaxf(n1, pm[i][1]);
+    for (int i = 0; i < STEP; ++i) n0 = fmaxf(n0, pm[i].x), n1 = fmaxf(n1, pm[i].y);
     const float z0 = n0 == -INFINITY ? 0.f : n0, z1 = n1 == -INFINITY ? 0.f : n1;
     const float f0 = kv_ex2(m0 - z0), f1 = kv_ex2(m1 - z1);
-    o.x *= f0, o.y *= f0, o.z *= f1, o.w *= f1, l0 *= f0, l1 *= f1;
+    o.x *= f0, o.y *= f1, o.z *= f0, o.w *= f1, l0 *= f0, l1 *= f1;
     m0 = n0, m1 = n1;
 #pragma unroll
     for (int i = 0; i < STEP; ++i) {
-      const float e0 = kv_ex2(pm[i][0] - z0), e1 = kv_ex2(pm[i][1] - z1);
-      o.x += x[i].x * e0, o.y += x[i].y * e0, o.z += x[i].z * e1, o.w += x[i].w * e1;
-      l0 += pl[i][0] * e0, l1 += pl[i][1] * e1;
+      const float e0 = kv_ex2(pm[i].x - z0), e1 = kv_ex2(pm[i].y - z1);
+      o.x += x[i].x * e0, o.y += x[i].y * e1, o.z += x[i].z * e0, o.w += x[i].w * e1;
+      l0 += pl[i].x * e0, l1 += pl[i].y * e1;
     }
   }
   const float i0 = l0 == 0.f ? 0.f : __fdiv_rn(1.f, l0), i1 = l1 == 0.f ? 0.f : __fdiv_rn(1.f, l1);
-  constexpr int CH = D / 8;
-  rows[gq][CH * col_perm<D>(2 * q) + j] = o.x * i0;
-  rows[gq][CH * col_perm<D>(2 * q + 1) + j] = o.y * i0;
-  rows[gq + 8][CH * col_perm<D>(2 * q) + j] = o.z * i1;
-  rows[gq + 8][CH * col_perm<D>(2 * q + 1) + j] = o.w * i1;
+  const int ch = D / 8 * col_perm<D>(gq) + 2 * j;
+  rows[col][ch] = o.x * i0;
+  rows[col + 1][ch] = o.y * i1;
+  rows[col][ch + 1] = o.z * i0;
+  rows[col + 1][ch + 1] = o.w * i1;
   __syncthreads();
   KvSegment g;
-  g.s = kv_seq<KV_BM, TK>(p.r, p.c.page_log2, p.group, a.x);
+  g.s = kv_seq<BM, TK>(p.r, p.c.page_log2, p.group, a.x);
   g.b = a.x, g.h = a.y, g.u = a.z;
-  for (int k = threadIdx.x; k < KV_BM * D / 8; k += 4 * D) {
-    const int row = k / (D / 8), ch = (k % (D / 8)) * 8;
-    const KvLaneRow x = kv_lane_row(p, g, row);
+  for (int k = threadIdx.x; k < BM * D / 8; k += 2 * D * NT) {
+    const int row = k / (D / 8), at = (k % (D / 8)) * 8;
+    const KvLaneRow x = kv_lane_row<BM>(p, g, row);
     if (x.q < 0) continue;
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = kv_pack(rows[row][ch + 2 * i], rows[row][ch + 2 * i + 1], p.is_f16);
-    *reinterpret_cast<uint4*>(p.out + x.o + ch) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int i = 0; i < 4; ++i) w[i] = kv_pack(rows[row][at + 2 * i], rows[row][at + 2 * i + 1], p.is_f16);
+    *reinterpret_cast<uint4*>(p.out + x.o + at) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -553,43 +628,45 @@ int kv_maps(CUtensorMap* mk, CUtensorMap* mv, const KvCache& c, int64_t D) {
   return make_tmap_2d(mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, c.v, 128, rows, 128, 128, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// CTAs of a pass: two per SM, no more than there can be tiles
-template <class I>
-I kv_grid(I units, I kt) {
-  const I most = 2 * static_cast<I>(device_sm_count());
+// CTAs of a pass: as many as stay on the chip together, no more than there can be tiles
+int64_t kv_grid(int64_t units, int64_t kt, int per_sm) {
+  const int64_t most = static_cast<int64_t>(per_sm) * device_sm_count();
   return units * kt < most ? units * kt : most;
 }
 
-template <int D, int FMT, int MODE>
+template <int D, int FMT, int MODE, int NT>
 int kv_launch(const CUtensorMap& mk, const CUtensorMap& mv, const KvAttnParams& p, int64_t grid, cudaStream_t stream) {
-  auto kern = kv_attn_kernel<D, FMT, MODE>;
-  const int smem = kv_narrow_smem<D>();
+  auto kern = kv_attn_kernel<D, FMT, MODE, NT>;
+  const int smem = kv_narrow_smem<D, NT>();
   if (int e = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "kv_attn smem attribute")) return e;
   return check_cuda(launch_chained(kern, dim3(static_cast<unsigned>(grid)), KV_NT, smem, stream, 1, mk, mv, p), "kv_attn launch");
 }
 
-// The plan of a call: grids and the pieces of its workspace
+// The plan of a call: rows per unit, grids and the pieces of its workspace
 struct KvPlan {
-  int64_t kt, grid, pre_kt, pre_grid, pre_splits;   // own pass; prefix pass
+  int nt, pre_nt;                                   // units of 8 * nt rows in the own pass and in the prefix pass
+  int64_t kt, grid, pre_kt, pre_grid, pre_splits;   // key tiles of a sequence at most, CTAs; the prefix pass: also into how many parts a unit may fall
   int64_t record, part, pre_ml, pre_o, bytes;       // byte offsets
 };
 KvPlan kv_plan(int64_t heads, int64_t group, int64_t page, int64_t D, int64_t per_seq, int64_t B, int64_t T, int64_t prefix) {
   KvPlan x{};
   const int64_t rows = T * group;
-  x.kt = (per_seq * page + TK - 1) / TK;
-  if (x.kt < 1) x.kt = 1;
-  x.grid = kv_grid<int64_t>(heads * (rows / KV_BM + (B < T ? B : T)), x.kt);
   auto take = [&](int64_t bytes) {
     const int64_t at = x.bytes;
     x.bytes += (bytes + 255) / 256 * 256;
     return at;
   };
+  x.nt = rows <= 8 * B ? 1 : 2;   // 8 rows a sequence on average fill a unit of 8
+  x.kt = (per_seq * page + TK - 1) / TK;
+  if (x.kt < 1) x.kt = 1;
+  x.grid = kv_grid(heads * (rows / (8 * x.nt) + (B < T ? B : T)), x.kt, x.nt == 1 ? 3 : 2);
   x.record = take(x.grid * 2 * sizeof(int4));
-  x.part = take(x.grid * 2 * (D == 128 ? kv_part_floats<128>() : kv_part_floats<64>()) * sizeof(float));
+  x.part = take(x.grid * 2 * (8 * x.nt * D + 16 * x.nt) * sizeof(float));
   if (prefix > 0) {
-    const int64_t units = heads * ((rows + KV_BM - 1) / KV_BM);
+    x.pre_nt = rows <= 8 ? 1 : 2;
+    const int64_t bm = 8 * x.pre_nt, units = heads * ((rows + bm - 1) / bm);
     x.pre_kt = (prefix + TK - 1) / TK;
-    x.pre_grid = kv_grid<int64_t>(units, x.pre_kt);
+    x.pre_grid = kv_grid(units, x.pre_kt, x.pre_nt == 1 ? 3 : 2);
     const int64_t run = units * x.pre_kt / x.pre_grid;    // tiles of the shortest run
     x.pre_splits = (x.pre_kt - 1) / run + 2;
     if (x.pre_splits > x.pre_kt) x.pre_splits = x.pre_kt;
@@ -641,32 +718,37 @@ extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t w
   CUtensorMap mk, mv;
   if (int e = kv_maps(&mk, &mv, p.c, a->D)) return e;
 
-  auto launch = [&](auto mode, const KvAttnParams& q, int64_t grid) {
-    constexpr int M = decltype(mode)::value;
-    if (a->D == 128)
-      return a->kind == RH3_KIND_I8 ? kv_launch<128, RH3_KIND_I8, M>(mk, mv, q, grid, stream) : kv_launch<128, RH3_KIND_F8, M>(mk, mv, q, grid, stream);
-    return a->kind == RH3_KIND_I8 ? kv_launch<64, RH3_KIND_I8, M>(mk, mv, q, grid, stream) : kv_launch<64, RH3_KIND_F8, M>(mk, mv, q, grid, stream);
+  // fn(D, NT) as compile-time constants
+  auto by_size = [&](int nt, auto&& fn) {
+    if (a->D == 128) return nt == 1 ? fn(std::integral_constant<int, 128>(), std::integral_constant<int, 1>()) : fn(std::integral_constant<int, 128>(), std::integral_constant<int, 2>());
+    return nt == 1 ? fn(std::integral_constant<int, 64>(), std::integral_constant<int, 1>()) : fn(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+  };
+  auto launch = [&](auto mode, const KvAttnParams& q, int64_t grid, int nt) {
+    return by_size(nt, [&](auto d, auto n) {
+      constexpr int M = decltype(mode)::value, DD = decltype(d)::value, N = decltype(n)::value;
+      return a->kind == RH3_KIND_I8 ? kv_launch<DD, RH3_KIND_I8, M, N>(mk, mv, q, grid, stream) : kv_launch<DD, RH3_KIND_F8, M, N>(mk, mv, q, grid, stream);
+    });
   };
   if (a->prefix > 0) {
     p.pre_ml = reinterpret_cast<float*>(ws + x.pre_ml);
     p.pre_o = reinterpret_cast<float*>(ws + x.pre_o);
     p.pre_kt = static_cast<int>(x.pre_kt);
-    p.pre_bm = KV_BM;
-    p.pre_w = a->heads * ((a->T * a->group + KV_BM - 1) / KV_BM) * x.pre_kt;
+    p.pre_bm = 8 * x.pre_nt;
+    p.pre_w = a->heads * ((a->T * a->group + p.pre_bm - 1) / p.pre_bm) * x.pre_kt;
     p.pre_g = static_cast<int>(x.pre_grid);
     // the prefix is one sequence whose rows are all rows of the call
     KvAttnParams q = p;
     q.r = KvRows{a->prefix_table, nullptr, nullptr, a->prefix_pages, 1, static_cast<int>(a->prefix_pages), static_cast<int>(a->T),
                  static_cast<int>(a->prefix)};
     q.causal = 0;
-    if (int e = launch(std::integral_constant<int, MODE_PREFIX>(), q, x.pre_grid)) return e;
-    if (int e = launch(std::integral_constant<int, MODE_OWN>(), p, x.grid)) return e;
-  } else if (int e = launch(std::integral_constant<int, MODE_PLAIN>(), p, x.grid)) {
+    if (int e = launch(std::integral_constant<int, MODE_PREFIX>(), q, x.pre_grid, x.pre_nt)) return e;
+    if (int e = launch(std::integral_constant<int, MODE_OWN>(), p, x.grid, x.nt)) return e;
+  } else if (int e = launch(std::integral_constant<int, MODE_PLAIN>(), p, x.grid, x.nt)) {
     return e;
   }
   if (x.kt == 1 || x.grid == 1) return 0;   // no unit can be cut
-  const unsigned blocks = static_cast<unsigned>(x.grid - 1);
-  return check_cuda(a->D == 128 ? launch_chained(kv_join_kernel<128>, dim3(blocks), 512, 0, stream, 1, p)
-                                : launch_chained(kv_join_kernel<64>, dim3(blocks), 256, 0, stream, 1, p),
-                    "kv_join launch");
+  return by_size(x.nt, [&](auto d, auto n) {
+    constexpr int DD = decltype(d)::value, N = decltype(n)::value;
+    return check_cuda(launch_chained(kv_join_kernel<DD, N>, dim3(static_cast<unsigned>(x.grid - 1)), 2 * DD * N, 0, stream, 1, p), "kv_join launch");
+  });
 }

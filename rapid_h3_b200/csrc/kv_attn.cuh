@@ -26,7 +26,7 @@ struct KvAttnParams {
   float sl2;          // softmax scale * log2 e
   int* status;
   // partial results of units that more than one CTA works on: two slots per CTA, and one record per CTA
-  float* part;        // [grid][2][KV_PART_FLOATS]
+  float* part;        // [grid][2][BM * D + 2 * BM]: O in fragment order, m, l
   int4* record;       // [grid][2]: {b, h, u, kt}, {k0, W low, W high, G}; b < 0: the CTA does not begin inside a unit
   // shared prefix. Its pass writes every unit's parts row by row; the pass over the own keys takes them in.
   //   pre_o [split][heads][rows][D], pre_ml [split][heads][rows][2], rows = T * group
@@ -35,10 +35,6 @@ struct KvAttnParams {
   long long pre_w;    // tiles and CTAs of the prefix pass, tiles of one of its units, rows of its units: which splits exist
   int pre_g, pre_kt, pre_bm;
 };
-
-constexpr int KV_BM = 16;                              // rows of a unit of the narrow kernel
-template <int D>
-constexpr int kv_part_floats() { return KV_BM * D + 2 * KV_BM; }
 
 // the CTA whose run [W * c / G, W * (c + 1) / G) holds tile x
 __device__ __forceinline__ int kv_owner(long long x, long long W, int G) { return static_cast<int>(((x + 1) * G - 1) / W); }
@@ -51,6 +47,11 @@ __device__ __forceinline__ float kv_ex2(float x) {
 __device__ __forceinline__ float kv_lg2(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float kv_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
