@@ -402,7 +402,9 @@ int rh3_vae_gemm_swiglu(const void* xq, int64_t lda, const void* wq, const float
  * rh3_kv_attn: out[t, head] = softmax(scale * q . k) v over the keys of the row's sequence, at most its own position if causal; heads * group
  *   query heads, head h * group + i reads KV head h. A row without a key gives 0. With prefix > 0 every row sees the first
  *   `prefix` tokens of prefix_table's pages as well, before its own keys; lens, starts and positions then count the own part alone.
- *   workspace: rh3_kv_attn_workspace_bytes() bytes, 256-byte aligned, in use until the call's kernels are done. */
+ *   workspace: rh3_kv_attn_workspace_bytes() bytes, 256-byte aligned, in use until the call's kernels are done. counters:
+ *   RH3_KV_COUNTERS ints on the device, 0 before a call and left 0 by it; calls that may overlap (other streams, graphs) need their own. */
+#define RH3_KV_COUNTERS 1024
 typedef struct rh3_kv_attn_args {
   const void* q; int64_t q_st, q_sh;   /* [T][heads * group][D], token and head strides */
   void* out; int64_t o_st, o_sh;
@@ -423,7 +425,7 @@ int rh3_kv_read(const void* kc, const void* vc, const float* ks, const float* vs
                 const int32_t* starts, int64_t B, int64_t T, void* k, void* v, int dtype, cudaStream_t stream);
 int64_t rh3_kv_attn_workspace_bytes(int64_t heads, int64_t group, int64_t page, int64_t D, int64_t per_seq, int64_t B, int64_t T,
                                     int64_t prefix);
-int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t workspace_bytes, cudaStream_t stream);
+int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t workspace_bytes, int32_t* counters, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

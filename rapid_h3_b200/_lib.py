@@ -78,7 +78,7 @@ SIGNATURES = {
     "rh3_kv_write": [_P, _I64, _I64, _P, _I64, _I64, _I, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _I64, _P, _P, _I64, _I64, _P],
     "rh3_kv_read": [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _I, _P],
     "rh3_kv_attn_workspace_bytes": [_I64] * 8,
-    "rh3_kv_attn": [_P, _P, _I64, _P],
+    "rh3_kv_attn": [_P, _P, _I64, _P, _P],
     "rh3_upsample_causal2x": [_P, _P, _I64, _I64, _I64, _I64, _I64, _P],
 }
 # entry points that return a value instead of a status

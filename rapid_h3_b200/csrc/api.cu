@@ -428,6 +428,7 @@ extern "C" int rh3_check_status(cudaStream_t stream, int* status_out) {
   if (v != 0) {
     if (int e = rh3::check_cuda(cudaMemsetAsync(w, 0, sizeof(int), stream), "status clear")) return e;
     if (v == rh3::ST_KV_BAD_PAGE) rh3::set_error(v, "a page table named a page outside its cache (status %d)", v);
+    else if (v == rh3::ST_KV_BAD_STARTS) rh3::set_error(v, "the row starts of a batch are not ascending (status %d)", v);
     else rh3::set_error(v, "a bounded device wait gave up (status %d)", v);
   }
   if (status_out) *status_out = v;

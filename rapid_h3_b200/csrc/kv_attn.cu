@@ -2,8 +2,8 @@
 //
 // A unit is BM = 8 or 16 rows (new tokens x query heads of one KV head) of one sequence against all of its keys. What bounds it is
 // reading the cache once: 2 * (D + 4) bytes per key and head. The key tiles of all units are dealt to the CTAs in equal runs
-// (kv_cache.cuh), so ragged batches, single sequences and many heads all spread over the chip; a unit cut by a run's end leaves
-// partial results that a second small kernel joins in a fixed order.
+// (kv_cache.cuh), so ragged batches, single sequences and many heads all spread over the chip; of a unit that runs cut, every CTA
+// leaves a partial result, and the one whose is the last joins them, in a fixed order.
 //
 // One CTA = a producer warp and four warps that compute, each on 32 of a tile's 128 keys with its own running maximum, sums and
 // output, joined at the unit's end: no barrier among them per tile. The producer brings pages by TMA into a ring
@@ -37,17 +37,20 @@ struct KvNarrow {
   static constexpr int STAGES = (D == 128 ? 1 : 2) * (NT == 1 ? 2 : 3);
   static constexpr int STAGE_BYTES = 2 * TK * D;
   static constexpr int SCALES = STAGES * STAGE_BYTES;             // [STAGES][2][TK] floats
-  static constexpr int MERGE = SCALES + STAGES * 2 * TK * 4;      // [NT][D / 16][32] float4
-  static constexpr int TAIL = MERGE + BM * D * 4;
-  static constexpr int PART = BM * D + 2 * BM;                    // floats of a partial result
+  static constexpr int TAIL = SCALES + STAGES * 2 * TK * 4;
+  static constexpr int PART = BM * D + 2 * BM;                    // floats of a partial result: NT * D / 16 fragments, m, l
+  static constexpr int PER = NT * (D / 16) / KV_WARPS;            // fragments that a warp joins
+};
+struct KvJoin {   // a cut unit that the CTA has a part of; parts = 0: none, or not to be joined here
+  KvSegment g;
+  int first, parts;
 };
 struct __align__(8) KvTail {
-  uint64_t full[6], empty[6];
-  float ml[KV_WARPS][16][2];
-  long long scan[KV_NT / 32];
-  KvRun run;
+  uint64_t full[6], empty[6], parts;
+  float ml[2][KV_WARPS][2][16];   // two units' (m, l) of each warp's rows in turn
   uint32_t pages[6];   // which of a stage's pages were there
   int abort_flag;
+  KvJoin join[2];
 };
 template <int D, int NT>
 constexpr int kv_narrow_smem() { return KvNarrow<D, NT>::TAIL + static_cast<int>(sizeof(KvTail)) + 1024; }
@@ -80,6 +83,9 @@ __device__ __forceinline__ void kv_settle() {
   for (int i = 0; i < 64; ++i) __nanosleep(1000);
 }
 
+// the computing warps' barrier
+__device__ __forceinline__ void kv_bar() { asm volatile("bar.sync 2, %0;" ::"n"(KV_WARPS * 32) : "memory"); }
+
 // where 16-byte chunk `ch` of key `key` lies in a swizzled tile
 template <int D>
 __device__ __forceinline__ int chunk_at(int key, int ch) {
@@ -97,26 +103,98 @@ __device__ __forceinline__ int col_perm(int n) {
 struct KvLaneRow {
   int64_t q, o;   // element offsets of the row in q and out; q < 0: no such row
   int pos;        // last key it sees
-  long long flat; // row number in the prefix pass
+  int flat;       // row number in the prefix pass
 };
 template <int BM>
 __device__ __forceinline__ KvLaneRow kv_lane_row(const KvAttnParams& p, const KvSegment& g, int r) {
   KvLaneRow x;
-  const long long flat = static_cast<long long>(g.u) * BM + r;
-  const int i = static_cast<int>(flat / p.group), hh = static_cast<int>(flat - static_cast<long long>(i) * p.group);
+  const int flat = g.u * BM + r;
+  const int i = flat / p.group, hh = flat - i * p.group;
   const bool there = i < g.s.n;
   const int64_t t = g.s.first + i, head = static_cast<int64_t>(g.h) * p.group + hh;
   x.q = there ? t * p.q_st + head * p.q_sh : -1;
   x.o = t * p.o_st + head * p.o_sh;
   x.pos = p.causal ? g.s.len - g.s.n + i : g.s.len - 1;
-  x.flat = t * p.group + hh;
+  x.flat = (g.s.first + i) * p.group + hh;
   return x;
+}
+// End of the tiles of a segment that are worked on: the ones behind the last visible key are not, but one always is (its part of the ring
+// is where the warps' results meet).
+template <int BM>
+__device__ __forceinline__ int kv_last_tile(const KvAttnParams& p, const KvSegment& g) {
+  return max(g.k0 + 1, min(g.k1, (kv_visible<BM>(g.s, p.group, g.u, p.causal) + TK - 1) / TK));
 }
 __device__ __forceinline__ float2 kv_unpack(uint32_t w, int is_f16) {
   if (is_f16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
   return make_float2(bf16_lo(w), bf16_hi(w));
 }
 __device__ __forceinline__ uint32_t kv_pack(float a, float b, int is_f16) { return is_f16 ? pack_half2(a, b) : pack_bf16x2(a, b); }
+
+// Joins the parts of a cut unit: slot 1 of CTA `first`, slot 0 of the ones behind it, in that order. They are
+// brought into the ring (which is done with) by bulk copies, as many as it holds at a time, and every thread sums its own fragments'
+// values in rolled loops: the code runs once, its instructions come from L2.
+template <int D, int NT>
+__device__ __forceinline__ bool kv_join_parts(const KvAttnParams& p, const KvJoin& join, uint8_t* ring, KvTail* tail, uint32_t& phase) {
+  using L = KvNarrow<D, NT>;
+  constexpr int BM = L::BM, MT = D / 16, ROOM = L::SCALES / (L::PART * 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, c = lane & 3;
+  const int col = 8 * (warp * L::PER / MT) + 2 * c;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+  float4 o[L::PER];
+#pragma unroll
+  for (int k = 0; k < L::PER; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int i0 = 0; i0 < join.parts; i0 += ROOM) {
+    const int n = min(ROOM, join.parts - i0);
+    if (warp == 0) {
+      asm volatile("fence.proxy.async;" ::: "memory");   // parts were written, and the ring was read, by ordinary accesses
+      if (lane == 0) mbar_arrive_expect_tx(&tail->parts, n * L::PART * 4);
+      __syncwarp();
+      if (lane < n) bulk_load(ring + lane * L::PART * 4, p.part + kv_slot(join.first, i0 + lane) * L::PART, L::PART * 4, &tail->parts);
+    }
+    const bool came = mbar_wait(&tail->parts, phase, &tail->abort_flag, p.status, ST_TIMEOUT_TMA_FULL);
+    if (bar_sync_or(1, KV_WARPS * 32, !came)) {
+      kv_settle();
+      return false;
+    }
+    phase ^= 1;
+    const float* part = reinterpret_cast<const float*>(ring);
+    float n0 = m0, n1 = m1;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float2 pm = *reinterpret_cast<const float2*>(part + i * L::PART + BM * D + col);
+      n0 = fmaxf(n0, pm.x), n1 = fmaxf(n1, pm.y);
+    }
+    const float z0 = n0 == -INFINITY ? 0.f : n0, z1 = n1 == -INFINITY ? 0.f : n1;
+    const float f0 = kv_ex2(m0 - z0), f1 = kv_ex2(m1 - z1);
+    l0 *= f0, l1 *= f1;
+#pragma unroll
+    for (int k = 0; k < L::PER; ++k) o[k].x *= f0, o[k].y *= f1, o[k].z *= f0, o[k].w *= f1;
+    m0 = n0, m1 = n1;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float* at = part + i * L::PART;
+      const float2 pm = *reinterpret_cast<const float2*>(at + BM * D + col), pl = *reinterpret_cast<const float2*>(at + BM * D + BM + col);
+      const float e0 = kv_ex2(pm.x - z0), e1 = kv_ex2(pm.y - z1);
+      l0 = fmaf(pl.x, e0, l0), l1 = fmaf(pl.y, e1, l1);
+#pragma unroll
+      for (int k = 0; k < L::PER; ++k) {
+        const float4 x = reinterpret_cast<const float4*>(at)[(warp * L::PER + k) * 32 + lane];
+        o[k].x = fmaf(x.x, e0, o[k].x), o[k].y = fmaf(x.y, e1, o[k].y), o[k].z = fmaf(x.z, e0, o[k].z), o[k].w = fmaf(x.w, e1, o[k].w);
+      }
+    }
+    kv_bar();   // before the ring is written again
+  }
+  const float i0 = l0 == 0.f ? 0.f : __fdiv_rn(1.f, l0), i1 = l1 == 0.f ? 0.f : __fdiv_rn(1.f, l1);
+  const KvLaneRow r0 = kv_lane_row<BM>(p, join.g, col), r1 = kv_lane_row<BM>(p, join.g, col + 1);
+#pragma unroll
+  for (int k = 0; k < L::PER; ++k) {   // a fragment is two neighbouring channels of two rows
+    const int ch = D / 8 * col_perm<D>(gq) + 2 * (warp * L::PER % MT + k);
+    if (r0.q >= 0) *reinterpret_cast<uint32_t*>(p.out + r0.o + ch) = kv_pack(o[k].x * i0, o[k].z * i0, p.is_f16);
+    if (r1.q >= 0) *reinterpret_cast<uint32_t*>(p.out + r1.o + ch) = kv_pack(o[k].y * i1, o[k].w * i1, p.is_f16);
+  }
+  return true;
+}
 
 template <int D, int FMT, int MODE, int NT>
 __global__ void __launch_bounds__(KV_NT, KvNarrow<D, NT>::CTAS)
@@ -126,7 +204,6 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* scales = reinterpret_cast<float*>(smem + L::SCALES);
-  float4* merge = reinterpret_cast<float4*>(smem + L::MERGE);
   KvTail* tail = reinterpret_cast<KvTail*>(smem + L::TAIL);
   volatile int* abort_flag = &tail->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -136,13 +213,15 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       mbar_init(&tail->full[s], 1);
       mbar_init(&tail->empty[s], KV_WARPS);
     }
+    mbar_init(&tail->parts, 1);
     tail->abort_flag = 0;
+    tail->join[0].parts = tail->join[1].parts = 0;
     fence_barrier_init();
   }
   __syncthreads();
   grid_dependency_begin();
-  kv_find_run<BM, TK, KV_NT>(p.r, p.c.page_log2, p.c.heads, p.group, tail->scan, &tail->run);
-  KvWalk<BM, TK> walk(tail->run);
+  const KvRun run = kv_find_run<BM, TK>(p.r, p.c.page_log2, p.c.heads, p.group, p.most, p.status);
+  KvWalk<BM, TK> walk(run);
   KvSegment g;
 
   if (warp == KV_WARPS) {
@@ -155,7 +234,7 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     int stage = 0;
     uint32_t ph = 1;
     while (walk.next(p.r, p.c.page_log2, p.c.heads, p.group, g)) {
-      const int kend = min(g.k1, (kv_visible<BM>(g.s, p.group, g.u, p.causal) + TK - 1) / TK);
+      const int kend = kv_last_tile<BM>(p, g);
       for (int kt = g.k0; kt < kend; ++kt) {
         const int at = kt * tile_pages + lane;
         const bool need = lane < tile_pages && (static_cast<int64_t>(at) << p.c.page_log2) < g.s.len;
@@ -195,17 +274,10 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   const int gq = lane >> 2, c = lane & 3;
   const int kg = col_perm<D>(gq), kc0 = col_perm<D>(2 * c), kc1 = col_perm<D>(2 * c + 1);
   const int ch0 = CH * col_perm<D>(gq);   // first of the lane's D / 8 output channels
-  bool ok = true, first = true;
-  int stage = 0;
+  bool ok = true;
+  int stage = 0, unit = 0;
   uint32_t ph = 0;
-  if (MODE != MODE_PREFIX && threadIdx.x == 0 && tail->run.x0 >= tail->run.x1) p.record[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);
   while (walk.next(p.r, p.c.page_log2, p.c.heads, p.group, g)) {
-    if (MODE != MODE_PREFIX && first && threadIdx.x == 0) {
-      p.record[2 * blockIdx.x] = make_int4(g.k0 > 0 ? g.b : -1, g.h, g.u, g.s.kt);
-      const unsigned long long W = static_cast<unsigned long long>(tail->run.W);
-      p.record[2 * blockIdx.x + 1] = make_int4(g.k0, static_cast<int>(W & 0xffffffffu), static_cast<int>(W >> 32), tail->run.G);
-    }
-    first = false;
     // query rows as B fragments of D / 16 products, row 8 nt + gq, channels 16c .. 16c+15 of each 64; per column: the factor from
     // accumulator to base-2 exponent, and where the accumulator begins
     uint32_t qb[NT][D / 16][2];
@@ -256,8 +328,8 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       for (int j = 0; j < MT; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
     }
 
-    const int kend = min(g.k1, (kv_visible<BM>(g.s, p.group, g.u, p.causal) + TK - 1) / TK);
-    const int pos_first = p.causal ? g.s.len - g.s.n + static_cast<int>(static_cast<long long>(g.u) * BM / p.group) : g.s.len - 1;
+    const int kend = kv_last_tile<BM>(p, g);
+    const int pos_first = p.causal ? g.s.len - g.s.n + g.u * BM / p.group : g.s.len - 1;
     for (int kt = g.k0; kt < kend; ++kt) {
       if (!__all_sync(0xffffffffu, mbar_wait(&tail->full[stage], ph, abort_flag, p.status, ST_TIMEOUT_TMA_FULL))) {
         ok = false;
@@ -411,6 +483,7 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
           }
       }
       __syncwarp();
+      if (kt + 1 == kend) break;   // the last tile's stage is kept for the join below
       if (lane == 0) mbar_arrive(&tail->empty[stage]);
       if (++stage == S) stage = 0, ph ^= 1;
     }
@@ -425,8 +498,8 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
           const KvLaneRow r = kv_lane_row<BM>(p, g, 8 * nt + 2 * c + e);
           int parts = 0;
           if (r.q >= 0) {
-            const long long unit = static_cast<long long>(g.h) * ((rows + p.pre_bm - 1) / p.pre_bm) + r.flat / p.pre_bm;
-            parts = kv_owner(unit * p.pre_kt + p.pre_kt - 1, p.pre_w, p.pre_g) - kv_owner(unit * p.pre_kt, p.pre_w, p.pre_g) + 1;
+            const int x = (g.h * ((static_cast<int>(rows) + p.pre_bm - 1) / p.pre_bm) + r.flat / p.pre_bm) * p.pre_kt;
+            parts = (x + p.pre_kt - 1) / p.pre_run - x / p.pre_run + 1;
           }
           for (int s = warp; s < parts; s += KV_WARPS) {
             const long long at = (static_cast<long long>(s) * p.c.heads + g.h) * rows + r.flat;
@@ -449,175 +522,111 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
         }
     }
 
-    // ---- join the four warps ----
+    // ---- join the four warps: each leaves its sums where its own keys of the last tile were ----
+    float4* own = reinterpret_cast<float4*>(smem + stage * L::STAGE_BYTES + warp * 32 * D);   // fragments of nt = 0 over its K rows, 1 over V
+    float(*ml)[2][16] = tail->ml[unit & 1];
+    ++unit;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 4);
         l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8);
         l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
-        if (gq == 0) tail->ml[warp][8 * nt + 2 * c + e][0] = m[nt][e], tail->ml[warp][8 * nt + 2 * c + e][1] = l[nt][e];
+        if (gq == 0) ml[warp][0][8 * nt + 2 * c + e] = m[nt][e], ml[warp][1][8 * nt + 2 * c + e] = l[nt][e];
       }
+#pragma unroll
+      for (int j = 0; j < MT; ++j) own[nt * (TK * D / 16) + j * 32 + lane] = make_float4(o[nt][j][0], o[nt][j][1], o[nt][j][2], o[nt][j][3]);
+    }
     if (bar_sync_or(1, KV_WARPS * 32, !ok)) {
       kv_settle();
       return;
     }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    // this thread: rows col, col + 1 of fragments warp * PER + k
+    const int jnt = warp * L::PER / MT, col = 8 * jnt + 2 * c;
+    float M[2], sum[2] = {0.f, 0.f};
+    float4 x[L::PER];
+    {
+      float f[KV_WARPS][2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int col = 8 * nt + 2 * c + e;
-        float M = -INFINITY, sum = 0.f;
+        M[e] = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < KV_WARPS; ++w) M = fmaxf(M, tail->ml[w][col][0]);
-        const float zz = M == -INFINITY ? 0.f : M;
+        for (int w = 0; w < KV_WARPS; ++w) M[e] = fmaxf(M[e], ml[w][0][col + e]);
+        const float zz = M[e] == -INFINITY ? 0.f : M[e];
 #pragma unroll
-        for (int w = 0; w < KV_WARPS; ++w) sum += tail->ml[w][col][1] * kv_ex2(tail->ml[w][col][0] - zz);
-        const float f = kv_ex2(m[nt][e] - zz);
-#pragma unroll
-        for (int j = 0; j < MT; ++j) o[nt][j][e] *= f, o[nt][j][2 + e] *= f;
-        m[nt][e] = M, l[nt][e] = sum;
+        for (int w = 0; w < KV_WARPS; ++w) {
+          f[w][e] = kv_ex2(ml[w][0][col + e] - zz);
+          sum[e] = fmaf(ml[w][1][col + e], f[w][e], sum[e]);
+        }
       }
 #pragma unroll
-    for (int w = 1; w <= KV_WARPS; ++w) {   // warp 1 writes, 2 and 3 add in place, 0 takes the sum
-      if (warp == (w & (KV_WARPS - 1))) {
+      for (int k = 0; k < L::PER; ++k) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+      for (int w = 0; w < KV_WARPS; ++w) {
+        const float4* src = reinterpret_cast<const float4*>(smem + stage * L::STAGE_BYTES + w * 32 * D) + jnt * (TK * D / 16) + (warp * L::PER % MT) * 32 + lane;
 #pragma unroll
-          for (int j = 0; j < MT; ++j) {
-            float4& at = merge[(nt * MT + j) * 32 + lane];
-            float* v = o[nt][j];
-            if (w > 1) {
-              const float4 x = at;
-              v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
-            }
-            if (w < KV_WARPS) at = make_float4(v[0], v[1], v[2], v[3]);
-          }
+        for (int k = 0; k < L::PER; ++k) {
+          const float4 y = src[k * 32];
+          x[k].x = fmaf(y.x, f[w][0], x[k].x), x[k].y = fmaf(y.y, f[w][1], x[k].y), x[k].z = fmaf(y.z, f[w][0], x[k].z), x[k].w = fmaf(y.w, f[w][1], x[k].w);
+        }
       }
-      if (w < KV_WARPS) asm volatile("bar.sync 2, %0;" ::"n"(KV_WARPS * 32) : "memory");
     }
-    if (warp != 0) continue;
+    fence_proxy_async_smem();   // the stage goes back to the TMA
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&tail->empty[stage]);
+    if (++stage == S) stage = 0, ph ^= 1;
 
-    if constexpr (MODE == MODE_PREFIX) {
-      const long long rows = static_cast<long long>(p.r.T) * p.group;
-      const long long unit = static_cast<long long>(g.h) * g.s.qt + g.u;
-      const int s = blockIdx.x - kv_owner(unit * g.s.kt, tail->run.W, tail->run.G);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const KvLaneRow r = kv_lane_row<BM>(p, g, 8 * nt + 2 * c + e);
-          if (r.q < 0) continue;
-          const long long at = (static_cast<long long>(s) * p.c.heads + g.h) * rows + r.flat;
-          if (gq == 0) p.pre_ml[2 * at] = m[nt][e], p.pre_ml[2 * at + 1] = l[nt][e];
-          float4* dst = reinterpret_cast<float4*>(p.pre_o + at * D + ch0);
-#pragma unroll
-          for (int j = 0; j < MT; j += 2)
-            dst[j >> 1] = make_float4(o[nt][j][e], o[nt][j][2 + e], o[nt][j + 1][e], o[nt][j + 1][2 + e]);
-        }
-    } else if (g.k0 == 0 && g.k1 == g.s.kt) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const KvLaneRow r = kv_lane_row<BM>(p, g, 8 * nt + 2 * c + e);
-          if (r.q < 0) continue;
-          const float inv = l[nt][e] == 0.f ? 0.f : __fdiv_rn(1.f, l[nt][e]);   // no key: 0
-          uint16_t* dst = p.out + r.o + ch0;
-#pragma unroll
-          for (int j = 0; j < MT; j += 4) {
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = kv_pack(o[nt][j + k][e] * inv, o[nt][j + k][2 + e] * inv, p.is_f16);
-            *reinterpret_cast<uint4*>(dst + 2 * j) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-    } else {
+    if (MODE != MODE_PREFIX && (g.k0 > 0 || g.k1 < g.s.kt)) {   // a part of a unit
+      const int at = g.x / run.run, parts = (g.x + g.s.kt - 1) / run.run - at + 1;
       float* slot = p.part + (2ll * blockIdx.x + (g.k0 > 0 ? 0 : 1)) * L::PART;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int j = 0; j < MT; ++j)
-          reinterpret_cast<float4*>(slot)[(nt * MT + j) * 32 + lane] = make_float4(o[nt][j][0], o[nt][j][1], o[nt][j][2], o[nt][j][3]);
-        if (gq == 0) {
-          float* ml = slot + BM * D + 8 * nt + 2 * c;
-          ml[0] = m[nt][0], ml[1] = m[nt][1];
-          ml[BM] = l[nt][0], ml[BM + 1] = l[nt][1];
-        }
+      for (int k = 0; k < L::PER; ++k) reinterpret_cast<float4*>(slot)[(warp * L::PER + k) * 32 + lane] = x[k];
+      if (gq == 0 && warp * L::PER % MT == 0) {
+        *reinterpret_cast<float2*>(slot + BM * D + col) = make_float2(M[0], M[1]);
+        *reinterpret_cast<float2*>(slot + BM * D + BM + col) = make_float2(sum[0], sum[1]);
       }
+      if (threadIdx.x == 0) {   // counted, and joined by whose part is the last, when the run is done
+        KvJoin& join = tail->join[g.k0 > 0 ? 0 : 1];
+        join.g = g, join.first = at, join.parts = parts;
+      }
+      continue;
     }
-  }
-}
-
-// Joins the parts of the unit that CTA c = blockIdx.x + 1 of the pass before began inside of, if it was the first to do so:
-// slot 1 of CTA c - 1 and slot 0 of c, c + 1, ... while their runs begin inside the unit. Parts are taken in order.
-template <int D, int NT>
-__global__ void __launch_bounds__(2 * D * NT) kv_join_kernel(const KvAttnParams p) {
-  constexpr int BM = 8 * NT, MT = D / 16, PART = KvNarrow<D, NT>::PART;
-  __shared__ float rows[BM][D + 4];
-  grid_dependency_begin();
-  const int c = blockIdx.x + 1;
-  const int4 a = p.record[2 * c];
-  if (a.x < 0) return;
-  const int4 r = p.record[2 * c + 1];
-  const long long W = static_cast<long long>((static_cast<unsigned long long>(static_cast<unsigned>(r.z)) << 32) | static_cast<unsigned>(r.y));
-  const int G = r.w;
-  const long long xs = W * c / G - r.x, xe = xs + a.w;
-  if (W * (c - 1) / G > xs) return;
-  const int n = kv_owner(xe - 1, W, G) - c + 2;
-  // thread = (block of columns nt, output block j, lane): four values of a fragment
-  const int lane = threadIdx.x & 31, j = (threadIdx.x >> 5) % MT, nt = (threadIdx.x >> 5) / MT, gq = lane >> 2, col = 8 * nt + 2 * (lane & 3);
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  constexpr int STEP = 8;
-  for (int i0 = 0; i0 < n; i0 += STEP) {
-    float4 x[STEP];
-    float2 pm[STEP], pl[STEP];
 #pragma unroll
-    for (int i = 0; i < STEP; ++i) {
-      if (i0 + i < n) {
-        const float* slot = p.part + (i0 + i == 0 ? 2ll * (c - 1) + 1 : 2ll * (c - 1 + i0 + i)) * PART;
-        x[i] = reinterpret_cast<const float4*>(slot)[threadIdx.x];
-        pm[i] = *reinterpret_cast<const float2*>(slot + BM * D + col);
-        pl[i] = *reinterpret_cast<const float2*>(slot + BM * D + BM + col);
+    for (int e = 0; e < 2; ++e) {
+      const KvLaneRow r = kv_lane_row<BM>(p, g, col + e);
+      if (r.q < 0) continue;
+      if constexpr (MODE == MODE_PREFIX) {
+        const long long at = (static_cast<long long>(blockIdx.x - g.x / run.run) * p.c.heads + g.h) * p.r.T * p.group + r.flat;
+        if (gq == 0 && warp * L::PER % MT == 0) *reinterpret_cast<float2*>(p.pre_ml + 2 * at) = make_float2(M[e], sum[e]);
+#pragma unroll
+        for (int k = 0; k < L::PER; ++k)
+          *reinterpret_cast<float2*>(p.pre_o + at * D + ch0 + 2 * (warp * L::PER % MT + k)) = e ? make_float2(x[k].y, x[k].w) : make_float2(x[k].x, x[k].z);
       } else {
-        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        pm[i] = make_float2(-INFINITY, -INFINITY), pl[i] = make_float2(0.f, 0.f);
+        const float inv = sum[e] == 0.f ? 0.f : __fdiv_rn(1.f, sum[e]);   // no key: 0
+#pragma unroll
+        for (int k = 0; k < L::PER; ++k)
+          *reinterpret_cast<uint32_t*>(p.out + r.o + ch0 + 2 * (warp * L::PER % MT + k)) =
+              kv_pack((e ? x[k].y : x[k].x) * inv, (e ? x[k].w : x[k].z) * inv, p.is_f16);
       }
     }
-    float n0 = m0, n1 = m1;
-#pragma unroll
-    for (int i = 0; i < STEP; ++i) n0 = fmaxf(n0, pm[i].x), n1 = fmaxf(n1, pm[i].y);
-    const float z0 = n0 == -INFINITY ? 0.f : n0, z1 = n1 == -INFINITY ? 0.f : n1;
-    const float f0 = kv_ex2(m0 - z0), f1 = kv_ex2(m1 - z1);
-    o.x *= f0, o.y *= f1, o.z *= f0, o.w *= f1, l0 *= f0, l1 *= f1;
-    m0 = n0, m1 = n1;
-#pragma unroll
-    for (int i = 0; i < STEP; ++i) {
-      const float e0 = kv_ex2(pm[i].x - z0), e1 = kv_ex2(pm[i].y - z1);
-      o.x += x[i].x * e0, o.y += x[i].y * e1, o.z += x[i].z * e0, o.w += x[i].w * e1;
-      l0 += pl[i].x * e0, l1 += pl[i].y * e1;
-    }
   }
-  const float i0 = l0 == 0.f ? 0.f : __fdiv_rn(1.f, l0), i1 = l1 == 0.f ? 0.f : __fdiv_rn(1.f, l1);
-  const int ch = D / 8 * col_perm<D>(gq) + 2 * j;
-  rows[col][ch] = o.x * i0;
-  rows[col + 1][ch] = o.y * i1;
-  rows[col][ch + 1] = o.z * i0;
-  rows[col + 1][ch + 1] = o.w * i1;
-  __syncthreads();
-  KvSegment g;
-  g.s = kv_seq<BM, TK>(p.r, p.c.page_log2, p.group, a.x);
-  g.b = a.x, g.h = a.y, g.u = a.z;
-  for (int k = threadIdx.x; k < BM * D / 8; k += 2 * D * NT) {
-    const int row = k / (D / 8), at = (k % (D / 8)) * 8;
-    const KvLaneRow x = kv_lane_row<BM>(p, g, row);
-    if (x.q < 0) continue;
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = kv_pack(rows[row][at + 2 * i], rows[row][at + 2 * i + 1], p.is_f16);
-    *reinterpret_cast<uint4*>(p.out + x.o + at) = make_uint4(w[0], w[1], w[2], w[3]);
+  if constexpr (MODE != MODE_PREFIX) {
+    __threadfence();
+    kv_bar();
+    if (threadIdx.x < 2) {
+      KvJoin& join = tail->join[threadIdx.x];
+      if (join.parts) {
+        if (atomicAdd(p.count + join.first, 1) == join.parts - 1) p.count[join.first] = 0;   // nobody else comes
+        else join.parts = 0;
+      }
+      __threadfence();
+    }
+    kv_bar();
+    uint32_t phase = 0;
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i)
+      if (tail->join[i].parts && !kv_join_parts<D, NT>(p, tail->join[i], smem, tail, phase)) return;
   }
 }
 
@@ -645,8 +654,9 @@ int kv_launch(const CUtensorMap& mk, const CUtensorMap& mv, const KvAttnParams& 
 // The plan of a call: rows per unit, grids and the pieces of its workspace
 struct KvPlan {
   int nt, pre_nt;                                   // units of 8 * nt rows in the own pass and in the prefix pass
-  int64_t kt, grid, pre_kt, pre_grid, pre_splits;   // key tiles of a sequence at most, CTAs; the prefix pass: also into how many parts a unit may fall
-  int64_t record, part, pre_ml, pre_o, bytes;       // byte offsets
+  int64_t kt, w, grid;                              // key tiles of a sequence and tiles of the call at most, CTAs
+  int64_t pre_kt, pre_w, pre_run, pre_grid, pre_splits;   // the prefix pass: also tiles of a CTA, and into how many parts a unit may fall
+  int64_t part, pre_ml, pre_o, bytes;       // byte offsets
 };
 KvPlan kv_plan(int64_t heads, int64_t group, int64_t page, int64_t D, int64_t per_seq, int64_t B, int64_t T, int64_t prefix) {
   KvPlan x{};
@@ -659,16 +669,19 @@ KvPlan kv_plan(int64_t heads, int64_t group, int64_t page, int64_t D, int64_t pe
   x.nt = rows <= 8 * B ? 1 : 2;   // 8 rows a sequence on average fill a unit of 8
   x.kt = (per_seq * page + TK - 1) / TK;
   if (x.kt < 1) x.kt = 1;
-  x.grid = kv_grid(heads * (rows / (8 * x.nt) + (B < T ? B : T)), x.kt, x.nt == 1 ? 3 : 2);
-  x.record = take(x.grid * 2 * sizeof(int4));
+  const int64_t units = heads * (rows / (8 * x.nt) + (B < T ? B : T));
+  x.w = units * x.kt;
+  x.grid = kv_grid(units, x.kt, x.nt == 1 ? 3 : 2);
   x.part = take(x.grid * 2 * (8 * x.nt * D + 16 * x.nt) * sizeof(float));
   if (prefix > 0) {
     x.pre_nt = rows <= 8 ? 1 : 2;
     const int64_t bm = 8 * x.pre_nt, units = heads * ((rows + bm - 1) / bm);
     x.pre_kt = (prefix + TK - 1) / TK;
-    x.pre_grid = kv_grid(units, x.pre_kt, x.pre_nt == 1 ? 3 : 2);
-    const int64_t run = units * x.pre_kt / x.pre_grid;    // tiles of the shortest run
-    x.pre_splits = (x.pre_kt - 1) / run + 2;
+    x.pre_w = units * x.pre_kt;
+    const int64_t grid = kv_grid(units, x.pre_kt, x.pre_nt == 1 ? 3 : 2);
+    x.pre_run = (x.pre_w + grid - 1) / grid;
+    x.pre_grid = (x.pre_w + x.pre_run - 1) / x.pre_run;
+    x.pre_splits = (x.pre_kt - 1) / x.pre_run + 2;
     if (x.pre_splits > x.pre_kt) x.pre_splits = x.pre_kt;
     x.pre_ml = take(x.pre_splits * heads * rows * 2 * sizeof(float));
     x.pre_o = take(x.pre_splits * heads * rows * D * sizeof(float));
@@ -687,7 +700,7 @@ extern "C" int64_t rh3_kv_attn_workspace_bytes(int64_t heads, int64_t group, int
   return kv_plan(heads, group, page, D, per_seq, B, T, prefix).bytes;
 }
 
-extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
+extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t workspace_bytes, int32_t* counters, cudaStream_t stream) {
   RH3_CHECK_ARG(a, "kv_attn: null arguments");
   KvAttnParams p{};
   if (int e = kv_fill_cache(&p.c, "kv_attn", a->k, a->v, a->ks, a->vs, a->pages, a->heads, a->page, a->D, a->kind)) return e;
@@ -704,6 +717,8 @@ extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t w
   const KvPlan x = kv_plan(a->heads, a->group, a->page, a->D, a->per_seq, a->B, a->T, a->prefix);
   RH3_CHECK_ARG(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= x.bytes,
                 "kv_attn: a workspace of %lld bytes, 256-byte aligned, is needed", (long long)x.bytes);
+  RH3_CHECK_ARG(counters && x.grid <= RH3_KV_COUNTERS, "kv_attn: the counters are missing, or too few for the device");
+  RH3_CHECK_ARG(x.w < (1ll << 31) && x.pre_w < (1ll << 31), "kv_attn: too many rows x tokens for one call");
   p.q = static_cast<const uint16_t*>(a->q);
   p.out = static_cast<uint16_t*>(a->out);
   p.q_st = a->q_st, p.q_sh = a->q_sh, p.o_st = a->o_st, p.o_sh = a->o_sh;
@@ -713,7 +728,8 @@ extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t w
   p.sl2 = static_cast<float>(static_cast<double>(a->scale) * 1.4426950408889634);
   p.status = device_status_word();
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.record = reinterpret_cast<int4*>(ws + x.record);
+  p.count = counters;
+  p.most = static_cast<int>(x.w);
   p.part = reinterpret_cast<float*>(ws + x.part);
   CUtensorMap mk, mv;
   if (int e = kv_maps(&mk, &mv, p.c, a->D)) return e;
@@ -734,21 +750,17 @@ extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t w
     p.pre_o = reinterpret_cast<float*>(ws + x.pre_o);
     p.pre_kt = static_cast<int>(x.pre_kt);
     p.pre_bm = 8 * x.pre_nt;
-    p.pre_w = a->heads * ((a->T * a->group + p.pre_bm - 1) / p.pre_bm) * x.pre_kt;
-    p.pre_g = static_cast<int>(x.pre_grid);
+    p.pre_run = static_cast<int>(x.pre_run);
     // the prefix is one sequence whose rows are all rows of the call
     KvAttnParams q = p;
     q.r = KvRows{a->prefix_table, nullptr, nullptr, a->prefix_pages, 1, static_cast<int>(a->prefix_pages), static_cast<int>(a->T),
                  static_cast<int>(a->prefix)};
     q.causal = 0;
+    q.most = static_cast<int>(x.pre_w);
     if (int e = launch(std::integral_constant<int, MODE_PREFIX>(), q, x.pre_grid, x.pre_nt)) return e;
     if (int e = launch(std::integral_constant<int, MODE_OWN>(), p, x.grid, x.nt)) return e;
   } else if (int e = launch(std::integral_constant<int, MODE_PLAIN>(), p, x.grid, x.nt)) {
     return e;
   }
-  if (x.kt == 1 || x.grid == 1) return 0;   // no unit can be cut
-  return by_size(x.nt, [&](auto d, auto n) {
-    constexpr int DD = decltype(d)::value, N = decltype(n)::value;
-    return check_cuda(launch_chained(kv_join_kernel<DD, N>, dim3(static_cast<unsigned>(x.grid - 1)), 2 * DD * N, 0, stream, 1, p), "kv_join launch");
-  });
+  return 0;
 }

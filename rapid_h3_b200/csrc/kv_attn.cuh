@@ -23,21 +23,22 @@ struct KvAttnParams {
   int is_f16;
   int group;          // query heads per KV head
   int causal;
+  int most;           // bound of the tiles of the pass
   float sl2;          // softmax scale * log2 e
   int* status;
-  // partial results of units that more than one CTA works on: two slots per CTA, and one record per CTA
-  float* part;        // [grid][2][BM * D + 2 * BM]: O in fragment order, m, l
-  int4* record;       // [grid][2]: {b, h, u, kt}, {k0, W low, W high, G}; b < 0: the CTA does not begin inside a unit
+  // partial results of units that more than one CTA works on: two slots per CTA (0: of the unit its run begins inside of, 1: of the unit
+  // its run ends inside of)
+  float* part;              // [grid][2][BM * D + 2 * BM]: O in fragment order, m, l
+  int* count;               // [grid] parts written of the unit in a CTA's slot 1; all 0 between calls
   // shared prefix. Its pass writes every unit's parts row by row; the pass over the own keys takes them in.
   //   pre_o [split][heads][rows][D], pre_ml [split][heads][rows][2], rows = T * group
   float* pre_o;
   float* pre_ml;
-  long long pre_w;    // tiles and CTAs of the prefix pass, tiles of one of its units, rows of its units: which splits exist
-  int pre_g, pre_kt, pre_bm;
+  int pre_run, pre_kt, pre_bm;  // the prefix pass: tiles of a CTA, tiles of a unit, rows of a unit
 };
 
-// the CTA whose run [W * c / G, W * (c + 1) / G) holds tile x
-__device__ __forceinline__ int kv_owner(long long x, long long W, int G) { return static_cast<int>(((x + 1) * G - 1) / W); }
+// The slot of part i of a unit whose first tile is CTA `first`'s
+__device__ __forceinline__ int64_t kv_slot(int first, int i) { return i == 0 ? 2ll * first + 1 : 2ll * (first + i); }
 
 __device__ __forceinline__ float kv_ex2(float x) {
   float y;

@@ -75,11 +75,12 @@ __device__ __forceinline__ int64_t kv_place(const KvCache& c, const KvRows& r, i
 // The rows of a sequence are its new tokens x the query heads of one KV head ("group"): row = token * group + head. A unit is
 // BM such rows of one sequence and KV head against all of its keys, in tiles of TK keys; every unit has at least one tile, so that rows
 // without a key are written too. The tiles of all units, in the order (sequence, head, row tile, key tile), are dealt to the CTAs
-// in equal runs [W * c / G, W * (c + 1) / G): a CTA's run begins and ends anywhere inside a unit.
+// in runs of `run` = W / grid, rounded up: a CTA's run begins and ends anywhere inside a unit. The entry knows a bound `most` below 2^31
+// of W; more than that comes of starts that are not ascending, and nothing is done then.
 struct KvSeq {
   int first, n, len;  // first row token of the call, new tokens, cached tokens
   int qt, kt;         // row tiles, key tiles of a unit
-  __device__ __forceinline__ long long tiles(int heads) const { return static_cast<long long>(heads) * qt * kt; }
+  __device__ __forceinline__ int tiles(int heads) const { return heads * qt * kt; }
 };
 template <int BM, int TK>
 __device__ __forceinline__ KvSeq kv_seq(const KvRows& r, int page_log2, int group, int b) {
@@ -89,90 +90,88 @@ __device__ __forceinline__ KvSeq kv_seq(const KvRows& r, int page_log2, int grou
   s.n = hi - lo;
   const long long room = static_cast<long long>(r.per_seq) << page_log2;
   s.len = static_cast<int>(min(static_cast<long long>(r.fixed_len ? r.fixed_len : max(r.lens[b], 0)), room));
-  s.qt = static_cast<int>((static_cast<long long>(s.n) * group + BM - 1) / BM);
+  s.qt = (s.n * group + BM - 1) / BM;
   s.kt = max(1, (s.len - 1 + TK) / TK);
   return s;
 }
-// What a CTA needs to begin: its run and the sequence it begins in. Filled by the whole block (a scan over the sequences).
 struct KvRun {
-  long long x0, x1;   // the CTA's tiles
-  long long xb;       // first tile of sequence b
-  long long W;
-  int b, G;           // sequence that x0 lies in; CTAs that have a run
+  int x0, x1;   // the CTA's tiles
+  int run;      // tiles of a CTA: x belongs to CTA x / run
+  int b, xb;    // the sequence that x0 lies in and its first tile
 };
-template <int BM, int TK, int NT>
-__device__ __forceinline__ void kv_find_run(const KvRows& r, int page_log2, int heads, int group, long long* scan /* NT/32 */,
-                                            KvRun* run) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (r.B + NT - 1) / NT;
-  const int b0 = min(r.B, tid * per), b1 = min(r.B, b0 + per);
-  long long own = 0;
-  for (int b = b0; b < b1; ++b) own += kv_seq<BM, TK>(r, page_log2, group, b).tiles(heads);
-  long long incl = own;
+// Every warp scans the sequences by itself (they are in L1 after the first): no barrier, one round of loads up to 32 sequences.
+template <int BM, int TK>
+__device__ __forceinline__ KvRun kv_find_run(const KvRows& r, int page_log2, int heads, int group, int most, int* status) {
+  const int lane = threadIdx.x & 31;
+  const int per = (r.B + 31) >> 5;
+  const int b0 = min(r.B, lane * per), b1 = min(r.B, b0 + per);
+  long long sum = 0;
+  for (int b = b0; b < b1; ++b) {
+    const KvSeq s = kv_seq<BM, TK>(r, page_log2, group, b);
+    sum += static_cast<long long>(heads) * s.qt * s.kt;
+  }
+  int own = static_cast<int>(min(sum, static_cast<long long>(most) + 1));
+  if (__any_sync(0xffffffffu, own > most)) own = lane == 0 ? most + 1 : 0;
+  long long total = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += up;
+    const long long up = __shfl_up_sync(0xffffffffu, total, o);
+    if (lane >= o) total += up;
   }
-  if (lane == 31) scan[warp] = incl;
-  __syncthreads();
-  long long before = 0, W = 0;
-#pragma unroll
-  for (int i = 0; i < NT / 32; ++i) {
-    if (i < warp) before += scan[i];
-    W += scan[i];
+  const long long all = __shfl_sync(0xffffffffu, total, 31);
+  if (all > most) {
+    if (threadIdx.x == 0) kv_report(status, ST_KV_BAD_STARTS);
+    own = 0, total = 0;
   }
-  incl += before;
-  const long long excl = incl - own;
-  const int G = static_cast<int>(min(static_cast<long long>(gridDim.x), W));
-  const long long c = blockIdx.x;
-  const long long x0 = c < G ? W * c / G : W, x1 = c < G ? W * (c + 1) / G : W;
-  if (tid == 0) {
-    run->x0 = x0, run->x1 = x1, run->W = W, run->G = G;
-    run->b = r.B, run->xb = W;
-  }
-  __syncthreads();
-  if (x0 < x1 && excl <= x0 && x0 < incl) {
-    long long xb = excl;
-    int b = b0;
+  const int incl = static_cast<int>(total), W = all > most ? 0 : static_cast<int>(all);
+  KvRun run;
+  run.run = max(1u, (static_cast<unsigned>(W) + gridDim.x - 1) / gridDim.x);
+  run.x0 = static_cast<int>(min(static_cast<long long>(W), static_cast<long long>(run.run) * blockIdx.x));
+  run.x1 = min(W - run.x0, run.run) + run.x0;
+  int xb = incl - own, b = b0;
+  const bool mine = run.x0 < run.x1 && xb <= run.x0 && run.x0 < incl;
+  if (mine && per > 1) {
     for (; b < b1; ++b) {
-      const long long w = kv_seq<BM, TK>(r, page_log2, group, b).tiles(heads);
-      if (x0 < xb + w) break;
+      const int w = kv_seq<BM, TK>(r, page_log2, group, b).tiles(heads);
+      if (run.x0 - xb < w) break;
       xb += w;
     }
-    run->b = b, run->xb = xb;
   }
-  __syncthreads();
+  const uint32_t who = __ballot_sync(0xffffffffu, mine);
+  run.b = __shfl_sync(0xffffffffu, b, who ? __ffs(who) - 1 : 0);
+  run.xb = __shfl_sync(0xffffffffu, xb, who ? __ffs(who) - 1 : 0);
+  return run;
 }
 // One unit's part of a CTA's run
 struct KvSegment {
   KvSeq s;
   int b, h, u;        // sequence, KV head, row tile
   int k0, k1;         // key tiles [k0, k1) of the unit's s.kt
+  int x;              // the unit's first tile
 };
 // Steps through a run; next() gives the segment at x and moves on.
 template <int BM, int TK>
 struct KvWalk {
-  long long x, x1, xb;
-  int b;
+  int x, x1, xb, b;
   KvSeq s;
   bool have;
   __device__ __forceinline__ KvWalk(const KvRun& run) : x(run.x0), x1(run.x1), xb(run.xb), b(run.b), have(false) {}
   __device__ __forceinline__ bool next(const KvRows& r, int page_log2, int heads, int group, KvSegment& g) {
     if (x >= x1) return false;
     if (!have) s = kv_seq<BM, TK>(r, page_log2, group, b), have = true;
-    while (x >= xb + s.tiles(heads)) {  // ends: the tiles of the sequences from b on reach beyond x < x1 <= W
+    while (x - xb >= s.tiles(heads)) {  // ends: the tiles of the sequences from b on reach beyond x < x1 <= W
       if (b + 1 >= r.B) return false;
       xb += s.tiles(heads);
       s = kv_seq<BM, TK>(r, page_log2, group, ++b);
     }
-    const long long rem = x - xb;
-    const long long unit = rem / s.kt;
+    const unsigned rem = x - xb;
+    const unsigned unit = rem / static_cast<unsigned>(s.kt);
     g.s = s, g.b = b;
-    g.k0 = static_cast<int>(rem - unit * s.kt);
-    g.h = static_cast<int>(unit / s.qt);
-    g.u = static_cast<int>(unit - static_cast<long long>(g.h) * s.qt);
-    g.k1 = static_cast<int>(min(static_cast<long long>(s.kt), g.k0 + (x1 - x)));
+    g.k0 = rem - unit * s.kt;
+    g.x = x - g.k0;
+    g.h = unit / static_cast<unsigned>(s.qt);
+    g.u = unit - static_cast<unsigned>(g.h) * s.qt;
+    g.k1 = min(s.kt, g.k0 + (x1 - x));
     x += g.k1 - g.k0;
     return true;
   }
@@ -181,7 +180,7 @@ struct KvWalk {
 template <int BM>
 __device__ __forceinline__ int kv_visible(const KvSeq& s, int group, int u, bool causal) {
   if (!causal) return s.len;
-  const int last = static_cast<int>((min(static_cast<long long>(u + 1) * BM, static_cast<long long>(s.n) * group) - 1) / group);
+  const int last = (min((u + 1) * BM, s.n * group) - 1) / group;
   return max(0, min(s.len, s.len - s.n + last + 1));
 }
 

@@ -94,6 +94,21 @@ class Rows:
                                            starts.data_ptr(), len(lens)))
 
 
+# counters of the attention kernels, per (device, stream): 0 between calls, so only calls that cannot overlap share them
+_COUNTERS = {}
+
+
+def _counters(device, stream):
+    """Zeros on `device` that no call uses at the same time as one on `stream`. A captured call gets its own, cleared by the graph: a
+    graph may be replayed on any stream."""
+    if torch._C._cuda_isCurrentStreamCapturing():
+        return torch.zeros(1024, device=device, dtype=torch.int32)
+    t = _COUNTERS.get((device.index, stream))
+    if t is None:
+        t = _COUNTERS.setdefault((device.index, stream), torch.zeros(1024, device=device, dtype=torch.int32))
+    return t
+
+
 class _on:
     """The device a call's work goes to; entering it costs nothing where it is the current one."""
 
@@ -183,7 +198,8 @@ def _attend(q, cache, rows, prefix, prefix_len, scale, causal, out):
         args = _ARGS.pack(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), *cache._args, table, stride,
                           per_seq, lens, starts, batch, t, group, prefix.data_ptr() if prefix is not None else 0,
                           prefix.numel() if prefix is not None else 0, prefix_len, scale, cache.kind, _DTYPES[q.dtype], bool(causal))
-        _lib.call("rh3_kv_attn", args, work.data_ptr(), need, _lib.stream())
+        stream = _lib.stream()
+        _lib.call("rh3_kv_attn", args, work.data_ptr(), need, _counters(q.device, stream).data_ptr(), stream)
     return out
 
 

@@ -54,19 +54,20 @@ def test_read_refuses(change, said):
     (dict(q=0), b"16-byte"), (dict(q_st=4), b"16-byte"), (dict(o_sh=129), b"16-byte"), (dict(out=P + 2), b"16-byte"), (dict(), b"workspace")])
 def test_attention_refuses(change, said):
     lib = _lib.lib()
-    assert lib.rh3_kv_attn(attn_args(**change), None, 0, None) < 0 and said in lib.rh3_last_error_string()
+    assert lib.rh3_kv_attn(attn_args(**change), None, 0, P, None) < 0 and said in lib.rh3_last_error_string()
     if not change:
         need = lib.rh3_kv_attn_workspace_bytes(2, 4, 64, 128, 4, 2, 3, 0)
         assert need > 0
-        assert lib.rh3_kv_attn(attn_args(), P, need - 1, None) < 0 and said in lib.rh3_last_error_string()
-        assert lib.rh3_kv_attn(attn_args(), P + 16, need, None) < 0 and said in lib.rh3_last_error_string()
-        assert lib.rh3_kv_attn(None, P, need, None) < 0
+        assert lib.rh3_kv_attn(attn_args(), P, need - 1, P, None) < 0 and said in lib.rh3_last_error_string()
+        assert lib.rh3_kv_attn(attn_args(), P + 16, need, P, None) < 0 and said in lib.rh3_last_error_string()
+        assert lib.rh3_kv_attn(attn_args(), P, need, None, None) < 0 and b"counters" in lib.rh3_last_error_string()
+        assert lib.rh3_kv_attn(None, P, need, P, None) < 0
 
 
 def test_calls_without_rows_do_nothing():
     lib = _lib.lib()
     assert lib.rh3_kv_write(*write_args(T=0, k=0, v=0)) == 0 and lib.rh3_kv_read(*read_args(T=0, k=0, v=0)) == 0
-    assert lib.rh3_kv_attn(attn_args(T=0, q=0, out=0), None, 0, None) == 0
+    assert lib.rh3_kv_attn(attn_args(T=0, q=0, out=0), None, 0, None, None) == 0
 
 
 def test_there_is_no_cpu_path():
@@ -80,46 +81,46 @@ def test_there_is_no_cpu_path():
         kv_cache.alloc(1, 1, kind="int4", device="cpu")
 
 
-def owner(x, w, g):
-    return ((x + 1) * g - 1) // w
-
-
 def test_every_tile_has_one_owner_and_every_cut_unit_is_joined_once():
-    """The device's arithmetic (runs, slots, records, the join's walk), restated: units of any sizes dealt to any grid."""
+    """The device's arithmetic (runs, slots, parts), restated: units of any sizes dealt to any grid."""
     rng = random.Random(1)
     for _ in range(400):
         units = [rng.choice([1, 1, 2, 5, rng.randint(1, 300)]) for _ in range(rng.randint(1, 60))]
-        grid = rng.choice([1, 2, 7, 296, rng.randint(1, 400)])
+        grid = rng.choice([1, 2, 7, 148, rng.randint(1, 400)])
         w = sum(units)
-        g = min(grid, w)
+        run = -(-w // grid)
         first = [sum(units[:i]) for i in range(len(units))]
-        slots, record, whole = {}, {}, set()
-        for c in range(g):
-            x, x1 = w * c // g, w * (c + 1) // g
-            assert x < x1
-            begins = True
+        slots, whole, counters = {}, set(), {}
+        for c in range(grid):
+            x, x1 = min(w, c * run), min(w, (c + 1) * run)
             while x < x1:
                 u = bisect.bisect_right(first, x) - 1
                 k0 = x - first[u]
                 k1 = min(units[u], k0 + x1 - x)
-                assert owner(x, w, g) == c
-                if begins:
-                    record[c], begins = (u if k0 else -1, k0), False
                 if k0 == 0 and k1 == units[u]:
                     whole.add(u)
                 else:
                     assert (c, k0 == 0) not in slots
                     slots[c, k0 == 0] = u, k0, k1
+                    counters.setdefault(first[u] // run, set()).add(u)   # the word a cut unit's parts are counted in
                 x += k1 - k0
-        joined = set()
-        for c in range(1, g):
-            u, k0 = record[c]
-            xs = w * c // g - k0
-            if u < 0 or w * (c - 1) // g > xs:
-                continue
-            n = owner(xs + units[u] - 1, w, g) - c + 2
-            parts = [slots[c - 1, True]] + [slots[c + i, False] for i in range(n - 1)]
-            assert all(p[0] == u for p in parts) and parts[0][1] == 0 and parts[-1][2] == units[u]
-            assert all(a[2] == b[1] for a, b in zip(parts, parts[1:])) and u not in joined
-            joined.add(u)
-        assert joined | whole == set(range(len(units))) and not joined & whole
+        assert all(len(v) == 1 and c < grid for c, v in counters.items())
+        cut = set()
+        for u in range(len(units)):
+            c, n = first[u] // run, (first[u] + units[u] - 1) // run - first[u] // run + 1
+            if n > 1:
+                parts = [slots[c, True]] + [slots[c + i, False] for i in range(1, n)]
+                assert all(p[0] == u for p in parts) and parts[0][1] == 0 and parts[-1][2] == units[u]
+                assert all(a[2] == b[1] for a, b in zip(parts, parts[1:]))
+                cut.add(u)
+        assert cut | whole == set(range(len(units))) and not cut & whole and len(slots) == sum(1 for s in slots)
+
+
+def test_a_prefix_falls_into_as_many_parts_as_the_workspace_holds():
+    rng = random.Random(2)
+    for _ in range(2000):
+        units, kt = rng.randint(1, 400), rng.randint(1, 300)
+        grid = min(rng.choice([148, 132]), units * kt)
+        run = -(-units * kt // grid)
+        room = min((kt - 1) // run + 2, kt)
+        assert all((u * kt + kt - 1) // run - u * kt // run + 1 <= room for u in range(units))
