@@ -26,6 +26,8 @@ namespace rh3 {
 namespace {
 
 constexpr int TK = 128;                 // keys of a tile
+// Rows of a sequence (new tokens x query heads of a KV head), on average, above which the 128-row tiles of kv_attn_wide.cu take a call
+constexpr int64_t KV_WIDE_FROM = 16;
 constexpr int KV_WARPS = 4;             // computing warps
 constexpr int KV_NT = KV_WARPS * 32 + 32;
 enum { MODE_PLAIN = 0, MODE_PREFIX = 1, MODE_OWN = 2 };
@@ -124,12 +126,6 @@ template <int BM>
 __device__ __forceinline__ int kv_last_tile(const KvAttnParams& p, const KvSegment& g) {
   return max(g.k0 + 1, min(g.k1, (kv_visible<BM>(g.s, p.group, g.u, p.causal) + TK - 1) / TK));
 }
-__device__ __forceinline__ float2 kv_unpack(uint32_t w, int is_f16) {
-  if (is_f16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
-  return make_float2(bf16_lo(w), bf16_hi(w));
-}
-__device__ __forceinline__ uint32_t kv_pack(float a, float b, int is_f16) { return is_f16 ? pack_half2(a, b) : pack_bf16x2(a, b); }
-
 // Joins the parts of a cut unit: slot 1 of CTA `first`, slot 0 of the ones behind it, in that order. They are
 // brought into the ring (which is done with) by bulk copies, as many as it holds at a time, and every thread sums its own fragments'
 // values in rolled loops: the code runs once, its instructions come from L2.
@@ -651,38 +647,45 @@ int kv_launch(const CUtensorMap& mk, const CUtensorMap& mv, const KvAttnParams& 
   return check_cuda(launch_chained(kern, dim3(static_cast<unsigned>(grid)), KV_NT, smem, stream, 1, mk, mv, p), "kv_attn launch");
 }
 
-// The plan of a call: rows per unit, grids and the pieces of its workspace
+// The plan of a call: which kernel and rows per unit, grids and the pieces of its workspace.
+struct KvPass {
+  int nt;                       // narrow: units of 8 * nt rows; 0: wide, units of 256
+  int64_t bm, kt, w, grid;      // rows of a unit, key tiles of a unit and tiles of the pass at most, CTAs
+};
+KvPass kv_pass(int64_t heads, int64_t rows, int64_t seqs, int64_t kt) {
+  KvPass x{};
+  x.nt = rows > KV_WIDE_FROM * seqs ? 0 : rows <= 8 * seqs ? 1 : 2;
+  x.bm = x.nt ? 8 * x.nt : KV_WIDE_BM;
+  x.kt = kt < 1 ? 1 : kt;
+  const int64_t units = heads * (rows / x.bm + seqs);
+  x.w = units * x.kt;
+  x.grid = kv_grid(units, x.kt, x.nt == 0 ? 1 : x.nt == 1 ? 3 : 2);
+  return x;
+}
 struct KvPlan {
-  int nt, pre_nt;                                   // units of 8 * nt rows in the own pass and in the prefix pass
-  int64_t kt, w, grid;                              // key tiles of a sequence and tiles of the call at most, CTAs
-  int64_t pre_kt, pre_w, pre_run, pre_grid, pre_splits;   // the prefix pass: also tiles of a CTA, and into how many parts a unit may fall
-  int64_t part, pre_ml, pre_o, bytes;       // byte offsets
+  KvPass own, pre;              // pre.grid = 0: no pass of its own for the prefix (none, or its tiles are among the wide units' own)
+  int64_t pre_run, pre_splits;  // tiles of a CTA of the prefix pass, into how many parts its units may fall
+  int64_t part, pre_ml, pre_o, bytes;   // byte offsets
 };
 KvPlan kv_plan(int64_t heads, int64_t group, int64_t page, int64_t D, int64_t per_seq, int64_t B, int64_t T, int64_t prefix) {
   KvPlan x{};
-  const int64_t rows = T * group;
+  const int64_t rows = T * group, pre_kt = (prefix + TK - 1) / TK, own_kt = (per_seq * page + TK - 1) / TK, seqs = B < T ? B : T;
   auto take = [&](int64_t bytes) {
     const int64_t at = x.bytes;
     x.bytes += (bytes + 255) / 256 * 256;
     return at;
   };
-  x.nt = rows <= 8 * B ? 1 : 2;   // 8 rows a sequence on average fill a unit of 8
-  x.kt = (per_seq * page + TK - 1) / TK;
-  if (x.kt < 1) x.kt = 1;
-  const int64_t units = heads * (rows / (8 * x.nt) + (B < T ? B : T));
-  x.w = units * x.kt;
-  x.grid = kv_grid(units, x.kt, x.nt == 1 ? 3 : 2);
-  x.part = take(x.grid * 2 * (8 * x.nt * D + 16 * x.nt) * sizeof(float));
-  if (prefix > 0) {
-    x.pre_nt = rows <= 8 ? 1 : 2;
-    const int64_t bm = 8 * x.pre_nt, units = heads * ((rows + bm - 1) / bm);
-    x.pre_kt = (prefix + TK - 1) / TK;
-    x.pre_w = units * x.pre_kt;
-    const int64_t grid = kv_grid(units, x.pre_kt, x.pre_nt == 1 ? 3 : 2);
-    x.pre_run = (x.pre_w + grid - 1) / grid;
-    x.pre_grid = (x.pre_w + x.pre_run - 1) / x.pre_run;
-    x.pre_splits = (x.pre_kt - 1) / x.pre_run + 2;
-    if (x.pre_splits > x.pre_kt) x.pre_splits = x.pre_kt;
+  x.own = kv_pass(heads, rows, seqs, own_kt);
+  if (x.own.nt == 0) x.own = kv_pass(heads, rows, seqs, own_kt + pre_kt);
+  x.part = take(x.own.grid * 2 * (x.own.nt ? x.own.bm * D + 2 * x.own.bm : kv_wide_part_floats(D)) * sizeof(float));
+  if (prefix > 0 && x.own.nt) {
+    x.pre = kv_pass(heads, rows, 1, pre_kt);
+    const int64_t units = heads * ((rows + x.pre.bm - 1) / x.pre.bm);
+    x.pre.w = units * pre_kt;
+    x.pre.grid = kv_grid(units, pre_kt, x.pre.nt == 0 ? 1 : x.pre.nt == 1 ? 3 : 2);
+    x.pre_run = (x.pre.w + x.pre.grid - 1) / x.pre.grid;
+    x.pre_splits = (pre_kt - 1) / x.pre_run + 2;
+    if (x.pre_splits > pre_kt) x.pre_splits = pre_kt;
     x.pre_ml = take(x.pre_splits * heads * rows * 2 * sizeof(float));
     x.pre_o = take(x.pre_splits * heads * rows * D * sizeof(float));
   }
@@ -717,8 +720,8 @@ extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t w
   const KvPlan x = kv_plan(a->heads, a->group, a->page, a->D, a->per_seq, a->B, a->T, a->prefix);
   RH3_CHECK_ARG(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= x.bytes,
                 "kv_attn: a workspace of %lld bytes, 256-byte aligned, is needed", (long long)x.bytes);
-  RH3_CHECK_ARG(counters && x.grid <= RH3_KV_COUNTERS, "kv_attn: the counters are missing, or too few for the device");
-  RH3_CHECK_ARG(x.w < (1ll << 31) && x.pre_w < (1ll << 31), "kv_attn: too many rows x tokens for one call");
+  RH3_CHECK_ARG(counters && x.own.grid <= RH3_KV_COUNTERS, "kv_attn: the counters are missing, or too few for the device");
+  RH3_CHECK_ARG(x.own.w < (1ll << 31) && x.pre.w < (1ll << 31), "kv_attn: too many rows x tokens for one call");
   p.q = static_cast<const uint16_t*>(a->q);
   p.out = static_cast<uint16_t*>(a->out);
   p.q_st = a->q_st, p.q_sh = a->q_sh, p.o_st = a->o_st, p.o_sh = a->o_sh;
@@ -729,38 +732,39 @@ extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t w
   p.status = device_status_word();
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.count = counters;
-  p.most = static_cast<int>(x.w);
+  p.most = static_cast<int>(x.own.w);
   p.part = reinterpret_cast<float*>(ws + x.part);
+  if (x.own.nt == 0) {
+    p.r.pre_tiles = static_cast<int>((a->prefix + TK - 1) / TK);
+    p.pre_table = a->prefix_table;
+    p.pre_len = static_cast<int>(a->prefix);
+    return kv_wide_launch(p, a->D, a->kind, false, x.own.grid, stream);
+  }
   CUtensorMap mk, mv;
   if (int e = kv_maps(&mk, &mv, p.c, a->D)) return e;
-
-  // fn(D, NT) as compile-time constants
-  auto by_size = [&](int nt, auto&& fn) {
-    if (a->D == 128) return nt == 1 ? fn(std::integral_constant<int, 128>(), std::integral_constant<int, 1>()) : fn(std::integral_constant<int, 128>(), std::integral_constant<int, 2>());
-    return nt == 1 ? fn(std::integral_constant<int, 64>(), std::integral_constant<int, 1>()) : fn(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+  auto launch = [&](auto mode, const KvAttnParams& q, const KvPass& pass) {
+    constexpr int M = decltype(mode)::value;
+    auto by_kind = [&](auto d, auto n) {
+      constexpr int DD = decltype(d)::value, N = decltype(n)::value;
+      return a->kind == RH3_KIND_I8 ? kv_launch<DD, RH3_KIND_I8, M, N>(mk, mv, q, pass.grid, stream) : kv_launch<DD, RH3_KIND_F8, M, N>(mk, mv, q, pass.grid, stream);
+    };
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    if (a->D == 128) return pass.nt == 1 ? by_kind(std::integral_constant<int, 128>(), One()) : by_kind(std::integral_constant<int, 128>(), Two());
+    return pass.nt == 1 ? by_kind(std::integral_constant<int, 64>(), One()) : by_kind(std::integral_constant<int, 64>(), Two());
   };
-  auto launch = [&](auto mode, const KvAttnParams& q, int64_t grid, int nt) {
-    return by_size(nt, [&](auto d, auto n) {
-      constexpr int M = decltype(mode)::value, DD = decltype(d)::value, N = decltype(n)::value;
-      return a->kind == RH3_KIND_I8 ? kv_launch<DD, RH3_KIND_I8, M, N>(mk, mv, q, grid, stream) : kv_launch<DD, RH3_KIND_F8, M, N>(mk, mv, q, grid, stream);
-    });
-  };
-  if (a->prefix > 0) {
-    p.pre_ml = reinterpret_cast<float*>(ws + x.pre_ml);
-    p.pre_o = reinterpret_cast<float*>(ws + x.pre_o);
-    p.pre_kt = static_cast<int>(x.pre_kt);
-    p.pre_bm = 8 * x.pre_nt;
-    p.pre_run = static_cast<int>(x.pre_run);
-    // the prefix is one sequence whose rows are all rows of the call
-    KvAttnParams q = p;
-    q.r = KvRows{a->prefix_table, nullptr, nullptr, a->prefix_pages, 1, static_cast<int>(a->prefix_pages), static_cast<int>(a->T),
-                 static_cast<int>(a->prefix)};
-    q.causal = 0;
-    q.most = static_cast<int>(x.pre_w);
-    if (int e = launch(std::integral_constant<int, MODE_PREFIX>(), q, x.pre_grid, x.pre_nt)) return e;
-    if (int e = launch(std::integral_constant<int, MODE_OWN>(), p, x.grid, x.nt)) return e;
-  } else if (int e = launch(std::integral_constant<int, MODE_PLAIN>(), p, x.grid, x.nt)) {
-    return e;
-  }
-  return 0;
+  if (a->prefix == 0) return launch(std::integral_constant<int, MODE_PLAIN>(), p, x.own);
+  p.pre_ml = reinterpret_cast<float*>(ws + x.pre_ml);
+  p.pre_o = reinterpret_cast<float*>(ws + x.pre_o);
+  p.pre_kt = static_cast<int>(x.pre.kt);
+  p.pre_bm = static_cast<int>(x.pre.bm);
+  p.pre_run = static_cast<int>(x.pre_run);
+  // the prefix is one sequence whose rows are all rows of the call
+  KvAttnParams q = p;
+  q.r = KvRows{a->prefix_table, nullptr, nullptr, a->prefix_pages, 1, static_cast<int>(a->prefix_pages), static_cast<int>(a->T),
+               static_cast<int>(a->prefix), 0};
+  q.causal = 0;
+  q.most = static_cast<int>(x.pre.w);
+  if (int e = x.pre.nt == 0 ? kv_wide_launch(q, a->D, a->kind, true, x.pre.grid, stream) : launch(std::integral_constant<int, MODE_PREFIX>(), q, x.pre)) return e;
+  return launch(std::integral_constant<int, MODE_OWN>(), p, x.own);
 }

@@ -35,6 +35,9 @@ struct KvAttnParams {
   float* pre_o;
   float* pre_ml;
   int pre_run, pre_kt, pre_bm;  // the prefix pass: tiles of a CTA, tiles of a unit, rows of a unit
+  // shared prefix in the wide kernel's single pass: r.pre_tiles tiles of it before a unit's own
+  const int* pre_table;
+  int pre_len;
 };
 
 // The slot of part i of a unit whose first tile is CTA `first`'s
@@ -87,5 +90,16 @@ __device__ __forceinline__ void kv_codes_to_half(uint32_t w, uint32_t& a, uint32
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(b) : "h"(static_cast<uint16_t>(w >> 16)));
   }
 }
+
+__device__ __forceinline__ float2 kv_unpack(uint32_t w, int is_f16) {
+  if (is_f16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return make_float2(bf16_lo(w), bf16_hi(w));
+}
+__device__ __forceinline__ uint32_t kv_pack(float a, float b, int is_f16) { return is_f16 ? pack_half2(a, b) : pack_bf16x2(a, b); }
+
+// kv_attn_wide.cu: the same parameters, units of 256 rows; floats of one of its partial results
+constexpr int KV_WIDE_BM = 256;
+int64_t kv_wide_part_floats(int64_t D);
+int kv_wide_launch(const KvAttnParams& p, int64_t D, int kind, bool prefix, int64_t grid, cudaStream_t stream);
 
 }  // namespace rh3

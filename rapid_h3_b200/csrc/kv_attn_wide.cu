@@ -1,0 +1,614 @@
+// Attention of many rows per sequence (prompts, long continuations, the shared prefix of a batch) to the quantized paged cache, on
+// the tensor cores' 128-row tiles.
+//
+// A unit is 256 rows (new tokens x query heads of one KV head) of one sequence, two tiles of 128, against all of its keys; the key tiles
+// of all units are dealt to one CTA per SM in equal runs, as in kv_attn.cu, and parts of cut units are joined the same way. Behind a shared
+// prefix a unit's keys are the prefix's tiles and then its own (or, in the prefix's own pass, the prefix's alone).
+//
+//   S_g = Q_g . K^T   fp16 x fp16 -> fp32 in TMEM (tcgen05 kind::f16), K the codes as fp16, exactly
+//   u = (s * ks_j) * c_row + log2 vs_j, w = 2^(u - m + 7), l += w / vs_j   (kv_attn.cuh)
+//   O_g += W_g . V    W fp16 from TMEM (over S), V the codes as fp16; fp32 in TMEM
+// m is a row's maximum when it was last set: it is set anew, and O and l scaled, only when the maximum outgrows it by 2^8, so W stays
+// at most 2^15 and O is hardly ever touched between products (a tile of 128 columns read, scaled and written costs its softmax
+// warps more than their exponentials).
+//
+// 512 threads, one CTA per SM: warp 0 brings pages by bulk copies (codes as they lie), warp 1 issues the products, warps 4-11 are the softmax of
+// the two row tiles (one row per thread), warps 12-15 turn codes into fp16 tiles: rows of keys, 128-byte swizzle, slabs of 64 channels.
+// The same layout is K-major for K and, with the channels as the product's N, MN-major for V, so nothing is transposed.
+// Shared memory: Q 2 x 32 KB | three fp16 tiles of 32 KB (K and V in turn) | three raw tiles of 16 KB. TMEM: S0 | S1 | O0 | O1.
+// Bound, per step of 128 keys and 256 rows: 2,048 cycles of the tensor pipe, as many of the exponential unit, about 3,000 of shared memory (products'
+// operands 1,536, conversion 768, the keys' scales that every softmax warp reads 768).
+#include "kv_attn.cuh"
+
+namespace rh3 {
+namespace {
+
+constexpr int TK = 128, WBM = 256, WTHREADS = 512, SLOTS = 3, RAW = 3;
+
+template <int D>
+struct KvWide {
+  static constexpr int Q_BYTES = 128 * D * 2;       // a tile of 128 rows, fp16
+  static constexpr int T_BYTES = TK * D * 2;        // a K or V tile, fp16
+  static constexpr int R_BYTES = TK * D;            // a K or V tile, codes
+  static constexpr int TILES = 2 * Q_BYTES;
+  static constexpr int RAWS = TILES + SLOTS * T_BYTES;
+  static constexpr int TAIL = RAWS + RAW * R_BYTES;
+  static constexpr int PART = WBM * D + 2 * WBM;    // floats of a partial result
+  static constexpr int O_COL = 256;                 // TMEM column of O of row tile 0
+};
+struct __align__(16) KvWideTail {
+  float scale[RAW][2][TK];        // as loaded with a K tile: of K, of V
+  float key[2][3][TK];            // per key of a tile, by the tile's parity: K scale, log2 and inverse of the V scale
+  uint64_t raw_full[RAW], raw_empty[RAW], full[SLOTS], empty[SLOTS];
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint32_t pages[RAW];
+  uint32_t tmem_base;
+  int abort_flag;
+  KvSegment join[2];
+  int first[2], parts[2];
+};
+template <int D>
+constexpr int kv_wide_smem() { return KvWide<D>::TAIL + static_cast<int>(sizeof(KvWideTail)) + 1024; }
+
+// as descriptor make_desc_k128, for an operand whose M or N runs along the 128-byte rows: 64-channel slabs `slab` bytes apart, groups
+// of 8 rows (the product's K) 1,024
+__device__ __forceinline__ uint64_t make_desc_mn128(uint32_t smem_addr, uint32_t slab) {
+  uint64_t d = make_desc_k128(smem_addr);
+  d &= ~(static_cast<uint64_t>(0x3FFF) << 16);
+  return d | static_cast<uint64_t>(slab >> 4) << 16;
+}
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ uint64_t pk2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void upk2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max_3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Registers: 128 a thread at launch; service 40, conversion 72, softmax 200 (128 * 40 + 128 * 72 + 256 * 200 = 512 * 128)
+static_assert(128 * 40 + 128 * 72 + 256 * 200 == WTHREADS * 128, "register pool must balance");
+
+constexpr float kSlack = 8.f;   // log2 of how far a row's maximum may outgrow m
+
+// after an abandoned wait: copies that are still on their way land before the CTA gives its shared memory back
+__device__ __forceinline__ void kv_wide_settle() {
+  for (int i = 0; i < 64; ++i) __nanosleep(1000);
+}
+
+// End of the tiles of a segment that are worked on (behind the last visible key they are not; one always is), row tiles that have rows.
+__device__ __forceinline__ int kv_wide_end(const KvAttnParams& p, const KvSegment& g) {
+  return max(g.k0 + 1, min(g.k1, p.r.pre_tiles + (kv_visible<WBM>(g.s, p.group, g.u, p.causal) + TK - 1) / TK));
+}
+__device__ __forceinline__ int kv_wide_row_tiles(const KvAttnParams& p, const KvSegment& g) { return g.s.n * p.group - g.u * WBM > 128 ? 2 : 1; }
+// where the keys of tile kt are
+struct KvTile {
+  const int* table;   // pages
+  int kt, len;        // tile and tokens of that table
+};
+__device__ __forceinline__ KvTile kv_wide_tile(const KvAttnParams& p, const KvSegment& g, int kt) {
+  if (kt < p.r.pre_tiles) return KvTile{p.pre_table, kt, p.pre_len};
+  return KvTile{p.r.table + g.b * p.r.table_stride, kt - p.r.pre_tiles, g.s.len};
+}
+
+template <int D, int FMT, bool PREFIX>
+__global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams p) {
+  using L = KvWide<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  KvWideTail* tail = reinterpret_cast<KvWideTail*>(smem + L::TAIL);
+  volatile int* abort_flag = &tail->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < RAW; ++i) mbar_init(&tail->raw_full[i], 1), mbar_init(&tail->raw_empty[i], 4);
+    for (int i = 0; i < SLOTS; ++i) mbar_init(&tail->full[i], 4), mbar_init(&tail->empty[i], 1);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&tail->q_full[g], 4);
+      mbar_init(&tail->s_full[g], 1);
+      mbar_init(&tail->p_full[g], 4);
+      mbar_init(&tail->o_full[g], 1);
+      tail->parts[g] = 0;
+    }
+    tail->abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&tail->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  grid_dependency_begin();
+  const uint32_t tmem_base = tail->tmem_base;
+  const KvRun run = kv_find_run<WBM, TK>(p.r, p.c.page_log2, p.c.heads, p.group, p.most, p.status);
+  KvWalk<WBM, TK> walk(run);
+  KvSegment g;
+  auto all_ok = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0) {
+      // ------------------------------ producer: raw tiles K, V, K, V ... ------------------------------
+      const int page = 1 << p.c.page_log2, tile_pages = TK >> p.c.page_log2;
+      unsigned i = 0;
+      bool ok = true;
+      while (ok && walk.next(p.r, p.c.page_log2, p.c.heads, p.group, g)) {
+        const int kend = kv_wide_end(p, g);
+        for (int kt = g.k0; kt < kend && ok; ++kt) {
+          const KvTile t = kv_wide_tile(p, g, kt);
+          const int at = t.kt * tile_pages + lane;
+          const bool need = lane < tile_pages && (static_cast<int64_t>(at) << p.c.page_log2) < t.len;
+          const int id = need ? t.table[at] : -1;
+          const bool good = need && id >= 0 && id < p.c.pages;
+          if (need && !good) kv_report(p.status, ST_KV_BAD_PAGE);
+          const uint32_t mask = __ballot_sync(0xffffffffu, good);
+          const int64_t row = (static_cast<int64_t>(id) * p.c.heads + g.h) << p.c.page_log2;
+#pragma unroll 1
+          for (int v = 0; v < 2; ++v, ++i) {
+            const int s = i % RAW;
+            ok = all_ok(mbar_wait_relaxed(&tail->raw_empty[s], (i / RAW & 1) ^ 1, abort_flag, p.status, ST_TIMEOUT_STAGE_EMPTY, 64));
+            if (!ok) break;
+            if (lane == 0) {
+              tail->pages[s] = mask;
+              if (mask) mbar_arrive_expect_tx(&tail->raw_full[s], static_cast<uint32_t>(__popc(mask)) * page * (v ? D : D + 8));
+              else mbar_arrive(&tail->raw_full[s]);
+            }
+            __syncwarp();
+            if (good) {
+              bulk_load(smem + L::RAWS + s * L::R_BYTES + lane * page * D, (v ? p.c.v : p.c.k) + row * D, page * D, &tail->raw_full[s]);
+              if (!v) {
+                bulk_load(&tail->scale[s][0][lane * page], p.c.ks + row, page * 4, &tail->raw_full[s]);
+                bulk_load(&tail->scale[s][1][lane * page], p.c.vs + row, page * 4, &tail->raw_full[s]);
+              }
+            }
+            __syncwarp();
+          }
+        }
+      }
+    } else if (warp == 1) {
+      // ------------------------------ products ------------------------------
+      // The whole warp runs the loop converged; one elected lane issues.
+      constexpr uint32_t idesc_qk = make_idesc(1, 0, 0, 128, TK);
+      constexpr uint32_t idesc_pv = make_idesc(1, 0, 0, 128, D) | (1u << 16);   // B runs along N
+      unsigned i = 0, nq[2] = {0, 0}, np[2] = {0, 0};   // tiles taken; uses of q_full and p_full
+      bool ok = true;
+      auto wait_tile = [&](unsigned t) {
+        return all_ok(mbar_wait_relaxed(&tail->full[t % SLOTS], t / SLOTS & 1, abort_flag, p.status, ST_TIMEOUT_TMA_FULL, 32));
+      };
+      auto issue_qk = [&](int r, unsigned t, bool free_tile) {
+        const uint32_t q = smem_u32(smem + r * L::Q_BYTES), k = smem_u32(smem + L::TILES + t % SLOTS * L::T_BYTES);
+        if (elect_one()) {
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            mma4_f16_ss(tmem_base + r * 128, make_desc_k128(q + c * 128 * 128), make_desc_k128(k + c * TK * 128), idesc_qk, c);
+          mma_commit(&tail->s_full[r]);
+          if (free_tile) mma_commit(&tail->empty[t % SLOTS]);
+        }
+        __syncwarp();
+      };
+      while (ok && walk.next(p.r, p.c.page_log2, p.c.heads, p.group, g)) {
+        const int kend = kv_wide_end(p, g), tiles = kv_wide_row_tiles(p, g), n = kend - g.k0;
+        for (int r = 0; r < tiles && ok; ++r) {
+          ok = all_ok(mbar_wait_relaxed(&tail->q_full[r], nq[r]++ & 1, abort_flag, p.status, ST_TIMEOUT_TMA_FULL, 32));
+          if (ok && r == 0) ok = wait_tile(i);
+          if (!ok) break;
+          tc_fence_after();
+          issue_qk(r, i, r == tiles - 1);
+        }
+        for (int j = 0; j < n && ok; ++j, i += 2) {   // i: K of tile j, i + 1: V of it, i + 2: K of the next
+          for (int r = 0; r < tiles; ++r) {
+            if (r == 0) ok = wait_tile(i + 1);
+            ok = ok && all_ok(mbar_wait_relaxed(&tail->p_full[r], np[r]++ & 1, abort_flag, p.status, ST_TIMEOUT_P_READY, 32));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t v = smem_u32(smem + L::TILES + (i + 1) % SLOTS * L::T_BYTES);
+            if (elect_one()) {
+#pragma unroll
+              for (int c = 0; c < TK / 16; ++c)
+                mma_f16_ts(tmem_base + L::O_COL + r * D, tmem_base + r * 128 + c * 8, make_desc_mn128(v + c * 16 * 128, TK * 128), idesc_pv, j > 0 || c > 0);
+              if (r == tiles - 1) mma_commit(&tail->empty[(i + 1) % SLOTS]);
+              if (j == n - 1) mma_commit(&tail->o_full[r]);
+            }
+            __syncwarp();
+            if (j + 1 < n) {
+              if (r == 0) ok = wait_tile(i + 2);
+              if (!ok) break;
+              tc_fence_after();
+              issue_qk(r, i + 2, r == tiles - 1);
+            }
+          }
+        }
+      }
+    }
+  } else if (warp >= 12) {
+    // ============================ conversion: codes -> fp16 tiles ============================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    const int tid = threadIdx.x - 384;
+    constexpr int PER_ROW = D / 16, ROWS = 128 / PER_ROW;   // 16-code chunks of a row, rows of a round of all 128 threads
+    const int q = tid % PER_ROW, r0 = tid / PER_ROW;
+    unsigned i = 0;
+    int parity = 0;
+    bool ok = true;
+    while (ok && walk.next(p.r, p.c.page_log2, p.c.heads, p.group, g)) {
+      const int kend = kv_wide_end(p, g);
+      for (int kt = g.k0; kt < kend && ok; ++kt, parity ^= 1) {
+        const KvTile t = kv_wide_tile(p, g, kt);
+#pragma unroll 1
+        for (int v = 0; v < 2; ++v, ++i) {
+          const int s = i % RAW;
+          ok = all_ok(mbar_wait(&tail->raw_full[s], i / RAW & 1, abort_flag, p.status, ST_TIMEOUT_TMA_FULL) &&
+                      mbar_wait(&tail->empty[i % SLOTS], (i / SLOTS & 1) ^ 1, abort_flag, p.status, ST_TIMEOUT_STAGE_EMPTY));
+          if (!ok) break;
+          const uint32_t pages = tail->pages[s];
+          const bool whole = pages == (0xffffffffu >> (32 - (TK >> p.c.page_log2))) && t.kt * TK + TK <= t.len;
+          auto there = [&](int key) { return whole || (t.kt * TK + key < t.len && ((pages >> (key >> p.c.page_log2)) & 1u)); };
+          const uint8_t* raw = smem + L::RAWS + s * L::R_BYTES + r0 * D + q * 16;
+          uint8_t* out = smem + L::TILES + i % SLOTS * L::T_BYTES + (q / 4) * TK * 128;
+          const int swap = (q / 4) & 1;   // the two slabs' rows begin in the same banks: one writes its chunks in the other order
+#pragma unroll 4
+          for (int r = r0; r < TK; r += ROWS, raw += ROWS * D) {
+            uint4 w = *reinterpret_cast<const uint4*>(raw);
+            if (!there(r)) w = make_uint4(0, 0, 0, 0);   // may be anything: a NaN code times a weight of 0 is a NaN
+            uint4 a, b;
+            kv_codes_to_half<FMT>(w.x, a.x, a.y);
+            kv_codes_to_half<FMT>(w.y, a.z, a.w);
+            kv_codes_to_half<FMT>(w.z, b.x, b.y);
+            kv_codes_to_half<FMT>(w.w, b.z, b.w);
+            uint8_t* row = out + r * 128;
+            const int c = (q % 4) * 2;
+            *reinterpret_cast<uint4*>(row + (((c + swap) ^ (r & 7)) << 4)) = swap ? b : a;
+            *reinterpret_cast<uint4*>(row + (((c + 1 - swap) ^ (r & 7)) << 4)) = swap ? a : b;
+          }
+          if (v == 0) {
+            const bool is = there(tid);
+            const float vs = fmaxf(tail->scale[s][1][tid], kVsMin);
+            tail->key[parity][0][tid] = is ? tail->scale[s][0][tid] : 0.f;
+            tail->key[parity][1][tid] = is ? kv_lg2(vs) : -INFINITY;
+            tail->key[parity][2][tid] = is ? kv_rcp(vs) : 0.f;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&tail->full[i % SLOTS]);
+            mbar_arrive(&tail->raw_empty[s]);
+          }
+        }
+      }
+    }
+  } else {
+    // ============================ softmax: one row per thread ============================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    const int rt = (warp >> 2) - 1, quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t s_row = tmem_base + rt * 128 + lane_off, o_row = tmem_base + L::O_COL + rt * D + lane_off;
+    unsigned ns = 0, no = 0;   // uses of s_full and o_full
+    int parity = 0;
+    bool ok = true;
+    while (ok && walk.next(p.r, p.c.page_log2, p.c.heads, p.group, g)) {
+      const int kend = kv_wide_end(p, g), n = kend - g.k0;
+      if (rt >= kv_wide_row_tiles(p, g)) {   // no rows for this tile
+        parity ^= n & 1;
+        continue;
+      }
+      // ---- the row of Q as fp16 into its tile ----
+      const int flat = g.u * WBM + rt * 128 + row, tok = flat / p.group, hh = flat - tok * p.group;
+      const bool there = tok < g.s.n;
+      const int64_t t = g.s.first + tok, head = static_cast<int64_t>(g.h) * p.group + hh;
+      float c_row;
+      {
+        const uint16_t* src = p.q + t * p.q_st + head * p.q_sh;
+        uint4 x[D / 8];
+        float amax = 0.f, up, down;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          x[c] = there ? ld_global_16(src + c * 8) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          const uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = kv_unpack(w[k], p.is_f16);
+            amax = max_3(amax, fabsf(f.x), fabsf(f.y));
+          }
+        }
+        kv_row_factor(amax, up, down);
+        c_row = p.sl2 * down;
+        uint8_t* dst = smem + rt * L::Q_BYTES + row * 128;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = kv_unpack(w[k], p.is_f16);
+            w[k] = pack_half2(f.x * up, f.y * up);
+          }
+          *reinterpret_cast<uint4*>(dst + (c / 8) * 128 * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tail->q_full[rt]);
+      }
+      // the last own key the row sees, and the first one that some row of the warp does not
+      const int last = p.causal ? g.s.len - g.s.n + tok : g.s.len - 1;
+      const int warp_last = __shfl_sync(0xffffffffu, last, 0);
+      float m = -INFINITY;
+      uint64_t l2 = pk2(0.f, 0.f);
+      const uint64_t c2 = pk2(c_row, c_row);
+      for (int j = 0; j < n; ++j, parity ^= 1) {
+        // S is there, and so are the keys' scales: the product waited for the tile they came with
+        ok = all_ok(mbar_wait(&tail->s_full[rt], ns++ & 1, abort_flag, p.status, ST_TIMEOUT_ACC_FULL));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t r[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_row + c * 32, r[c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_wait_regs(r[c]);
+        const float* ks = tail->key[parity][0];
+        const float* lv = tail->key[parity][1];
+        const float* iv = tail->key[parity][2];
+        // ---- u = s * ks * c + log2 vs, and its maximum ----
+        float top = -INFINITY, top2 = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+            const float4 a = *reinterpret_cast<const float4*>(ks + c * 32 + k), b = *reinterpret_cast<const float4*>(lv + c * 32 + k);
+            uint64_t x = pk2(__uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1])), y = pk2(__uint_as_float(r[c][k + 2]), __uint_as_float(r[c][k + 3]));
+            x = fma_2(mul_2(x, pk2(a.x, a.y)), c2, pk2(b.x, b.y));
+            y = fma_2(mul_2(y, pk2(a.z, a.w)), c2, pk2(b.z, b.w));
+            float u0, u1, u2, u3;
+            upk2(x, u0, u1), upk2(y, u2, u3);
+            r[c][k] = __float_as_uint(u0), r[c][k + 1] = __float_as_uint(u1), r[c][k + 2] = __float_as_uint(u2), r[c][k + 3] = __float_as_uint(u3);
+          }
+        const int key0 = (g.k0 + j - p.r.pre_tiles) * TK;
+        const bool cut = !PREFIX && p.causal && key0 >= 0 && key0 + TK - 1 > warp_last;   // lane 0's row sees least; the prefix is seen by all
+        if (cut) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (key0 + c * 32 + k > last) r[c][k] = 0xFF800000u;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+            top = max_3(top, __uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1]));
+            top2 = max_3(top2, __uint_as_float(r[c][k + 2]), __uint_as_float(r[c][k + 3]));
+          }
+        top = fmaxf(top, top2);
+        // ---- a maximum that outgrew m: O and l are scaled (the product before this one is done: its commit lies before s_full's) ----
+        const bool grew = top > m + kSlack || (m == -INFINITY && top > m);
+        if (__any_sync(0xffffffffu, grew)) {
+          const float f = grew ? kv_ex2(m - top) : 1.f;
+          if (j > 0) {
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16_async(o_row + c * 16, o);
+              tmem_ld_wait16(o);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st16(o_row + c * 16, o);
+            }
+            tmem_st_wait();
+          }
+          l2 = mul_2(l2, pk2(f, f));
+          if (grew) m = top;
+        }
+        const float z = (m == -INFINITY ? 0.f : m) - (kWeightLog2 - kSlack);
+        const uint64_t z2 = pk2(-z, -z);
+        // ---- weights: fp16 over S, l += w / vs ----
+        uint64_t l3 = pk2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[16];
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+            float4 a = *reinterpret_cast<const float4*>(iv + c * 32 + k);
+            float w0, w1, w2, w3;
+            upk2(add_2(pk2(__uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1])), z2), w0, w1);
+            upk2(add_2(pk2(__uint_as_float(r[c][k + 2]), __uint_as_float(r[c][k + 3])), z2), w2, w3);
+            w0 = kv_ex2(w0), w1 = kv_ex2(w1), w2 = kv_ex2(w2), w3 = kv_ex2(w3);
+            if (cut) {   // a key that the row does not see may have any scale
+              if (w0 == 0.f) a.x = 0.f;
+              if (w1 == 0.f) a.y = 0.f;
+              if (w2 == 0.f) a.z = 0.f;
+              if (w3 == 0.f) a.w = 0.f;
+            }
+            l2 = fma_2(pk2(w0, w1), pk2(a.x, a.y), l2);
+            l3 = fma_2(pk2(w2, w3), pk2(a.z, a.w), l3);
+            w[k / 2] = pack_half2(w0, w1);
+            w[k / 2 + 1] = pack_half2(w2, w3);
+          }
+          tmem_st16(s_row + c * 16, w);
+        }
+        l2 = add_2(l2, l3);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tail->p_full[rt]);
+      }
+      if (!ok) break;
+      ok = all_ok(mbar_wait(&tail->o_full[rt], no++ & 1, abort_flag, p.status, ST_TIMEOUT_PV_DONE));
+      if (!ok) break;
+      tc_fence_after();
+      float la, lb;
+      upk2(l2, la, lb);
+      const float l = la + lb;
+      const bool part = !PREFIX && (g.k0 > 0 || g.k1 < g.s.kt);
+      if (PREFIX || part) {
+        // m as the narrow kernel means it: weights 2^(u - m + 15)
+        const float m_out = m + kSlack;
+        float* dst;
+        if (PREFIX) {
+          const int64_t at = (static_cast<int64_t>(blockIdx.x - g.x / run.run) * p.c.heads + g.h) * p.r.T * p.group + flat;
+          dst = p.pre_o + at * D;
+          if (there) *reinterpret_cast<float2*>(p.pre_ml + 2 * at) = make_float2(m_out, l);
+        } else {
+          float* slot = p.part + (2ll * blockIdx.x + (g.k0 > 0 ? 0 : 1)) * L::PART;
+          dst = slot + (rt * 128 + row) * D;
+          slot[WBM * D + rt * 128 + row] = m_out;
+          slot[WBM * D + WBM + rt * 128 + row] = l;
+        }
+#pragma unroll 1
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld16_async(o_row + c * 16, o);
+          tmem_ld_wait16(o);
+          if (!PREFIX || there) {
+            st_global_32(dst + c * 16, make_uint4(o[0], o[1], o[2], o[3]), make_uint4(o[4], o[5], o[6], o[7]));
+            st_global_32(dst + c * 16 + 8, make_uint4(o[8], o[9], o[10], o[11]), make_uint4(o[12], o[13], o[14], o[15]));
+          }
+        }
+        if (part && warp == 4 && lane == 0) {
+          const int slot = g.k0 > 0 ? 0 : 1;
+          tail->join[slot] = g;
+          tail->first[slot] = g.x / run.run;
+          tail->parts[slot] = (g.x + g.s.kt - 1) / run.run - g.x / run.run + 1;
+        }
+      } else {
+        const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);   // no key: 0
+        uint16_t* dst = p.out + t * p.o_st + head * p.o_sh;
+#pragma unroll 1
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t o[16], w[8];
+          tmem_ld16_async(o_row + c * 16, o);
+          tmem_ld_wait16(o);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) w[k] = kv_pack(__uint_as_float(o[2 * k]) * inv, __uint_as_float(o[2 * k + 1]) * inv, p.is_f16);
+          if (there) {
+            *reinterpret_cast<uint4*>(dst + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(dst + c * 16 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+        }
+      }
+      tc_fence_before();   // O has been read: the next unit's products may write it behind the next p_full
+    }
+    // ---- the run is done: its parts are counted, and units whose last parts they are joined, a row per thread ----
+    if (!PREFIX) {
+      __threadfence();
+      if (!bar_sync_or(1, 256, !ok)) {
+        const int tid = threadIdx.x - 128;
+        if (tid < 2 && tail->parts[tid]) {
+          const int first = tail->first[tid];
+          if (atomicAdd(p.count + first, 1) == tail->parts[tid] - 1) p.count[first] = 0;   // nobody else comes
+          else tail->parts[tid] = 0;
+          __threadfence();
+        }
+        asm volatile("bar.sync 2, 256;" ::: "memory");
+#pragma unroll 1
+        for (int k = 0; k < 2; ++k) {
+          const int parts = tail->parts[k], first = tail->first[k];
+          if (!parts) continue;
+          const KvSegment& u = tail->join[k];
+          const int flat = u.u * WBM + tid, tok = flat / p.group, hh = flat - tok * p.group;
+          if (tok >= u.s.n) continue;
+          const int at = WBM * D + tid;
+          float m = -INFINITY, l = 0.f;
+          for (int i2 = 0; i2 < parts; ++i2) m = fmaxf(m, __ldcg(p.part + kv_slot(first, i2) * L::PART + at));
+          if (m == -INFINITY) m = 0.f;
+          for (int i2 = 0; i2 < parts; ++i2) {
+            const float* slot = p.part + kv_slot(first, i2) * L::PART + at;
+            l = fmaf(__ldcg(slot + WBM), kv_ex2(__ldcg(slot) - m), l);
+          }
+          const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+          uint16_t* dst = p.out + (u.s.first + static_cast<int64_t>(tok)) * p.o_st + (static_cast<int64_t>(u.h) * p.group + hh) * p.o_sh;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0.f;
+#pragma unroll 1
+            for (int i2 = 0; i2 < parts; ++i2) {
+              const float* slot = p.part + kv_slot(first, i2) * L::PART;
+              const float f = kv_ex2(__ldcg(slot + at) - m);
+              float4 x[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = __ldcg(reinterpret_cast<const float4*>(slot + tid * D + c * 32) + e);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                o[4 * e] = fmaf(x[e].x, f, o[4 * e]), o[4 * e + 1] = fmaf(x[e].y, f, o[4 * e + 1]);
+                o[4 * e + 2] = fmaf(x[e].z, f, o[4 * e + 2]), o[4 * e + 3] = fmaf(x[e].w, f, o[4 * e + 3]);
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int y = 0; y < 4; ++y) w[y] = kv_pack(o[e + 2 * y] * inv, o[e + 2 * y + 1] * inv, p.is_f16);
+              *reinterpret_cast<uint4*>(dst + c * 32 + e) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // ------------------------------ teardown ------------------------------
+  __syncwarp();
+  if (*abort_flag && threadIdx.x == 0) kv_wide_settle();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+template <int D, int FMT, bool PREFIX>
+int kv_wide_start(const KvAttnParams& p, int64_t grid, cudaStream_t stream) {
+  auto kern = kv_wide_kernel<D, FMT, PREFIX>;
+  if (int e = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kv_wide_smem<D>()), "kv_attn smem attribute")) return e;
+  return check_cuda(launch_chained(kern, dim3(static_cast<unsigned>(grid)), WTHREADS, kv_wide_smem<D>(), stream, 1, p), "kv_attn (wide) launch");
+}
+
+}  // namespace
+
+int64_t kv_wide_part_floats(int64_t D) { return D == 128 ? KvWide<128>::PART : KvWide<64>::PART; }
+
+int kv_wide_launch(const KvAttnParams& p, int64_t D, int kind, bool prefix, int64_t grid, cudaStream_t stream) {
+  auto by_mode = [&](auto d, auto f) {
+    constexpr int DD = decltype(d)::value, F = decltype(f)::value;
+    return prefix ? kv_wide_start<DD, F, true>(p, grid, stream) : kv_wide_start<DD, F, false>(p, grid, stream);
+  };
+  using I8 = std::integral_constant<int, RH3_KIND_I8>;
+  using F8 = std::integral_constant<int, RH3_KIND_F8>;
+  if (D == 128) return kind == RH3_KIND_I8 ? by_mode(std::integral_constant<int, 128>(), I8()) : by_mode(std::integral_constant<int, 128>(), F8());
+  return kind == RH3_KIND_I8 ? by_mode(std::integral_constant<int, 64>(), I8()) : by_mode(std::integral_constant<int, 64>(), F8());
+}
+
+}  // namespace rh3

@@ -261,7 +261,7 @@ int kv_fill_rows(KvRows* r, const char* what, const int32_t* table, int64_t tabl
                 (long long)table_stride);
   RH3_CHECK_ARG(T >= 0 && T < (1 << 26), "%s: %lld rows: must be below 2^26", what, (long long)T);
   RH3_CHECK_ARG((table || per_seq == 0) && lens && starts, "%s: null batch pointer", what);
-  *r = KvRows{table, lens, starts, table_stride, static_cast<int>(B), static_cast<int>(per_seq), static_cast<int>(T), 0};
+  *r = KvRows{table, lens, starts, table_stride, static_cast<int>(B), static_cast<int>(per_seq), static_cast<int>(T), 0, 0};
   return 0;
 }
 

@@ -28,6 +28,7 @@ struct KvRows {
   int B, per_seq;  // sequences; pages per row of the table
   int T;           // rows of the call
   int fixed_len;   // > 0: one sequence of this many tokens whose rows are all of the call's (a shared prefix; lens and starts are not read)
+  int pre_tiles;   // key tiles of a shared prefix before every unit's own
 };
 
 __device__ __forceinline__ void kv_report(int* status, int code) {
@@ -91,7 +92,7 @@ __device__ __forceinline__ KvSeq kv_seq(const KvRows& r, int page_log2, int grou
   const long long room = static_cast<long long>(r.per_seq) << page_log2;
   s.len = static_cast<int>(min(static_cast<long long>(r.fixed_len ? r.fixed_len : max(r.lens[b], 0)), room));
   s.qt = (s.n * group + BM - 1) / BM;
-  s.kt = max(1, (s.len - 1 + TK) / TK);
+  s.kt = max(1, r.pre_tiles + (s.len + TK - 1) / TK);
   return s;
 }
 struct KvRun {

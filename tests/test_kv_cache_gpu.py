@@ -229,3 +229,17 @@ def test_attention_behind_a_shared_prefix(kv, kind, dtype, d, page, heads, group
     q = (torch.randn(starts[-1], heads * group, d, generator=g) * 1.5).to(dtype).cuda()
     out = kv.attention_shared(q, cache, rows, torch.tensor(ids, dtype=torch.int32, device="cuda"), prefix, causal=causal)
     check_attention(out, q, cache, table[:-1], lens, starts[:-1], causal=causal, prefix=ids, prefix_len=prefix)
+
+
+@pytest.mark.parametrize("kind,dtype,d,page,heads,group", SHAPES[:4])
+@pytest.mark.parametrize("lens,news", [([700, 1, 333], [520, 1, 333]), ([2000], [65])])
+def test_attention_of_many_rows(kv, kind, dtype, d, page, heads, group, lens, news):
+    """Units of 256 rows over several key tiles, cut between CTAs."""
+    pages = sum(-(-n // page) for n in lens) + 2
+    cache = kv.alloc(pages, heads, d, page, kind)
+    fill(cache, 21)
+    rows, table, starts = batch(kv, lens, news, page, pages, 22)
+    g = torch.Generator().manual_seed(23)
+    q = (torch.randn(starts[-1], heads * group, d, generator=g) * 1.5).to(dtype).cuda()
+    out = kv.attention(q, cache, rows)
+    check_attention(out, q, cache, table, lens, starts)
