@@ -13,11 +13,13 @@
 // warps more than their exponentials).
 //
 // 512 threads, one CTA per SM: warp 0 brings pages by bulk copies (codes as they lie), warp 1 issues the products, warps 4-11 are the softmax of
-// the two row tiles (one row per thread), warps 12-15 turn codes into fp16 tiles: rows of keys, 128-byte swizzle, slabs of 64 channels.
+// the two row tiles, warps 12-15 turn codes into fp16 tiles: rows of keys, 128-byte swizzle, slabs of 64 channels.
+// A softmax thread takes S by 16x256b loads: a pair of columns of every eight, of four rows, so that it needs the scales of a quarter of
+// the keys (a row per thread would have every thread load all 128 keys' three floats: 3,000 cycles of the shared-memory return path per step).
 // The same layout is K-major for K and, with the channels as the product's N, MN-major for V, so nothing is transposed.
 // Shared memory: Q 2 x 32 KB | three fp16 tiles of 32 KB (K and V in turn) | three raw tiles of 16 KB. TMEM: S0 | S1 | O0 | O1.
 // Bound, per step of 128 keys and 256 rows: 2,048 cycles of the tensor pipe, as many of the exponential unit, about 3,000 of shared memory (products'
-// operands 1,536, conversion 768, the keys' scales that every softmax warp reads 768).
+// operands 1,536, conversion 768, the keys' scales 768).
 #include "kv_attn.cuh"
 
 namespace rh3 {
@@ -57,15 +59,49 @@ __device__ __forceinline__ uint64_t make_desc_mn128(uint32_t smem_addr, uint32_t
   d &= ~(static_cast<uint64_t>(0x3FFF) << 16);
   return d | static_cast<uint64_t>(slab >> 4) << 16;
 }
-// D[tmem] (+)= A[tmem] * B[smem]
-__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[tmem] * B[smem] over 128 keys: eight products of 16, A 8 columns further and B 16 rows of 128 bytes for each, in a single
+// instruction sequence (as mma4_*: scalar instructions between two products cost tensor-pipe time). accumulate = 0: the first overwrites D.
+__device__ __forceinline__ void mma8_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t"
-      ".reg .pred p;\n\t"
+      ".reg .pred p, q;\n\t"
+      ".reg .b32 a1, a2, a3, a4, a5, a6, a7;\n\t"
+      ".reg .b64 b1, b2, b3, b4, b5, b6, b7;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.eq.b32 q, 0, 0;\n\t"
+      "add.u32 a1, %1, 8;\n\tadd.u32 a2, %1, 16;\n\tadd.u32 a3, %1, 24;\n\tadd.u32 a4, %1, 32;\n\t"
+      "add.u32 a5, %1, 40;\n\tadd.u32 a6, %1, 48;\n\tadd.u32 a7, %1, 56;\n\t"
+      "add.u64 b1, %2, 128;\n\tadd.u64 b2, %2, 256;\n\tadd.u64 b3, %2, 384;\n\tadd.u64 b4, %2, 512;\n\t"
+      "add.u64 b5, %2, 640;\n\tadd.u64 b6, %2, 768;\n\tadd.u64 b7, %2, 896;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a4], b4, %3, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a5], b5, %3, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a6], b6, %3, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a7], b7, %3, q;\n\t"
       "}\n" ::"r"(d_tmem),
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// 16 lanes x 16 columns: thread t has columns 2 (t % 4), + 1 of each eight, of lanes t / 4 (r[4b], r[4b + 1]) and t / 4 + 8 (r[4b + 2], r[4b + 3])
+__device__ __forceinline__ void tmem_ld_frag2(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+// 16 lanes x 64 columns: thread t has column t % 4 of each four, of lanes t / 4 (r[2b]) and t / 4 + 8 (r[2b + 1])
+__device__ __forceinline__ void tmem_st_frag16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+      "r"(r[30]), "r"(r[31])
       : "memory");
 }
 __device__ __forceinline__ uint64_t pk2(float lo, float hi) {
@@ -95,8 +131,8 @@ __device__ __forceinline__ float max_3(float a, float b, float c) {
   return d;
 }
 
-// Registers: 128 a thread at launch; service 40, conversion 72, softmax 200 (128 * 40 + 128 * 72 + 256 * 200 = 512 * 128)
-static_assert(128 * 40 + 128 * 72 + 256 * 200 == WTHREADS * 128, "register pool must balance");
+// Registers: 128 a thread at launch; service 56, conversion 72, softmax 192 (128 * 56 + 128 * 72 + 256 * 192 = 512 * 128)
+static_assert(128 * 56 + 128 * 72 + 256 * 192 == WTHREADS * 128, "register pool must balance");
 
 constexpr float kSlack = 8.f;   // log2 of how far a row's maximum may outgrow m
 
@@ -157,7 +193,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
   auto all_ok = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0) {
       // ------------------------------ producer: raw tiles K, V, K, V ... ------------------------------
       const int page = 1 << p.c.page_log2, tile_pages = TK >> p.c.page_log2;
@@ -207,11 +243,11 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
         return all_ok(mbar_wait_relaxed(&tail->full[t % SLOTS], t / SLOTS & 1, abort_flag, p.status, ST_TIMEOUT_TMA_FULL, 32));
       };
       auto issue_qk = [&](int r, unsigned t, bool free_tile) {
-        const uint32_t q = smem_u32(smem + r * L::Q_BYTES), k = smem_u32(smem + L::TILES + t % SLOTS * L::T_BYTES);
+        const uint64_t q = make_desc_k128(smem_u32(smem + r * L::Q_BYTES)), k = make_desc_k128(smem_u32(smem + L::TILES + t % SLOTS * L::T_BYTES));
         if (elect_one()) {
 #pragma unroll
-          for (int c = 0; c < D / 64; ++c)
-            mma4_f16_ss(tmem_base + r * 128, make_desc_k128(q + c * 128 * 128), make_desc_k128(k + c * TK * 128), idesc_qk, c);
+          for (int c = 0; c < D / 64; ++c)   // slabs of 64 channels, 16 KB apart
+            mma4_f16_ss(tmem_base + r * 128, q + c * (128 * 128 >> 4), k + c * (TK * 128 >> 4), idesc_qk, c);
           mma_commit(&tail->s_full[r]);
           if (free_tile) mma_commit(&tail->empty[t % SLOTS]);
         }
@@ -232,11 +268,9 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
             ok = ok && all_ok(mbar_wait_relaxed(&tail->p_full[r], np[r]++ & 1, abort_flag, p.status, ST_TIMEOUT_P_READY, 32));
             if (!ok) break;
             tc_fence_after();
-            const uint32_t v = smem_u32(smem + L::TILES + (i + 1) % SLOTS * L::T_BYTES);
+            const uint64_t v = make_desc_mn128(smem_u32(smem + L::TILES + (i + 1) % SLOTS * L::T_BYTES), TK * 128);
             if (elect_one()) {
-#pragma unroll
-              for (int c = 0; c < TK / 16; ++c)
-                mma_f16_ts(tmem_base + L::O_COL + r * D, tmem_base + r * 128 + c * 8, make_desc_mn128(v + c * 16 * 128, TK * 128), idesc_pv, j > 0 || c > 0);
+              mma8_f16_ts(tmem_base + L::O_COL + r * D, tmem_base + r * 128, v, idesc_pv, j > 0);
               if (r == tiles - 1) mma_commit(&tail->empty[(i + 1) % SLOTS]);
               if (j == n - 1) mma_commit(&tail->o_full[r]);
             }
@@ -276,19 +310,27 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
           const uint8_t* raw = smem + L::RAWS + s * L::R_BYTES + r0 * D + q * 16;
           uint8_t* out = smem + L::TILES + i % SLOTS * L::T_BYTES + (q / 4) * TK * 128;
           const int swap = (q / 4) & 1;   // the two slabs' rows begin in the same banks: one writes its chunks in the other order
-#pragma unroll 4
-          for (int r = r0; r < TK; r += ROWS, raw += ROWS * D) {
-            uint4 w = *reinterpret_cast<const uint4*>(raw);
-            if (!there(r)) w = make_uint4(0, 0, 0, 0);   // may be anything: a NaN code times a weight of 0 is a NaN
+          constexpr int N = TK / ROWS;
+          uint4 w[N];
+#pragma unroll
+          for (int k = 0; k < N; ++k) w[k] = *reinterpret_cast<const uint4*>(raw + k * ROWS * D);
+          if (!whole) {   // what was not loaded, or lies behind the end, may be anything: a NaN code times a weight of 0 is a NaN
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+              if (!there(r0 + k * ROWS)) w[k] = make_uint4(0, 0, 0, 0);
+          }
+          const int c = (q % 4) * 2;
+          uint8_t* first = out + r0 * 128 + (((c + swap) ^ (r0 & 7)) << 4);        // ROWS is a multiple of 8: the same chunk of every row
+          uint8_t* second = out + r0 * 128 + (((c + 1 - swap) ^ (r0 & 7)) << 4);
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
             uint4 a, b;
-            kv_codes_to_half<FMT>(w.x, a.x, a.y);
-            kv_codes_to_half<FMT>(w.y, a.z, a.w);
-            kv_codes_to_half<FMT>(w.z, b.x, b.y);
-            kv_codes_to_half<FMT>(w.w, b.z, b.w);
-            uint8_t* row = out + r * 128;
-            const int c = (q % 4) * 2;
-            *reinterpret_cast<uint4*>(row + (((c + swap) ^ (r & 7)) << 4)) = swap ? b : a;
-            *reinterpret_cast<uint4*>(row + (((c + 1 - swap) ^ (r & 7)) << 4)) = swap ? a : b;
+            kv_codes_to_half<FMT>(swap ? w[k].z : w[k].x, a.x, a.y);
+            kv_codes_to_half<FMT>(swap ? w[k].w : w[k].y, a.z, a.w);
+            kv_codes_to_half<FMT>(swap ? w[k].x : w[k].z, b.x, b.y);
+            kv_codes_to_half<FMT>(swap ? w[k].y : w[k].w, b.z, b.w);
+            *reinterpret_cast<uint4*>(first + k * ROWS * 128) = a;
+            *reinterpret_cast<uint4*>(second + k * ROWS * 128) = b;
           }
           if (v == 0) {
             const bool is = there(tid);
@@ -307,8 +349,9 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
       }
     }
   } else {
-    // ============================ softmax: one row per thread ============================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // ============================ softmax ============================
+    // Q is brought in, and O given out, by a thread per row; of S a thread has rows 8k + lane / 4 of its warp's 32, k = 0 .. 3.
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     const int rt = (warp >> 2) - 1, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t s_row = tmem_base + rt * 128 + lane_off, o_row = tmem_base + L::O_COL + rt * D + lane_off;
@@ -360,103 +403,130 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
         __syncwarp();
         if (lane == 0) mbar_arrive(&tail->q_full[rt]);
       }
-      // the last own key the row sees, and the first one that some row of the warp does not
-      const int last = p.causal ? g.s.len - g.s.n + tok : g.s.len - 1;
-      const int warp_last = __shfl_sync(0xffffffffu, last, 0);
-      float m = -INFINITY;
-      uint64_t l2 = pk2(0.f, 0.f);
-      const uint64_t c2 = pk2(c_row, c_row);
+      // of the four rows: factor, the last own key that is seen (keys at the thread's column pair), maximum and sum
+      const int last_row = p.causal ? g.s.len - g.s.n + tok : g.s.len - 1;
+      const int warp_last = __shfl_sync(0xffffffffu, last_row, 0);
+      uint64_t c2[4], l2[4];
+      int last[4];
+      float m[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float c = __shfl_sync(0xffffffffu, c_row, 8 * k + (lane >> 2));
+        c2[k] = pk2(c, c);
+        last[k] = __shfl_sync(0xffffffffu, last_row, 8 * k + (lane >> 2)) - 2 * (lane & 3);
+        m[k] = -INFINITY;
+        l2[k] = pk2(0.f, 0.f);
+      }
+      // a value of row 8k + lane / 4 of each k, held by that row's four lanes, for the thread of row `lane`
+      auto to_row = [&](const float* v) {
+        float r = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float x = __shfl_sync(0xffffffffu, v[k], (lane & 7) * 4);
+          if ((lane >> 3) == k) r = x;
+        }
+        return r;
+      };
       for (int j = 0; j < n; ++j, parity ^= 1) {
         // S is there, and so are the keys' scales: the product waited for the tile they came with
         ok = all_ok(mbar_wait(&tail->s_full[rt], ns++ & 1, abort_flag, p.status, ST_TIMEOUT_ACC_FULL));
         if (!ok) break;
         tc_fence_after();
-        uint32_t r[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(s_row + c * 32, r[c]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_wait_regs(r[c]);
-        const float* ks = tail->key[parity][0];
-        const float* lv = tail->key[parity][1];
-        const float* iv = tail->key[parity][2];
-        // ---- u = s * ks * c + log2 vs, and its maximum ----
-        float top = -INFINITY, top2 = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            const float4 a = *reinterpret_cast<const float4*>(ks + c * 32 + k), b = *reinterpret_cast<const float4*>(lv + c * 32 + k);
-            uint64_t x = pk2(__uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1])), y = pk2(__uint_as_float(r[c][k + 2]), __uint_as_float(r[c][k + 3]));
-            x = fma_2(mul_2(x, pk2(a.x, a.y)), c2, pk2(b.x, b.y));
-            y = fma_2(mul_2(y, pk2(a.z, a.w)), c2, pk2(b.z, b.w));
-            float u0, u1, u2, u3;
-            upk2(x, u0, u1), upk2(y, u2, u3);
-            r[c][k] = __float_as_uint(u0), r[c][k + 1] = __float_as_uint(u1), r[c][k + 2] = __float_as_uint(u2), r[c][k + 3] = __float_as_uint(u3);
-          }
+        const float* ks = &tail->key[parity][0][2 * (lane & 3)];
+        const float* lv = ks + TK;
+        const float* iv = lv + TK;
         const int key0 = (g.k0 + j - p.r.pre_tiles) * TK;
         const bool cut = !PREFIX && p.causal && key0 >= 0 && key0 + TK - 1 > warp_last;   // lane 0's row sees least; the prefix is seen by all
-        if (cut) {
+        uint32_t w[2][32];
+        uint64_t sum[4];
+        float top[4];
+        // One pass over the rows, 16 columns at a time: u, its maximum, weights against the maximum as it was set before, their sum.
+        auto pass = [&](auto masked) {
+          uint64_t z2[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (key0 + c * 32 + k > last) r[c][k] = 0xFF800000u;
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            top = max_3(top, __uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1]));
-            top2 = max_3(top2, __uint_as_float(r[c][k + 2]), __uint_as_float(r[c][k + 3]));
+          for (int k = 0; k < 4; ++k) {
+            const float z = (kWeightLog2 - kSlack) - (m[k] == -INFINITY ? 0.f : m[k]);
+            z2[k] = pk2(z, z);
+            top[k] = -INFINITY;
+            sum[k] = pk2(0.f, 0.f);
           }
-        top = fmaxf(top, top2);
-        // ---- a maximum that outgrew m: O and l are scaled (the product before this one is done: its commit lies before s_full's) ----
-        const bool grew = top > m + kSlack || (m == -INFINITY && top > m);
+          uint32_t r[2][2][8];
+          tmem_ld_frag2(s_row, r[0][0]);
+          tmem_ld_frag2(s_row + (16u << 16), r[0][1]);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            tmem_ld_wait8(r[c & 1][0]);
+            tmem_ld_wait8(r[c & 1][1]);
+            if (c < 7) {
+              tmem_ld_frag2(s_row + (c + 1) * 16, r[(c + 1) & 1][0]);
+              tmem_ld_frag2(s_row + (c + 1) * 16 + (16u << 16), r[(c + 1) & 1][1]);
+            }
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const int col = c * 16 + b * 8;
+              const float2 a = *reinterpret_cast<const float2*>(ks + col), d = *reinterpret_cast<const float2*>(lv + col),
+                           e = *reinterpret_cast<const float2*>(iv + col);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t* s = r[c & 1][k >> 1] + 4 * b + 2 * (k & 1);
+                uint64_t x = fma_2(mul_2(pk2(__uint_as_float(s[0]), __uint_as_float(s[1])), pk2(a.x, a.y)), c2[k], pk2(d.x, d.y));
+                float u0, u1;
+                upk2(x, u0, u1);
+                float2 f = e;
+                if constexpr (decltype(masked)::value) {   // a key that the row does not see may have any scale
+                  if (key0 + col > last[k]) u0 = -INFINITY, f.x = 0.f;
+                  if (key0 + col + 1 > last[k]) u1 = -INFINITY, f.y = 0.f;
+                  x = pk2(u0, u1);
+                }
+                top[k] = max_3(top[k], u0, u1);
+                upk2(add_2(x, z2[k]), u0, u1);
+                u0 = kv_ex2(u0), u1 = kv_ex2(u1);
+                sum[k] = fma_2(pk2(u0, u1), pk2(f.x, f.y), sum[k]);
+                w[k >> 1][(c * 2 + b) * 2 + (k & 1)] = pack_half2(u0, u1);
+              }
+            }
+          }
+        };
+        auto either = [&] {
+          if (cut) pass(std::true_type());
+          else pass(std::false_type());
+        };
+        either();
+        bool grew = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) grew |= top[k] > m[k] + kSlack || (m[k] == -INFINITY && top[k] > m[k]);
         if (__any_sync(0xffffffffu, grew)) {
-          const float f = grew ? kv_ex2(m - top) : 1.f;
+          // a maximum outgrew m (always in a unit's first tile): m is set anew, O and l are scaled (the product before is done: its commit
+          // lies before s_full's), and the weights made again
+          float f[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float t = top[k];
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+            const bool set = t > m[k] + kSlack || (m[k] == -INFINITY && t > m[k]);
+            f[k] = set ? kv_ex2(m[k] - t) : 1.f;
+            l2[k] = mul_2(l2[k], pk2(f[k], f[k]));
+            if (set) m[k] = t;
+          }
           if (j > 0) {
+            const float mine = to_row(f);
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
               uint32_t o[16];
               tmem_ld16_async(o_row + c * 16, o);
               tmem_ld_wait16(o);
 #pragma unroll
-              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * mine);
               tmem_st16(o_row + c * 16, o);
             }
-            tmem_st_wait();
           }
-          l2 = mul_2(l2, pk2(f, f));
-          if (grew) m = top;
+          either();
         }
-        const float z = (m == -INFINITY ? 0.f : m) - (kWeightLog2 - kSlack);
-        const uint64_t z2 = pk2(-z, -z);
-        // ---- weights: fp16 over S, l += w / vs ----
-        uint64_t l3 = pk2(0.f, 0.f);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t w[16];
-#pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            float4 a = *reinterpret_cast<const float4*>(iv + c * 32 + k);
-            float w0, w1, w2, w3;
-            upk2(add_2(pk2(__uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1])), z2), w0, w1);
-            upk2(add_2(pk2(__uint_as_float(r[c][k + 2]), __uint_as_float(r[c][k + 3])), z2), w2, w3);
-            w0 = kv_ex2(w0), w1 = kv_ex2(w1), w2 = kv_ex2(w2), w3 = kv_ex2(w3);
-            if (cut) {   // a key that the row does not see may have any scale
-              if (w0 == 0.f) a.x = 0.f;
-              if (w1 == 0.f) a.y = 0.f;
-              if (w2 == 0.f) a.z = 0.f;
-              if (w3 == 0.f) a.w = 0.f;
-            }
-            l2 = fma_2(pk2(w0, w1), pk2(a.x, a.y), l2);
-            l3 = fma_2(pk2(w2, w3), pk2(a.z, a.w), l3);
-            w[k / 2] = pack_half2(w0, w1);
-            w[k / 2 + 1] = pack_half2(w2, w3);
-          }
-          tmem_st16(s_row + c * 16, w);
-        }
-        l2 = add_2(l2, l3);
+        for (int k = 0; k < 4; ++k) l2[k] = add_2(l2[k], sum[k]);
+        tmem_st_frag16(s_row, w[0]);
+        tmem_st_frag16(s_row + (16u << 16), w[1]);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -466,13 +536,20 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
       ok = all_ok(mbar_wait(&tail->o_full[rt], no++ & 1, abort_flag, p.status, ST_TIMEOUT_PV_DONE));
       if (!ok) break;
       tc_fence_after();
-      float la, lb;
-      upk2(l2, la, lb);
-      const float l = la + lb;
+      float lk[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float even, odd;
+        upk2(l2[k], even, odd);
+        lk[k] = even + odd;
+        lk[k] += __shfl_xor_sync(0xffffffffu, lk[k], 1);
+        lk[k] += __shfl_xor_sync(0xffffffffu, lk[k], 2);
+      }
+      const float l = to_row(lk);
       const bool part = !PREFIX && (g.k0 > 0 || g.k1 < g.s.kt);
       if (PREFIX || part) {
         // m as the narrow kernel means it: weights 2^(u - m + 15)
-        const float m_out = m + kSlack;
+        const float m_out = to_row(m) + kSlack;
         float* dst;
         if (PREFIX) {
           const int64_t at = (static_cast<int64_t>(blockIdx.x - g.x / run.run) * p.c.heads + g.h) * p.r.T * p.group + flat;
