@@ -5,27 +5,29 @@
 // of all units are dealt to one CTA per SM in equal runs, as in kv_attn.cu, and parts of cut units are joined the same way. Behind a shared
 // prefix a unit's keys are the prefix's tiles and then its own (or, in the prefix's own pass, the prefix's alone).
 //
-//   S_g = Q_g . K^T   fp16 x fp16 -> fp32 in TMEM (tcgen05 kind::f16), K the codes as fp16, exactly
-//   u = (s * ks_j) * c_row + log2 vs_j, w = 2^(u - m + 7), l += w / vs_j   (kv_attn.cuh)
-//   O_g += W_g . V    W fp16 from TMEM (over S), V the codes as fp16; fp32 in TMEM
+//   S_g = Q_g . K^T        fp16 x fp16 -> fp32 in TMEM (tcgen05 kind::f16), K the codes as fp16, exactly
+//   t = (s * ks_j) * c_row,  w = 2^(t - m + 7),  l += w
+//   O_g += W_g . V         W fp16 from TMEM (over S), V = fp16(code * vs_j * 2^-e); fp32 in TMEM;  o = O / l * 2^e
 // m is a row's maximum when it was last set: it is set anew, and O and l scaled, only when the maximum outgrows it by 2^8, so W stays
-// at most 2^15 and O is hardly ever touched between products (a tile of 128 columns read, scaled and written costs its softmax
-// warps more than their exponentials).
+// at most 2^15 and O is hardly ever touched between products. e is the exponent of the largest V scale so far: V's one rounding
+// is 2^-11 of a value (2^-25 of the largest row's magnitude for what is smaller than 2^-14 of it), as much as that of the
+// weights. (In the exponent, as in kv_attn.cu, the V scales cost a softmax thread two more floats a key and two more operations a
+// score.) A key whose V scale is not finite has V = 0 and a K scale that is not a number: only the rows that see it become NaN.
 //
-// 512 threads, one CTA per SM: warp 0 brings pages by bulk copies (codes as they lie), warp 1 issues the products, warps 4-11 are the softmax of
-// the two row tiles, warps 12-15 turn codes into fp16 tiles: rows of keys, 128-byte swizzle, slabs of 64 channels.
-// A softmax thread takes S by 16x256b loads: a pair of columns of every eight, of four rows, so that it needs the scales of a quarter of
-// the keys (a row per thread would have every thread load all 128 keys' three floats: 3,000 cycles of the shared-memory return path per step).
+// 896 threads, one CTA per SM: warp 0 brings pages by bulk copies (codes as they lie), warp 1 issues the products, warps 4-19 are the softmax, eight
+// to a row tile, 16 rows to a warp, warps 20-23 turn K codes into fp16 tiles, warps 24-27 V codes: rows of keys, 128-byte swizzle, slabs of 64 channels. A softmax
+// thread takes S by 16x256b loads, a pair of columns of every eight, of two rows: it needs the scales of a quarter of the keys (with a
+// row per thread every thread loads all of them, 128 keys' floats: the shared-memory return path becomes the bound).
 // The same layout is K-major for K and, with the channels as the product's N, MN-major for V, so nothing is transposed.
 // Shared memory: Q 2 x 32 KB | three fp16 tiles of 32 KB (K and V in turn) | three raw tiles of 16 KB. TMEM: S0 | S1 | O0 | O1.
-// Bound, per step of 128 keys and 256 rows: 2,048 cycles of the tensor pipe, as many of the exponential unit, about 3,000 of shared memory (products'
-// operands 1,536, conversion 768, the keys' scales 768).
+// Bound, per step of 128 keys and 256 rows: 2,048 cycles of the tensor pipe, as many of the exponential unit, about 2,800 of shared memory (products'
+// operands 1,536, conversion 768, the keys' scales 512).
 #include "kv_attn.cuh"
 
 namespace rh3 {
 namespace {
 
-constexpr int TK = 128, WBM = 256, WTHREADS = 512, SLOTS = 3, RAW = 3;
+constexpr int TK = 128, WBM = 256, WTHREADS = 896, SLOTS = 3, RAW = 3;
 
 template <int D>
 struct KvWide {
@@ -40,9 +42,14 @@ struct KvWide {
 };
 struct __align__(16) KvWideTail {
   float scale[RAW][2][TK];        // as loaded with a K tile: of K, of V
-  float key[2][3][TK];            // per key of a tile, by the tile's parity: K scale, log2 and inverse of the V scale
-  uint64_t raw_full[RAW], raw_empty[RAW], full[SLOTS], empty[SLOTS];
+  float key[2][TK];               // per key of a tile, by the tile's parity: K scale (-inf: no such key)
+  float value[2][TK];             // and V scale * 2^-e
+  float row[2][2][128];           // per row of a row tile: factor c, then l; m
+  uint64_t raw_full[2 * RAW];     // two for a raw tile: for when it holds K, and V, each waited for by its own warps alone
+  uint64_t raw_empty[RAW], full[SLOTS], empty[SLOTS], value_full[2];
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  float top[2][4];                // largest V scale of a warp's keys
+  int exponent[2], whole[2];      // e, and whether all of the tile's keys are there, by the tile's parity
   uint32_t pages[RAW];
   uint32_t tmem_base;
   int abort_flag;
@@ -92,6 +99,11 @@ __device__ __forceinline__ void tmem_ld_frag2(uint32_t taddr, uint32_t* r) {
                : "r"(taddr)
                : "memory");
 }
+__device__ __forceinline__ void tmem_st_frag2(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 // 16 lanes x 64 columns: thread t has column t % 4 of each four, of lanes t / 4 (r[2b]) and t / 4 + 8 (r[2b + 1])
 __device__ __forceinline__ void tmem_st_frag16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
@@ -131,8 +143,8 @@ __device__ __forceinline__ float max_3(float a, float b, float c) {
   return d;
 }
 
-// Registers: 128 a thread at launch; service 56, conversion 72, softmax 192 (128 * 56 + 128 * 72 + 256 * 192 = 512 * 128)
-static_assert(128 * 56 + 128 * 72 + 256 * 192 == WTHREADS * 128, "register pool must balance");
+// Registers: 72 a thread at launch; service 40, softmax 88, conversion 56
+static_assert(128 * 40 + 512 * 88 + 256 * 56 <= WTHREADS * 72, "the shares must not exceed the pool");
 
 constexpr float kSlack = 8.f;   // log2 of how far a row's maximum may outgrow m
 
@@ -166,13 +178,15 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < RAW; ++i) mbar_init(&tail->raw_full[i], 1), mbar_init(&tail->raw_empty[i], 4);
+    for (int i = 0; i < RAW; ++i) mbar_init(&tail->raw_empty[i], 4);
+    for (int i = 0; i < 2 * RAW; ++i) mbar_init(&tail->raw_full[i], 1);
     for (int i = 0; i < SLOTS; ++i) mbar_init(&tail->full[i], 4), mbar_init(&tail->empty[i], 1);
     for (int g = 0; g < 2; ++g) {
-      mbar_init(&tail->q_full[g], 4);
+      mbar_init(&tail->q_full[g], 1);
       mbar_init(&tail->s_full[g], 1);
-      mbar_init(&tail->p_full[g], 4);
+      mbar_init(&tail->p_full[g], 8);
       mbar_init(&tail->o_full[g], 1);
+      mbar_init(&tail->value_full[g], 4);
       tail->parts[g] = 0;
     }
     tail->abort_flag = 0;
@@ -193,7 +207,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
   auto all_ok = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0) {
       // ------------------------------ producer: raw tiles K, V, K, V ... ------------------------------
       const int page = 1 << p.c.page_log2, tile_pages = TK >> p.c.page_log2;
@@ -215,17 +229,18 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
             const int s = i % RAW;
             ok = all_ok(mbar_wait_relaxed(&tail->raw_empty[s], (i / RAW & 1) ^ 1, abort_flag, p.status, ST_TIMEOUT_STAGE_EMPTY, 64));
             if (!ok) break;
+            uint64_t* full = &tail->raw_full[i % (2 * RAW)];
             if (lane == 0) {
               tail->pages[s] = mask;
-              if (mask) mbar_arrive_expect_tx(&tail->raw_full[s], static_cast<uint32_t>(__popc(mask)) * page * (v ? D : D + 8));
-              else mbar_arrive(&tail->raw_full[s]);
+              if (mask) mbar_arrive_expect_tx(full, static_cast<uint32_t>(__popc(mask)) * page * (v ? D : D + 8));
+              else mbar_arrive(full);
             }
             __syncwarp();
             if (good) {
-              bulk_load(smem + L::RAWS + s * L::R_BYTES + lane * page * D, (v ? p.c.v : p.c.k) + row * D, page * D, &tail->raw_full[s]);
+              bulk_load(smem + L::RAWS + s * L::R_BYTES + lane * page * D, (v ? p.c.v : p.c.k) + row * D, page * D, full);
               if (!v) {
-                bulk_load(&tail->scale[s][0][lane * page], p.c.ks + row, page * 4, &tail->raw_full[s]);
-                bulk_load(&tail->scale[s][1][lane * page], p.c.vs + row, page * 4, &tail->raw_full[s]);
+                bulk_load(&tail->scale[s][0][lane * page], p.c.ks + row, page * 4, full);
+                bulk_load(&tail->scale[s][1][lane * page], p.c.vs + row, page * 4, full);
               }
             }
             __syncwarp();
@@ -285,76 +300,106 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
         }
       }
     }
-  } else if (warp >= 12) {
+  } else if (warp >= 20) {
     // ============================ conversion: codes -> fp16 tiles ============================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    const int tid = threadIdx.x - 384;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    const int v = warp >= 24, tid = (threadIdx.x - 640) & 127;   // K or V
     constexpr int PER_ROW = D / 16, ROWS = 128 / PER_ROW;   // 16-code chunks of a row, rows of a round of all 128 threads
     const int q = tid % PER_ROW, r0 = tid / PER_ROW;
-    unsigned i = 0;
-    int parity = 0;
+    const int swap = (q / 4) & 1;   // the two slabs' rows begin in the same banks: one writes its chunks in the other order
+    const int chunk = (q % 4) * 2;
+    // ROWS is a multiple of 8: a thread writes the same chunks of all of its rows
+    const int first = (q / 4) * TK * 128 + r0 * 128 + (((chunk + swap) ^ (r0 & 7)) << 4);
+    const int second = (q / 4) * TK * 128 + r0 * 128 + (((chunk + 1 - swap) ^ (r0 & 7)) << 4);
+    unsigned i = v, tiles = 0;   // tile of the rings, tiles
     bool ok = true;
     while (ok && walk.next(p.r, p.c.page_log2, p.c.heads, p.group, g)) {
       const int kend = kv_wide_end(p, g);
-      for (int kt = g.k0; kt < kend && ok; ++kt, parity ^= 1) {
+      int e = -60;   // exponent of the unit's V; scales below 2^-60 count as 0
+      for (int kt = g.k0; kt < kend; ++kt, i += 2, ++tiles) {
         const KvTile t = kv_wide_tile(p, g, kt);
-#pragma unroll 1
-        for (int v = 0; v < 2; ++v, ++i) {
-          const int s = i % RAW;
-          ok = all_ok(mbar_wait(&tail->raw_full[s], i / RAW & 1, abort_flag, p.status, ST_TIMEOUT_TMA_FULL) &&
-                      mbar_wait(&tail->empty[i % SLOTS], (i / SLOTS & 1) ^ 1, abort_flag, p.status, ST_TIMEOUT_STAGE_EMPTY));
+        const int parity = tiles & 1;
+        const int s = i % RAW;
+        ok = all_ok(mbar_wait(&tail->raw_full[i % (2 * RAW)], i / (2 * RAW) & 1, abort_flag, p.status, ST_TIMEOUT_TMA_FULL) &&
+                    mbar_wait(&tail->empty[i % SLOTS], (i / SLOTS & 1) ^ 1, abort_flag, p.status, ST_TIMEOUT_STAGE_EMPTY));
+        if (!ok && v) break;   // the K warps leave together, behind their barrier
+        const uint32_t pages = tail->pages[s];
+        const bool whole = pages == (0xffffffffu >> (32 - (TK >> p.c.page_log2))) && t.kt * TK + TK <= t.len;
+        auto there = [&](int key) { return whole || (t.kt * TK + key < t.len && ((pages >> (key >> p.c.page_log2)) & 1u)); };
+        if (v) {
+          ok = all_ok(mbar_wait(&tail->value_full[parity], tiles >> 1 & 1, abort_flag, p.status, ST_TIMEOUT_TMA_FULL));
           if (!ok) break;
-          const uint32_t pages = tail->pages[s];
-          const bool whole = pages == (0xffffffffu >> (32 - (TK >> p.c.page_log2))) && t.kt * TK + TK <= t.len;
-          auto there = [&](int key) { return whole || (t.kt * TK + key < t.len && ((pages >> (key >> p.c.page_log2)) & 1u)); };
-          const uint8_t* raw = smem + L::RAWS + s * L::R_BYTES + r0 * D + q * 16;
-          uint8_t* out = smem + L::TILES + i % SLOTS * L::T_BYTES + (q / 4) * TK * 128;
-          const int swap = (q / 4) & 1;   // the two slabs' rows begin in the same banks: one writes its chunks in the other order
-          constexpr int N = TK / ROWS;
-          uint4 w[N];
+        } else {   // the keys' scales
+          const bool is = there(tid);
+          float ks = tail->scale[s][0][tid], vs = is ? tail->scale[s][1][tid] : 0.f;
+          if (!(vs < INFINITY)) vs = 0.f, ks = __uint_as_float(0x7FC00000u);
+          const float top = warp_max(vs);
+          if (lane == 0) tail->top[parity][warp & 3] = top;
+          if (bar_sync_or(5, 128, !ok)) {
+            ok = false;
+            break;
+          }
+          const float most = fmaxf(fmaxf(tail->top[parity][0], tail->top[parity][1]), fmaxf(tail->top[parity][2], tail->top[parity][3]));
+          e = min(126, max(e, static_cast<int>(__float_as_uint(most) >> 23) - 126));   // most < 2^e (4 at the very top)
+          tail->key[parity][tid] = is ? ks : -INFINITY;
+          tail->value[parity][tid] = vs * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+          if (tid == 0) tail->exponent[parity] = e, tail->whole[parity] = whole;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tail->value_full[parity]);
+        }
+        const uint8_t* raw = smem + L::RAWS + s * L::R_BYTES + r0 * D + q * 16;
+        uint8_t* out = smem + L::TILES + i % SLOTS * L::T_BYTES;
+        constexpr int N = TK / ROWS, STEP = 4;
+#pragma unroll 1
+        for (int k0 = 0; k0 < N; k0 += STEP) {
+          uint4 w[STEP];
 #pragma unroll
-          for (int k = 0; k < N; ++k) w[k] = *reinterpret_cast<const uint4*>(raw + k * ROWS * D);
+          for (int k = 0; k < STEP; ++k) w[k] = *reinterpret_cast<const uint4*>(raw + (k0 + k) * ROWS * D);
           if (!whole) {   // what was not loaded, or lies behind the end, may be anything: a NaN code times a weight of 0 is a NaN
 #pragma unroll
-            for (int k = 0; k < N; ++k)
-              if (!there(r0 + k * ROWS)) w[k] = make_uint4(0, 0, 0, 0);
+            for (int k = 0; k < STEP; ++k)
+              if (!there(r0 + (k0 + k) * ROWS)) w[k] = make_uint4(0, 0, 0, 0);
           }
-          const int c = (q % 4) * 2;
-          uint8_t* first = out + r0 * 128 + (((c + swap) ^ (r0 & 7)) << 4);        // ROWS is a multiple of 8: the same chunk of every row
-          uint8_t* second = out + r0 * 128 + (((c + 1 - swap) ^ (r0 & 7)) << 4);
 #pragma unroll
-          for (int k = 0; k < N; ++k) {
-            uint4 a, b;
-            kv_codes_to_half<FMT>(swap ? w[k].z : w[k].x, a.x, a.y);
-            kv_codes_to_half<FMT>(swap ? w[k].w : w[k].y, a.z, a.w);
-            kv_codes_to_half<FMT>(swap ? w[k].x : w[k].z, b.x, b.y);
-            kv_codes_to_half<FMT>(swap ? w[k].y : w[k].w, b.z, b.w);
-            *reinterpret_cast<uint4*>(first + k * ROWS * 128) = a;
-            *reinterpret_cast<uint4*>(second + k * ROWS * 128) = b;
+          for (int k = 0; k < STEP; ++k) {
+            uint32_t h[8];
+            kv_codes_to_half<FMT>(swap ? w[k].z : w[k].x, h[0], h[1]);
+            kv_codes_to_half<FMT>(swap ? w[k].w : w[k].y, h[2], h[3]);
+            kv_codes_to_half<FMT>(swap ? w[k].x : w[k].z, h[4], h[5]);
+            kv_codes_to_half<FMT>(swap ? w[k].y : w[k].w, h[6], h[7]);
+            if (v) {   // times the key's scale in two fp16 pieces: rounded once
+              const float f = tail->value[parity][r0 + (k0 + k) * ROWS];
+              const __half hi = __float2half_rn(f), lo = __float2half_rn(f - __half2float(hi));
+              const __half2 hi2 = __half2half2(hi), lo2 = __half2half2(lo);
+#pragma unroll
+              for (int x = 0; x < 8; ++x) {
+                const __half2 c = *reinterpret_cast<const __half2*>(&h[x]);
+                const __half2 y = __hfma2(c, hi2, __hmul2(c, lo2));
+                h[x] = *reinterpret_cast<const uint32_t*>(&y);
+              }
+            }
+            *reinterpret_cast<uint4*>(out + first + (k0 + k) * ROWS * 128) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(out + second + (k0 + k) * ROWS * 128) = make_uint4(h[4], h[5], h[6], h[7]);
           }
-          if (v == 0) {
-            const bool is = there(tid);
-            const float vs = fmaxf(tail->scale[s][1][tid], kVsMin);
-            tail->key[parity][0][tid] = is ? tail->scale[s][0][tid] : 0.f;
-            tail->key[parity][1][tid] = is ? kv_lg2(vs) : -INFINITY;
-            tail->key[parity][2][tid] = is ? kv_rcp(vs) : 0.f;
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&tail->full[i % SLOTS]);
-            mbar_arrive(&tail->raw_empty[s]);
-          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&tail->full[i % SLOTS]);
+          mbar_arrive(&tail->raw_empty[s]);
         }
       }
     }
   } else {
     // ============================ softmax ============================
-    // Q is brought in, and O given out, by a thread per row; of S a thread has rows 8k + lane / 4 of its warp's 32, k = 0 .. 3.
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-    const int rt = (warp >> 2) - 1, quad = warp & 3, row = quad * 32 + lane;
-    const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t s_row = tmem_base + rt * 128 + lane_off, o_row = tmem_base + L::O_COL + rt * D + lane_off;
+    // Q is brought in, and O given out, by two threads per row, half of the channels each; of S a warp has 16 rows of its TMEM quadrant,
+    // a thread rows 8k + lane / 4 of these, k = 0, 1, and the column pairs 2 (lane % 4) of each eight.
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+    const int rt = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t quad_off = static_cast<uint32_t>(quad * 32) << 16, half_off = static_cast<uint32_t>(half * 16) << 16;
+    const uint32_t s_frag = tmem_base + rt * 128 + quad_off + half_off, o_base = tmem_base + L::O_COL + rt * D + quad_off;
+    const int frag_row = quad * 32 + half * 16 + (lane >> 2);
+    auto tile_bar = [&] { asm volatile("bar.sync %0, 256;" ::"r"(3 + rt) : "memory"); };
     unsigned ns = 0, no = 0;   // uses of s_full and o_full
     int parity = 0;
     bool ok = true;
@@ -368,201 +413,197 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
       const int flat = g.u * WBM + rt * 128 + row, tok = flat / p.group, hh = flat - tok * p.group;
       const bool there = tok < g.s.n;
       const int64_t t = g.s.first + tok, head = static_cast<int64_t>(g.h) * p.group + hh;
-      float c_row;
       {
         const uint16_t* src = p.q + t * p.q_st + head * p.q_sh;
-        uint4 x[D / 8];
         float amax = 0.f, up, down;
-#pragma unroll
+#pragma unroll 4
         for (int c = 0; c < D / 8; ++c) {
-          x[c] = there ? ld_global_16(src + c * 8) : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          const uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 f = kv_unpack(w[k], p.is_f16);
-            amax = max_3(amax, fabsf(f.x), fabsf(f.y));
-          }
+          const uint4 x = there ? ld_global_16(src + c * 8) : make_uint4(0, 0, 0, 0);
+          const float2 f0 = kv_unpack(x.x, p.is_f16), f1 = kv_unpack(x.y, p.is_f16), f2 = kv_unpack(x.z, p.is_f16), f3 = kv_unpack(x.w, p.is_f16);
+          amax = max_3(max_3(amax, fabsf(f0.x), fabsf(f0.y)), max_3(fabsf(f1.x), fabsf(f1.y), fabsf(f2.x)), max_3(fabsf(f2.y), fabsf(f3.x), fabsf(f3.y)));
         }
         kv_row_factor(amax, up, down);
-        c_row = p.sl2 * down;
+        if (half == 0) tail->row[rt][0][row] = fmaxf(p.sl2 * down, 0x1p-126f);   // not 0: a masked score is -inf
         uint8_t* dst = smem + rt * L::Q_BYTES + row * 128;
+#pragma unroll 4
+        for (int k = 0; k < D / 16; ++k) {
+          const int c = half * (D / 16) + k;
+          const uint4 x = there ? ld_global_16(src + c * 8) : make_uint4(0, 0, 0, 0);
+          uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 f = kv_unpack(w[k], p.is_f16);
-            w[k] = pack_half2(f.x * up, f.y * up);
+          for (int y = 0; y < 4; ++y) {
+            const float2 f = kv_unpack(w[y], p.is_f16);
+            w[y] = pack_half2(f.x * up, f.y * up);
           }
           *reinterpret_cast<uint4*>(dst + (c / 8) * 128 * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
         fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&tail->q_full[rt]);
+        tile_bar();
+        if (half == 0 && quad == 0 && lane == 0) mbar_arrive(&tail->q_full[rt]);
       }
-      // of the four rows: factor, the last own key that is seen (keys at the thread's column pair), maximum and sum
-      const int last_row = p.causal ? g.s.len - g.s.n + tok : g.s.len - 1;
-      const int warp_last = __shfl_sync(0xffffffffu, last_row, 0);
-      uint64_t c2[4], l2[4];
-      int last[4];
-      float m[4];
+      // of the thread's two rows: factor, the last own key that is seen, maximum (of t) and sum
+      const int warp_first = (g.u * WBM + rt * 128 + quad * 32 + half * 16) / p.group;   // token of the warp's first row: it sees least
+      const int warp_last = p.causal ? g.s.len - g.s.n + warp_first : g.s.len - 1;
+      uint64_t c2[2];
+      float m[2], l[2];
+      int e = 0;   // of O as it is
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float c = __shfl_sync(0xffffffffu, c_row, 8 * k + (lane >> 2));
+      for (int k = 0; k < 2; ++k) {
+        const float c = tail->row[rt][0][frag_row + 8 * k];
         c2[k] = pk2(c, c);
-        last[k] = __shfl_sync(0xffffffffu, last_row, 8 * k + (lane >> 2)) - 2 * (lane & 3);
-        m[k] = -INFINITY;
-        l2[k] = pk2(0.f, 0.f);
+        m[k] = -INFINITY, l[k] = 0.f;
       }
-      // a value of row 8k + lane / 4 of each k, held by that row's four lanes, for the thread of row `lane`
-      auto to_row = [&](const float* v) {
-        float r = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float x = __shfl_sync(0xffffffffu, v[k], (lane & 7) * 4);
-          if ((lane >> 3) == k) r = x;
-        }
-        return r;
-      };
       for (int j = 0; j < n; ++j, parity ^= 1) {
         // S is there, and so are the keys' scales: the product waited for the tile they came with
         ok = all_ok(mbar_wait(&tail->s_full[rt], ns++ & 1, abort_flag, p.status, ST_TIMEOUT_ACC_FULL));
         if (!ok) break;
         tc_fence_after();
-        const float* ks = &tail->key[parity][0][2 * (lane & 3)];
-        const float* lv = ks + TK;
-        const float* iv = lv + TK;
+        const float* ks = &tail->key[parity][2 * (lane & 3)];
+        const int e_new = tail->exponent[parity];
         const int key0 = (g.k0 + j - p.r.pre_tiles) * TK;
-        const bool cut = !PREFIX && p.causal && key0 >= 0 && key0 + TK - 1 > warp_last;   // lane 0's row sees least; the prefix is seen by all
-        uint32_t w[2][32];
-        uint64_t sum[4];
-        float top[4];
-        // One pass over the rows, 16 columns at a time: u, its maximum, weights against the maximum as it was set before, their sum.
-        auto pass = [&](auto masked) {
-          uint64_t z2[4];
+        const bool cut = !PREFIX && p.causal && key0 >= 0 && key0 + TK - 1 > warp_last;   // the prefix is seen by all
+        const bool masked = cut || !tail->whole[parity];
+        uint32_t w[32];
+        uint64_t sum[2];
+        float top[2];
+        // One pass over the rows, 16 columns at a time: s * ks, its maximum, weights against the maximum as it was set before, their sum.
+        auto pass = [&](auto mask) {
+          uint64_t z2[2];
+          int last[2] = {0, 0};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < 2; ++k) {
             const float z = (kWeightLog2 - kSlack) - (m[k] == -INFINITY ? 0.f : m[k]);
             z2[k] = pk2(z, z);
             top[k] = -INFINITY;
             sum[k] = pk2(0.f, 0.f);
+            if constexpr (decltype(mask)::value)
+              last[k] = cut ? g.s.len - g.s.n + (g.u * WBM + rt * 128 + frag_row + 8 * k) / p.group - key0 - 2 * (lane & 3) : TK;
           }
-          uint32_t r[2][2][8];
-          tmem_ld_frag2(s_row, r[0][0]);
-          tmem_ld_frag2(s_row + (16u << 16), r[0][1]);
+          uint32_t r[2][8];
+          float2 key[2][2];   // of the column pairs, fetched 16 columns ahead as S is
+          auto fetch = [&](int c) {
+            tmem_ld_frag2(s_frag + c * 16, r[c & 1]);
+            key[c & 1][0] = *reinterpret_cast<const float2*>(ks + c * 16);
+            key[c & 1][1] = *reinterpret_cast<const float2*>(ks + c * 16 + 8);
+          };
+          fetch(0);
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
-            tmem_ld_wait8(r[c & 1][0]);
-            tmem_ld_wait8(r[c & 1][1]);
-            if (c < 7) {
-              tmem_ld_frag2(s_row + (c + 1) * 16, r[(c + 1) & 1][0]);
-              tmem_ld_frag2(s_row + (c + 1) * 16 + (16u << 16), r[(c + 1) & 1][1]);
-            }
+            tmem_ld_wait8(r[c & 1]);
+            if (c < 7) fetch(c + 1);
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
               const int col = c * 16 + b * 8;
-              const float2 a = *reinterpret_cast<const float2*>(ks + col), d = *reinterpret_cast<const float2*>(lv + col),
-                           e = *reinterpret_cast<const float2*>(iv + col);
+              const float2 a = key[c & 1][b];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint32_t* s = r[c & 1][k >> 1] + 4 * b + 2 * (k & 1);
-                uint64_t x = fma_2(mul_2(pk2(__uint_as_float(s[0]), __uint_as_float(s[1])), pk2(a.x, a.y)), c2[k], pk2(d.x, d.y));
+              for (int k = 0; k < 2; ++k) {
+                const uint32_t* s = r[c & 1] + 4 * b + 2 * k;
+                uint64_t x = mul_2(pk2(__uint_as_float(s[0]), __uint_as_float(s[1])), pk2(a.x, a.y));
                 float u0, u1;
                 upk2(x, u0, u1);
-                float2 f = e;
-                if constexpr (decltype(masked)::value) {   // a key that the row does not see may have any scale
-                  if (key0 + col > last[k]) u0 = -INFINITY, f.x = 0.f;
-                  if (key0 + col + 1 > last[k]) u1 = -INFINITY, f.y = 0.f;
+                if constexpr (decltype(mask)::value) {
+                  if (a.x == -INFINITY || col > last[k]) u0 = -INFINITY;
+                  if (a.y == -INFINITY || col + 1 > last[k]) u1 = -INFINITY;
                   x = pk2(u0, u1);
                 }
                 top[k] = max_3(top[k], u0, u1);
-                upk2(add_2(x, z2[k]), u0, u1);
+                upk2(fma_2(x, c2[k], z2[k]), u0, u1);
                 u0 = kv_ex2(u0), u1 = kv_ex2(u1);
-                sum[k] = fma_2(pk2(u0, u1), pk2(f.x, f.y), sum[k]);
-                w[k >> 1][(c * 2 + b) * 2 + (k & 1)] = pack_half2(u0, u1);
+                sum[k] = add_2(sum[k], pk2(u0, u1));
+                w[(c * 2 + b) * 2 + k] = pack_half2(u0, u1);
               }
             }
           }
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float c, same;
+            upk2(c2[k], c, same);
+            top[k] *= c;
+          }
         };
         auto either = [&] {
-          if (cut) pass(std::true_type());
+          if (masked) pass(std::true_type());
           else pass(std::false_type());
         };
         either();
-        bool grew = false;
+        bool grew = j == 0 || e_new != e;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) grew |= top[k] > m[k] + kSlack || (m[k] == -INFINITY && top[k] > m[k]);
+        for (int k = 0; k < 2; ++k) grew |= top[k] > m[k] + kSlack || (m[k] == -INFINITY && top[k] > m[k]);
         if (__any_sync(0xffffffffu, grew)) {
-          // a maximum outgrew m (always in a unit's first tile): m is set anew, O and l are scaled (the product before is done: its commit
-          // lies before s_full's), and the weights made again
-          float f[4];
+          // a maximum outgrew m, or V's exponent changed: m is set anew, O and l are scaled (the product before is done: its commit lies
+          // before s_full's), and the weights made again
+          float f[2];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float t = top[k];
-            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-            const bool set = t > m[k] + kSlack || (m[k] == -INFINITY && t > m[k]);
-            f[k] = set ? kv_ex2(m[k] - t) : 1.f;
-            l2[k] = mul_2(l2[k], pk2(f[k], f[k]));
-            if (set) m[k] = t;
+          for (int k = 0; k < 2; ++k) {
+            float x = top[k];
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+            const bool set = x > m[k] + kSlack || (m[k] == -INFINITY && x > m[k]);
+            f[k] = set ? kv_ex2(m[k] - x) : 1.f;
+            l[k] *= f[k];
+            if (set) m[k] = x;
           }
           if (j > 0) {
-            const float mine = to_row(f);
+            const float down = kv_ex2(static_cast<float>(e - e_new));
+            f[0] *= down, f[1] *= down;
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
-              uint32_t o[16];
-              tmem_ld16_async(o_row + c * 16, o);
-              tmem_ld_wait16(o);
+              uint32_t o[8];
+              tmem_ld_frag2(o_base + half_off + c * 16, o);
+              tmem_ld_wait8(o);
 #pragma unroll
-              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * mine);
-              tmem_st16(o_row + c * 16, o);
+              for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f[(k >> 1) & 1]);
+              tmem_st_frag2(o_base + half_off + c * 16, o);
             }
           }
+          e = e_new;
           either();
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) l2[k] = add_2(l2[k], sum[k]);
-        tmem_st_frag16(s_row, w[0]);
-        tmem_st_frag16(s_row + (16u << 16), w[1]);
+        for (int k = 0; k < 2; ++k) {
+          float even, odd;
+          upk2(sum[k], even, odd);
+          l[k] += even + odd;
+        }
+        tmem_st_frag16(s_frag, w);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&tail->p_full[rt]);
       }
-      if (!ok) break;
-      ok = all_ok(mbar_wait(&tail->o_full[rt], no++ & 1, abort_flag, p.status, ST_TIMEOUT_PV_DONE));
-      if (!ok) break;
+      ok = ok && all_ok(mbar_wait(&tail->o_full[rt], no++ & 1, abort_flag, p.status, ST_TIMEOUT_PV_DONE));
       tc_fence_after();
-      float lk[4];
+      // ---- sums and maxima to the threads of the rows ----
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float even, odd;
-        upk2(l2[k], even, odd);
-        lk[k] = even + odd;
-        lk[k] += __shfl_xor_sync(0xffffffffu, lk[k], 1);
-        lk[k] += __shfl_xor_sync(0xffffffffu, lk[k], 2);
+      for (int k = 0; k < 2; ++k) {
+        float x = l[k];
+        x += __shfl_xor_sync(0xffffffffu, x, 1);
+        x += __shfl_xor_sync(0xffffffffu, x, 2);
+        if ((lane & 3) == 0) tail->row[rt][0][frag_row + 8 * k] = x, tail->row[rt][1][frag_row + 8 * k] = m[k];
       }
-      const float l = to_row(lk);
+      if (bar_sync_or(3 + rt, 256, !ok)) {
+        ok = false;
+        break;
+      }
+      const float l_row = tail->row[rt][0][row], m_row = tail->row[rt][1][row];
+      const uint32_t o_row = o_base + half * (D / 2);   // this thread's half of the row's channels
       const bool part = !PREFIX && (g.k0 > 0 || g.k1 < g.s.kt);
       if (PREFIX || part) {
-        // m as the narrow kernel means it: weights 2^(u - m + 15)
-        const float m_out = to_row(m) + kSlack;
+        // as the narrow kernel means it: weights 2^(t + log2 vs - m + 15) for the codes, their sum against vs
+        const float m_out = m_row + kSlack + static_cast<float>(e), l_out = l_row * kv_ex2(static_cast<float>(-e));
         float* dst;
         if (PREFIX) {
           const int64_t at = (static_cast<int64_t>(blockIdx.x - g.x / run.run) * p.c.heads + g.h) * p.r.T * p.group + flat;
           dst = p.pre_o + at * D;
-          if (there) *reinterpret_cast<float2*>(p.pre_ml + 2 * at) = make_float2(m_out, l);
+          if (there && half == 0) *reinterpret_cast<float2*>(p.pre_ml + 2 * at) = make_float2(m_out, l_out);
         } else {
           float* slot = p.part + (2ll * blockIdx.x + (g.k0 > 0 ? 0 : 1)) * L::PART;
           dst = slot + (rt * 128 + row) * D;
-          slot[WBM * D + rt * 128 + row] = m_out;
-          slot[WBM * D + WBM + rt * 128 + row] = l;
+          if (half == 0) slot[WBM * D + rt * 128 + row] = m_out, slot[WBM * D + WBM + rt * 128 + row] = l_out;
         }
+        dst += half * (D / 2);
 #pragma unroll 1
-        for (int c = 0; c < D / 16; ++c) {
+        for (int c = 0; c < D / 32; ++c) {
           uint32_t o[16];
           tmem_ld16_async(o_row + c * 16, o);
           tmem_ld_wait16(o);
@@ -578,10 +619,10 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
           tail->parts[slot] = (g.x + g.s.kt - 1) / run.run - g.x / run.run + 1;
         }
       } else {
-        const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);   // no key: 0
-        uint16_t* dst = p.out + t * p.o_st + head * p.o_sh;
+        const float inv = l_row == 0.f ? 0.f : __fdiv_rn(kv_ex2(static_cast<float>(e)), l_row);   // no key: 0
+        uint16_t* dst = p.out + t * p.o_st + head * p.o_sh + half * (D / 2);
 #pragma unroll 1
-        for (int c = 0; c < D / 16; ++c) {
+        for (int c = 0; c < D / 32; ++c) {
           uint32_t o[16], w[8];
           tmem_ld16_async(o_row + c * 16, o);
           tmem_ld_wait16(o);
@@ -594,11 +635,12 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
         }
       }
       tc_fence_before();   // O has been read: the next unit's products may write it behind the next p_full
+      tile_bar();          // and `row` has been
     }
     // ---- the run is done: its parts are counted, and units whose last parts they are joined, a row per thread ----
     if (!PREFIX) {
       __threadfence();
-      if (!bar_sync_or(1, 256, !ok)) {
+      if (!bar_sync_or(1, 512, !ok)) {
         const int tid = threadIdx.x - 128;
         if (tid < 2 && tail->parts[tid]) {
           const int first = tail->first[tid];
@@ -606,15 +648,16 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
           else tail->parts[tid] = 0;
           __threadfence();
         }
-        asm volatile("bar.sync 2, 256;" ::: "memory");
+        asm volatile("bar.sync 2, 512;" ::: "memory");
 #pragma unroll 1
         for (int k = 0; k < 2; ++k) {
           const int parts = tail->parts[k], first = tail->first[k];
           if (!parts) continue;
           const KvSegment& u = tail->join[k];
-          const int flat = u.u * WBM + tid, tok = flat / p.group, hh = flat - tok * p.group;
+          const int row = tid & 255, half = tid >> 8;
+          const int flat = u.u * WBM + row, tok = flat / p.group, hh = flat - tok * p.group;
           if (tok >= u.s.n) continue;
-          const int at = WBM * D + tid;
+          const int at = WBM * D + row;
           float m = -INFINITY, l = 0.f;
           for (int i2 = 0; i2 < parts; ++i2) m = fmaxf(m, __ldcg(p.part + kv_slot(first, i2) * L::PART + at));
           if (m == -INFINITY) m = 0.f;
@@ -625,7 +668,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
           const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
           uint16_t* dst = p.out + (u.s.first + static_cast<int64_t>(tok)) * p.o_st + (static_cast<int64_t>(u.h) * p.group + hh) * p.o_sh;
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
+          for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
             float o[32];
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0.f;
@@ -635,7 +678,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
               const float f = kv_ex2(__ldcg(slot + at) - m);
               float4 x[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) x[e] = __ldcg(reinterpret_cast<const float4*>(slot + tid * D + c * 32) + e);
+              for (int e = 0; e < 8; ++e) x[e] = __ldcg(reinterpret_cast<const float4*>(slot + row * D + c * 32) + e);
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 o[4 * e] = fmaf(x[e].x, f, o[4 * e]), o[4 * e + 1] = fmaf(x[e].y, f, o[4 * e + 1]);
