@@ -409,33 +409,38 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
         parity ^= n & 1;
         continue;
       }
-      // ---- the row of Q as fp16 into its tile ----
-      const int flat = g.u * WBM + rt * 128 + row, tok = flat / p.group, hh = flat - tok * p.group;
-      const bool there = tok < g.s.n;
-      const int64_t t = g.s.first + tok, head = static_cast<int64_t>(g.h) * p.group + hh;
+      // ---- 16 rows of Q as fp16 into their tile, D / 8 lanes to a row, all loads in flight ----
       {
-        const uint16_t* src = p.q + t * p.q_st + head * p.q_sh;
-        float amax = 0.f, up, down;
-#pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 x = there ? ld_global_16(src + c * 8) : make_uint4(0, 0, 0, 0);
-          const float2 f0 = kv_unpack(x.x, p.is_f16), f1 = kv_unpack(x.y, p.is_f16), f2 = kv_unpack(x.z, p.is_f16), f3 = kv_unpack(x.w, p.is_f16);
-          amax = max_3(max_3(amax, fabsf(f0.x), fabsf(f0.y)), max_3(fabsf(f1.x), fabsf(f1.y), fabsf(f2.x)), max_3(fabsf(f2.y), fabsf(f3.x), fabsf(f3.y)));
+        constexpr int LANES = D / 8, ROWS = 32 / LANES, N = 16 / ROWS;
+        const int ch = lane % LANES, r0 = ((warp - 4) & 7) * 16 + lane / LANES;
+        uint4 x[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const int flat = g.u * WBM + rt * 128 + r0 + k * ROWS, tok = flat / p.group, hh = flat - tok * p.group;
+          const int64_t at = static_cast<int64_t>(g.s.first + tok) * p.q_st + (static_cast<int64_t>(g.h) * p.group + hh) * p.q_sh + ch * 8;
+          x[k] = tok < g.s.n ? ld_global_16(p.q + at) : make_uint4(0, 0, 0, 0);
         }
-        kv_row_factor(amax, up, down);
-        if (half == 0) tail->row[rt][0][row] = fmaxf(p.sl2 * down, 0x1p-126f);   // not 0: a masked score is -inf
-        uint8_t* dst = smem + rt * L::Q_BYTES + row * 128;
-#pragma unroll 4
-        for (int k = 0; k < D / 16; ++k) {
-          const int c = half * (D / 16) + k;
-          const uint4 x = there ? ld_global_16(src + c * 8) : make_uint4(0, 0, 0, 0);
-          uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        uint8_t* dst = smem + rt * L::Q_BYTES + (ch / 8) * 128 * 128;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+          float amax = 0.f, up, down;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const float2 f = kv_unpack(w[y], p.is_f16);
+            amax = max_3(amax, fabsf(f.x), fabsf(f.y));
+          }
+#pragma unroll
+          for (int o = LANES / 2; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+          kv_row_factor(amax, up, down);
+          const int row = r0 + k * ROWS;
+          if (ch == 0) tail->row[rt][0][row] = fmaxf(p.sl2 * down, 0x1p-126f);   // not 0: a masked score is -inf
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
             const float2 f = kv_unpack(w[y], p.is_f16);
             w[y] = pack_half2(f.x * up, f.y * up);
           }
-          *reinterpret_cast<uint4*>(dst + (c / 8) * 128 * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(dst + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
         fence_proxy_async_smem();
         tile_bar();
@@ -585,29 +590,35 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
         ok = false;
         break;
       }
+      const int flat = g.u * WBM + rt * 128 + row, tok = flat / p.group, hh = flat - tok * p.group;
+      const bool there = tok < g.s.n;
+      const int64_t t = g.s.first + tok, head = static_cast<int64_t>(g.h) * p.group + hh;
       const float l_row = tail->row[rt][0][row], m_row = tail->row[rt][1][row];
       const uint32_t o_row = o_base + half * (D / 2);   // this thread's half of the row's channels
       const bool part = !PREFIX && (g.k0 > 0 || g.k1 < g.s.kt);
       if (PREFIX || part) {
         // as the narrow kernel means it: weights 2^(t + log2 vs - m + 15) for the codes, their sum against vs
         const float m_out = m_row + kSlack + static_cast<float>(e), l_out = l_row * kv_ex2(static_cast<float>(-e));
-        float* dst;
+        float* dst;   // of the prefix's rows; a partial result is [D / 4][256 rows] float4, so that lanes write, and a join reads, side by side
         if (PREFIX) {
           const int64_t at = (static_cast<int64_t>(blockIdx.x - g.x / run.run) * p.c.heads + g.h) * p.r.T * p.group + flat;
-          dst = p.pre_o + at * D;
+          dst = p.pre_o + at * D + half * (D / 2);
           if (there && half == 0) *reinterpret_cast<float2*>(p.pre_ml + 2 * at) = make_float2(m_out, l_out);
         } else {
           float* slot = p.part + (2ll * blockIdx.x + (g.k0 > 0 ? 0 : 1)) * L::PART;
-          dst = slot + (rt * 128 + row) * D;
+          dst = slot + (half * (D / 8) * WBM + rt * 128 + row) * 4;
           if (half == 0) slot[WBM * D + rt * 128 + row] = m_out, slot[WBM * D + WBM + rt * 128 + row] = l_out;
         }
-        dst += half * (D / 2);
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[16];
           tmem_ld16_async(o_row + c * 16, o);
           tmem_ld_wait16(o);
-          if (!PREFIX || there) {
+          if (!PREFIX) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              reinterpret_cast<uint4*>(dst)[(c * 4 + k) * WBM] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          } else if (there) {
             st_global_32(dst + c * 16, make_uint4(o[0], o[1], o[2], o[3]), make_uint4(o[4], o[5], o[6], o[7]));
             st_global_32(dst + c * 16 + 8, make_uint4(o[8], o[9], o[10], o[11]), make_uint4(o[12], o[13], o[14], o[15]));
           }
@@ -628,7 +639,9 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
           tmem_ld_wait16(o);
 #pragma unroll
           for (int k = 0; k < 8; ++k) w[k] = kv_pack(__uint_as_float(o[2 * k]) * inv, __uint_as_float(o[2 * k + 1]) * inv, p.is_f16);
-          if (there) {
+          if (there && (reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
+            st_global_32(dst + c * 16, make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7]));
+          } else if (there) {
             *reinterpret_cast<uint4*>(dst + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
             *reinterpret_cast<uint4*>(dst + c * 16 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
           }
@@ -678,7 +691,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
               const float f = kv_ex2(__ldcg(slot + at) - m);
               float4 x[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) x[e] = __ldcg(reinterpret_cast<const float4*>(slot + row * D + c * 32) + e);
+              for (int e = 0; e < 8; ++e) x[e] = __ldcg(reinterpret_cast<const float4*>(slot) + (c * 8 + e) * WBM + row);
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 o[4 * e] = fmaf(x[e].x, f, o[4 * e]), o[4 * e + 1] = fmaf(x[e].y, f, o[4 * e + 1]);
