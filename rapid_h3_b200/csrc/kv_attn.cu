@@ -494,8 +494,8 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
           const KvLaneRow r = kv_lane_row<BM>(p, g, 8 * nt + 2 * c + e);
           int parts = 0;
           if (r.q >= 0) {
-            const int x = (g.h * ((static_cast<int>(rows) + p.pre_bm - 1) / p.pre_bm) + r.flat / p.pre_bm) * p.pre_kt;
-            parts = (x + p.pre_kt - 1) / p.pre_run - x / p.pre_run + 1;
+            const int x = (g.h * ((static_cast<int>(rows) + p.pre_bm - 1) / p.pre_bm) + r.flat / p.pre_bm) * p.pre_unit;
+            parts = (x + p.pre_last) / p.pre_run - (x + p.pre_first) / p.pre_run + 1;
           }
           for (int s = warp; s < parts; s += KV_WARPS) {
             const long long at = (static_cast<long long>(s) * p.c.heads + g.h) * rows + r.flat;
@@ -664,7 +664,8 @@ KvPass kv_pass(int64_t heads, int64_t rows, int64_t seqs, int64_t kt) {
 }
 struct KvPlan {
   KvPass own, pre;              // pre.grid = 0: no pass of its own for the prefix (none, or its tiles are among the wide units' own)
-  int64_t pre_run, pre_splits;  // tiles of a CTA of the prefix pass, into how many parts its units may fall
+  int64_t pre_run, pre_unit, pre_first, pre_last;   // see KvAttnParams
+  int64_t pre_splits;           // into how many parts the prefix pass's units may fall
   int64_t part, pre_ml, pre_o, bytes;   // byte offsets
 };
 KvPlan kv_plan(int64_t heads, int64_t group, int64_t page, int64_t D, int64_t per_seq, int64_t B, int64_t T, int64_t prefix) {
@@ -681,10 +682,14 @@ KvPlan kv_plan(int64_t heads, int64_t group, int64_t page, int64_t D, int64_t pe
   if (prefix > 0 && x.own.nt) {
     x.pre = kv_pass(heads, rows, 1, pre_kt);
     const int64_t units = heads * ((rows + x.pre.bm - 1) / x.pre.bm);
-    x.pre.w = units * pre_kt;
+    x.pre_unit = x.pre.nt ? pre_kt : KV_WIDE_UNIT_COST + prefix;   // tiles, or keys and the unit's own cost
+    x.pre_first = x.pre.nt ? 0 : KV_WIDE_UNIT_COST;
+    x.pre_last = x.pre.nt ? pre_kt - 1 : KV_WIDE_UNIT_COST + (pre_kt - 1) * TK;
+    x.pre.w = units * x.pre_unit;
     x.pre.grid = kv_grid(units, pre_kt, x.pre.nt == 0 ? 1 : x.pre.nt == 1 ? 3 : 2);
     x.pre_run = (x.pre.w + x.pre.grid - 1) / x.pre.grid;
-    x.pre_splits = (pre_kt - 1) / x.pre_run + 2;
+    if (x.pre.nt == 0 && x.pre_run < TK) x.pre_run = TK;
+    x.pre_splits = (x.pre_last - x.pre_first) / x.pre_run + 2;
     if (x.pre_splits > pre_kt) x.pre_splits = pre_kt;
     x.pre_ml = take(x.pre_splits * heads * rows * 2 * sizeof(float));
     x.pre_o = take(x.pre_splits * heads * rows * D * sizeof(float));
@@ -756,7 +761,9 @@ extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t w
   if (a->prefix == 0) return launch(std::integral_constant<int, MODE_PLAIN>(), p, x.own);
   p.pre_ml = reinterpret_cast<float*>(ws + x.pre_ml);
   p.pre_o = reinterpret_cast<float*>(ws + x.pre_o);
-  p.pre_kt = static_cast<int>(x.pre.kt);
+  p.pre_unit = static_cast<int>(x.pre_unit);
+  p.pre_first = static_cast<int>(x.pre_first);
+  p.pre_last = static_cast<int>(x.pre_last);
   p.pre_bm = static_cast<int>(x.pre.bm);
   p.pre_run = static_cast<int>(x.pre_run);
   // the prefix is one sequence whose rows are all rows of the call

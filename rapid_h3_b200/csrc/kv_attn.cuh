@@ -34,7 +34,9 @@ struct KvAttnParams {
   //   pre_o [split][heads][rows][D], pre_ml [split][heads][rows][2], rows = T * group
   float* pre_o;
   float* pre_ml;
-  int pre_run, pre_kt, pre_bm;  // the prefix pass: tiles of a CTA, tiles of a unit, rows of a unit
+  // which parts the prefix pass leaves of a unit, in its measure of work: a CTA has pre_run of it, a unit weighs pre_unit; the CTAs that
+  // positions pre_first and pre_last of a unit belong to have its first and its last part
+  int pre_run, pre_unit, pre_first, pre_last, pre_bm;
   // shared prefix in the wide kernel's single pass: r.pre_tiles tiles of it before a unit's own
   const int* pre_table;
   int pre_len;
@@ -99,6 +101,7 @@ __device__ __forceinline__ uint32_t kv_pack(float a, float b, int is_f16) { retu
 
 // kv_attn_wide.cu: the same parameters, units of 256 rows; floats of one of its partial results
 constexpr int KV_WIDE_BM = 256;
+constexpr int KV_WIDE_UNIT_COST = 256;   // what a unit costs besides its keys, in keys
 int64_t kv_wide_part_floats(int64_t D);
 int kv_wide_launch(const KvAttnParams& p, int64_t D, int kind, bool prefix, int64_t grid, cudaStream_t stream);
 

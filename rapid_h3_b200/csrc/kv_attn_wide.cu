@@ -6,15 +6,16 @@
 // prefix a unit's keys are the prefix's tiles and then its own (or, in the prefix's own pass, the prefix's alone).
 //
 //   S_g = Q_g . K^T        fp16 x fp16 -> fp32 in TMEM (tcgen05 kind::f16), K the codes as fp16, exactly
-//   t = (s * ks_j) * c_row,  w = 2^(t - m + 7),  l += w
+//   t = (s * ks_j) * c_row,  w = 2^(t - m + 3),  l += w
 //   O_g += W_g . V         W fp16 from TMEM (over S), V = fp16(code * vs_j * 2^-e); fp32 in TMEM;  o = O / l * 2^e
-// m is a row's maximum when it was last set: it is set anew, and O and l scaled, only when the maximum outgrows it by 2^8, so W stays
-// at most 2^15 and O is hardly ever touched between products. e is the exponent of the largest V scale so far: V's one rounding
+// m is a row's maximum when it was last set: it is set anew, and O and l scaled, only when the maximum outgrows it by 2^12, so W stays
+// at most 2^15 and O is hardly ever touched between products (2,011 tokens behind 16,000: 632 us where it might outgrow it by 2^8, 618 by 2^12). e is the exponent of the largest V scale so far: V's one rounding
 // is 2^-11 of a value (2^-25 of the largest row's magnitude for what is smaller than 2^-14 of it), as much as that of the
 // weights. (In the exponent, as in kv_attn.cu, the V scales cost a softmax thread two more floats a key and two more operations a
 // score.) A key whose V scale is not finite has V = 0 and a K scale that is not a number: only the rows that see it become NaN.
 //
-// 896 threads, one CTA per SM: warp 0 brings pages by bulk copies (codes as they lie), warp 1 issues the products, warps 4-19 are the softmax, eight
+// 896 threads, one CTA per SM: warp 0 brings pages by bulk copies (codes as they lie), warp 1 issues the products, warp 2 works out the run's segments and tells
+// the others, warps 4-19 are the softmax, eight
 // to a row tile, 16 rows to a warp, warps 20-23 turn K codes into fp16 tiles, warps 24-27 V codes: rows of keys, 128-byte swizzle, slabs of 64 channels. A softmax
 // thread takes S by 16x256b loads, a pair of columns of every eight, of two rows: it needs the scales of a quarter of the keys (with a
 // row per thread every thread loads all of them, 128 keys' floats: the shared-memory return path becomes the bound).
@@ -27,7 +28,8 @@
 namespace rh3 {
 namespace {
 
-constexpr int TK = 128, WBM = 256, WTHREADS = 896, SLOTS = 3, RAW = 3;
+constexpr int TK = 128, WBM = 256, WTHREADS = 896, SLOTS = 3, RAW = 3, SEGS = 4;
+constexpr int SEG_READERS = 26;   // warps that are told of a segment: two of the service, eight of the conversion, sixteen of the softmax
 
 template <int D>
 struct KvWide {
@@ -40,21 +42,29 @@ struct KvWide {
   static constexpr int PART = WBM * D + 2 * WBM;    // floats of a partial result
   static constexpr int O_COL = 256;                 // TMEM column of O of row tile 0
 };
+// one unit's part of a CTA's run
+struct KvWideSegment {
+  int first, n, len;      // of the sequence
+  int b, h, u;            // sequence, KV head, row tile
+  int k0, k1, kt;         // tiles [k0, k1) of the unit's kt
+  int cta, parts;         // CTAs cta .. cta + parts - 1 have a part of the unit
+};
 struct __align__(16) KvWideTail {
   float scale[RAW][2][TK];        // as loaded with a K tile: of K, of V
   float key[2][TK];               // per key of a tile, by the tile's parity: K scale (-inf: no such key)
   float value[2][TK];             // and V scale * 2^-e
-  float row[2][2][128];           // per row of a row tile: factor c, then l; m
+  float row[2][2][2][128];        // per row of a row tile: factor c, then l; m; two units' in turn
   uint64_t raw_full[2 * RAW];     // two for a raw tile: for when it holds K, and V, each waited for by its own warps alone
   uint64_t raw_empty[RAW], full[SLOTS], empty[SLOTS], value_full[2];
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2], seg_full[SEGS], seg_empty[SEGS];
   float top[2][4];                // largest V scale of a warp's keys
   int exponent[2], whole[2];      // e, and whether all of the tile's keys are there, by the tile's parity
   uint32_t pages[RAW];
   uint32_t tmem_base;
   int abort_flag;
-  KvSegment join[2];
-  int first[2], parts[2];
+  KvWideSegment seg[SEGS];        // the run's segments in turn; k1 = 0: there are no more
+  KvWideSegment join[2];
+  int parts[2];
 };
 template <int D>
 constexpr int kv_wide_smem() { return KvWide<D>::TAIL + static_cast<int>(sizeof(KvWideTail)) + 1024; }
@@ -146,26 +156,112 @@ __device__ __forceinline__ float max_3(float a, float b, float c) {
 // Registers: 72 a thread at launch; service 40, softmax 88, conversion 56
 static_assert(128 * 40 + 512 * 88 + 256 * 56 <= WTHREADS * 72, "the shares must not exceed the pool");
 
-constexpr float kSlack = 8.f;   // log2 of how far a row's maximum may outgrow m
+constexpr float kSlack = 12.f;   // log2 of how far a row's maximum may outgrow m
 
 // after an abandoned wait: copies that are still on their way land before the CTA gives its shared memory back
 __device__ __forceinline__ void kv_wide_settle() {
   for (int i = 0; i < 64; ++i) __nanosleep(1000);
 }
 
-// End of the tiles of a segment that are worked on (behind the last visible key they are not; one always is), row tiles that have rows.
-__device__ __forceinline__ int kv_wide_end(const KvAttnParams& p, const KvSegment& g) {
-  return max(g.k0 + 1, min(g.k1, p.r.pre_tiles + (kv_visible<WBM>(g.s, p.group, g.u, p.causal) + TK - 1) / TK));
+// How the work is dealt. A unit's weight is what it costs in keys: UNIT_COST for Q, the join of sums and the output, and the keys that its rows
+// see, prefix tiles included, taken as linear in the number u of the row tile, w(u) = base + step * u, so that sums over units have a closed
+// form. CTAs get equal runs of weight (at least a tile); inside a unit weight position y stands for tile min(kt, ceil((y - UNIT_COST) / TK)),
+// the last one for kt, so neighbouring runs meet at the same tile. Tiles behind the last visible key are no work and in nobody's run.
+constexpr int UNIT_COST = KV_WIDE_UNIT_COST;
+struct KvWideSeq {
+  int first, n, len, qt;      // first row token of the call, new tokens, cached tokens, row tiles
+  int step;
+  long long base, head;       // of one unit; weight of all units of a head
+};
+__device__ __forceinline__ KvWideSeq kv_wide_seq(const KvAttnParams& p, int b) {
+  const KvSeq q = kv_seq<WBM, TK>(p.r, p.c.page_log2, p.group, b);
+  KvWideSeq s;
+  s.first = q.first, s.n = q.n, s.len = q.len, s.qt = q.qt;
+  s.step = p.causal ? WBM / p.group : 0;
+  s.base = UNIT_COST + p.r.pre_tiles * TK + max(1, p.causal ? q.len - q.n + max(1, s.step) : q.len);
+  s.head = s.base * s.qt + static_cast<long long>(s.step) * s.qt * (s.qt - 1) / 2;
+  return s;
 }
-__device__ __forceinline__ int kv_wide_row_tiles(const KvAttnParams& p, const KvSegment& g) { return g.s.n * p.group - g.u * WBM > 128 ? 2 : 1; }
+// tiles that row tile u works on (one at least: rows without a key are written too)
+__device__ __forceinline__ int kv_wide_tiles(const KvAttnParams& p, const KvWideSeq& s, int u) {
+  int seen = s.len;
+  if (p.causal) seen = max(0, min(s.len, s.len - s.n + (min((u + 1) * WBM, s.n * p.group) - 1) / p.group + 1));
+  return max(1, p.r.pre_tiles + (seen + TK - 1) / TK);
+}
+struct KvWideWalk {
+  long long x, x1, run, xb;   // position, end and length of the CTA's run; where sequence b begins
+  int b;
+  KvWideSeq s;
+  // Every warp scans the sequences by itself.
+  __device__ __forceinline__ KvWideWalk(const KvAttnParams& p) {
+    const int lane = threadIdx.x & 31, per = (p.r.B + 31) >> 5;
+    const int b0 = min(p.r.B, lane * per), b1 = min(p.r.B, b0 + per);
+    long long own = 0;
+    for (int i = b0; i < b1; ++i) own += p.c.heads * kv_wide_seq(p, i).head;
+    long long incl = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    const long long W = __shfl_sync(0xffffffffu, incl, 31);
+    run = max(static_cast<long long>(TK), (W + gridDim.x - 1) / gridDim.x);
+    x = min(W, run * blockIdx.x), x1 = min(W, x + run);
+    long long at = incl - own;
+    int i = b0;
+    const bool mine = x < x1 && at <= x && x < incl;
+    if (mine) {
+      for (; i < b1; ++i) {
+        const long long w = p.c.heads * kv_wide_seq(p, i).head;
+        if (x < at + w) break;
+        at += w;
+      }
+    }
+    const uint32_t who = __ballot_sync(0xffffffffu, mine);
+    b = __shfl_sync(0xffffffffu, i, who ? __ffs(who) - 1 : 0);
+    xb = __shfl_sync(0xffffffffu, at, who ? __ffs(who) - 1 : 0);
+    if (x < x1) s = kv_wide_seq(p, b);
+  }
+  // the next unit of which the run has tiles
+  __device__ __forceinline__ bool next(const KvAttnParams& p, KvWideSegment& g) {
+    while (x < x1) {
+      while (x - xb >= p.c.heads * s.head) {
+        if (b + 1 >= p.r.B) return false;
+        xb += p.c.heads * s.head;
+        s = kv_wide_seq(p, ++b);
+      }
+      const int h = static_cast<int>((x - xb) / s.head);
+      const long long xh = xb + h * s.head;   // where the head begins
+      // the row tile: the last u whose units before it weigh no more than x - xh
+      auto before = [&](long long u) { return s.base * u + s.step * (u * (u - 1) / 2); };
+      int u = 0;
+      for (int d = 1 << (31 - __clz(s.qt)); d; d >>= 1)
+        if (u + d < s.qt && before(u + d) <= x - xh) u += d;
+      const long long xu = xh + before(u), w = s.base + static_cast<long long>(s.step) * u;
+      const int kt = kv_wide_tiles(p, s, u);
+      auto tile = [&](long long y) { return y >= w ? kt : y <= UNIT_COST ? 0 : static_cast<int>(min(static_cast<long long>(kt), (y - UNIT_COST + TK - 1) / TK)); };
+      const long long end = min(w, x1 - xu);
+      g.k0 = tile(x - xu), g.k1 = tile(end);
+      x = xu + end;
+      if (g.k0 >= g.k1) continue;
+      g.first = s.first, g.n = s.n, g.len = s.len, g.b = b, g.h = h, g.u = u, g.kt = kt;
+      const long long full = min(w, static_cast<long long>(UNIT_COST) + static_cast<long long>(kt - 1) * TK + 1);   // from here on all tiles are dealt
+      g.cta = static_cast<int>((xu + UNIT_COST) / run);
+      g.parts = static_cast<int>((xu + full - 1) / run) - g.cta + 1;
+      return true;
+    }
+    return false;
+  }
+};
+__device__ __forceinline__ int kv_wide_row_tiles(const KvAttnParams& p, const KvWideSegment& g) { return g.n * p.group - g.u * WBM > 128 ? 2 : 1; }
 // where the keys of tile kt are
 struct KvTile {
   const int* table;   // pages
   int kt, len;        // tile and tokens of that table
 };
-__device__ __forceinline__ KvTile kv_wide_tile(const KvAttnParams& p, const KvSegment& g, int kt) {
+__device__ __forceinline__ KvTile kv_wide_tile(const KvAttnParams& p, const KvWideSegment& g, int kt) {
   if (kt < p.r.pre_tiles) return KvTile{p.pre_table, kt, p.pre_len};
-  return KvTile{p.r.table + g.b * p.r.table_stride, kt - p.r.pre_tiles, g.s.len};
+  return KvTile{p.r.table + g.b * p.r.table_stride, kt - p.r.pre_tiles, g.len};
 }
 
 template <int D, int FMT, bool PREFIX>
@@ -189,6 +285,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
       mbar_init(&tail->value_full[g], 4);
       tail->parts[g] = 0;
     }
+    for (int i = 0; i < SEGS; ++i) mbar_init(&tail->seg_full[i], 1), mbar_init(&tail->seg_empty[i], SEG_READERS);
     tail->abort_flag = 0;
     fence_barrier_init();
   }
@@ -201,10 +298,16 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
   tc_fence_after();
   grid_dependency_begin();
   const uint32_t tmem_base = tail->tmem_base;
-  const KvRun run = kv_find_run<WBM, TK>(p.r, p.c.page_log2, p.c.heads, p.group, p.most, p.status);
-  KvWalk<WBM, TK> walk(run);
-  KvSegment g;
   auto all_ok = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
+  // the i-th segment of the run, once it is known; done with it
+  auto segment = [&](unsigned i, bool& ok) {
+    ok = all_ok(mbar_wait(&tail->seg_full[i % SEGS], i / SEGS & 1, abort_flag, p.status, ST_TIMEOUT_TMA_FULL));
+    return ok && tail->seg[i % SEGS].k1 > 0;
+  };
+  auto release = [&](unsigned i) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&tail->seg_empty[i % SEGS]);
+  };
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
@@ -213,9 +316,10 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
       const int page = 1 << p.c.page_log2, tile_pages = TK >> p.c.page_log2;
       unsigned i = 0;
       bool ok = true;
-      while (ok && walk.next(p.r, p.c.page_log2, p.c.heads, p.group, g)) {
-        const int kend = kv_wide_end(p, g);
-        for (int kt = g.k0; kt < kend && ok; ++kt) {
+      for (unsigned seg = 0; ok && segment(seg, ok); ++seg) {
+        const KvWideSegment g = tail->seg[seg % SEGS];
+        release(seg);
+        for (int kt = g.k0; kt < g.k1 && ok; ++kt) {
           const KvTile t = kv_wide_tile(p, g, kt);
           const int at = t.kt * tile_pages + lane;
           const bool need = lane < tile_pages && (static_cast<int64_t>(at) << p.c.page_log2) < t.len;
@@ -268,8 +372,10 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
         }
         __syncwarp();
       };
-      while (ok && walk.next(p.r, p.c.page_log2, p.c.heads, p.group, g)) {
-        const int kend = kv_wide_end(p, g), tiles = kv_wide_row_tiles(p, g), n = kend - g.k0;
+      for (unsigned seg = 0; ok && segment(seg, ok); ++seg) {
+        const KvWideSegment& g = tail->seg[seg % SEGS];
+        const int tiles = kv_wide_row_tiles(p, g), n = g.k1 - g.k0;
+        release(seg);
         for (int r = 0; r < tiles && ok; ++r) {
           ok = all_ok(mbar_wait_relaxed(&tail->q_full[r], nq[r]++ & 1, abort_flag, p.status, ST_TIMEOUT_TMA_FULL, 32));
           if (ok && r == 0) ok = wait_tile(i);
@@ -299,6 +405,23 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
           }
         }
       }
+    } else if (warp == 2) {
+      // ------------------------------ the run ------------------------------
+      KvWideWalk walk(p);
+      unsigned i = 0;
+      bool ok = true;
+      for (bool more = true; more; ++i) {
+        KvWideSegment g;
+        more = walk.next(p, g);
+        if (!more) g.k1 = 0;
+        ok = all_ok(mbar_wait_relaxed(&tail->seg_empty[i % SEGS], (i / SEGS & 1) ^ 1, abort_flag, p.status, ST_TIMEOUT_STAGE_EMPTY, 64));
+        if (!ok) break;
+        if (lane == 0) {
+          tail->seg[i % SEGS] = g;
+          mbar_arrive(&tail->seg_full[i % SEGS]);
+        }
+        __syncwarp();
+      }
     }
   } else if (warp >= 20) {
     // ============================ conversion: codes -> fp16 tiles ============================
@@ -313,16 +436,20 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
     const int second = (q / 4) * TK * 128 + r0 * 128 + (((chunk + 1 - swap) ^ (r0 & 7)) << 4);
     unsigned i = v, tiles = 0;   // tile of the rings, tiles
     bool ok = true;
-    while (ok && walk.next(p.r, p.c.page_log2, p.c.heads, p.group, g)) {
-      const int kend = kv_wide_end(p, g);
+    for (unsigned seg = 0;; ++seg) {
+      const bool more = segment(seg, ok);
+      if (v ? !ok : bar_sync_or(5, 128, !ok)) break;   // the K warps leave together: they have barriers
+      if (!more) break;
+      const KvWideSegment g = tail->seg[seg % SEGS];
+      release(seg);
       int e = -60;   // exponent of the unit's V; scales below 2^-60 count as 0
-      for (int kt = g.k0; kt < kend; ++kt, i += 2, ++tiles) {
+      for (int kt = g.k0; kt < g.k1; ++kt, i += 2, ++tiles) {
         const KvTile t = kv_wide_tile(p, g, kt);
         const int parity = tiles & 1;
         const int s = i % RAW;
         ok = all_ok(mbar_wait(&tail->raw_full[i % (2 * RAW)], i / (2 * RAW) & 1, abort_flag, p.status, ST_TIMEOUT_TMA_FULL) &&
                     mbar_wait(&tail->empty[i % SLOTS], (i / SLOTS & 1) ^ 1, abort_flag, p.status, ST_TIMEOUT_STAGE_EMPTY));
-        if (!ok && v) break;   // the K warps leave together, behind their barrier
+        if (!ok && v) break;
         const uint32_t pages = tail->pages[s];
         const bool whole = pages == (0xffffffffu >> (32 - (TK >> p.c.page_log2))) && t.kt * TK + TK <= t.len;
         auto there = [&](int key) { return whole || (t.kt * TK + key < t.len && ((pages >> (key >> p.c.page_log2)) & 1u)); };
@@ -403,44 +530,56 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
     unsigned ns = 0, no = 0;   // uses of s_full and o_full
     int parity = 0;
     bool ok = true;
-    while (ok && walk.next(p.r, p.c.page_log2, p.c.heads, p.group, g)) {
-      const int kend = kv_wide_end(p, g), n = kend - g.k0;
+    constexpr int LANES = D / 8, ROWS = 32 / LANES, N = 16 / ROWS;   // lanes of a row of Q, rows of a load, loads of the warp's 16 rows
+    const int ch = lane % LANES, q_row = ((warp - 4) & 7) * 16 + lane / LANES;
+    unsigned seg = 0;
+    bool more = segment(0, ok);
+    ok = !bar_sync_or(3 + rt, 256, !ok);   // the warps of a row tile leave together
+    while (ok && more) {
+      const KvWideSegment& g = tail->seg[seg % SEGS];
+      const int n = g.k1 - g.k0;
       if (rt >= kv_wide_row_tiles(p, g)) {   // no rows for this tile
         parity ^= n & 1;
+        release(seg);
+        more = segment(++seg, ok);
+        ok = !bar_sync_or(3 + rt, 256, !ok);
         continue;
       }
-      // ---- 16 rows of Q as fp16 into their tile, D / 8 lanes to a row, all loads in flight ----
+      float(*row_of)[128] = tail->row[seg & 1][rt];
+      // ---- the rows of Q as fp16 into their tile, all loads in flight ----
       {
-        constexpr int LANES = D / 8, ROWS = 32 / LANES, N = 16 / ROWS;
-        const int ch = lane % LANES, r0 = ((warp - 4) & 7) * 16 + lane / LANES;
         uint4 x[N];
+        const int flat = g.u * WBM + rt * 128 + q_row;
+        int tok = flat / p.group, hh = flat - tok * p.group;
+        const uint16_t* src = p.q + static_cast<int64_t>(g.first) * p.q_st + static_cast<int64_t>(g.h) * p.group * p.q_sh + ch * 8;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-          const int flat = g.u * WBM + rt * 128 + r0 + k * ROWS, tok = flat / p.group, hh = flat - tok * p.group;
-          const int64_t at = static_cast<int64_t>(g.s.first + tok) * p.q_st + (static_cast<int64_t>(g.h) * p.group + hh) * p.q_sh + ch * 8;
-          x[k] = tok < g.s.n ? ld_global_16(p.q + at) : make_uint4(0, 0, 0, 0);
+          x[k] = tok < g.n ? ld_global_16(src + tok * p.q_st + hh * p.q_sh) : make_uint4(0, 0, 0, 0);
+          for (hh += ROWS; hh >= p.group; hh -= p.group) ++tok;
+        }
+        if (p.is_f16) {   // as it is
+          if (lane < 16) row_of[0][((warp - 4) & 7) * 16 + lane] = p.sl2;
+        } else {
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+            float amax = 0.f, up, down;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) amax = max_3(amax, fabsf(bf16_lo(w[y])), fabsf(bf16_hi(w[y])));
+#pragma unroll
+            for (int o = LANES / 2; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            kv_row_factor(amax, up, down);
+            if (ch == 0) row_of[0][q_row + k * ROWS] = fmaxf(p.sl2 * down, 0x1p-126f);   // not 0: a masked score is -inf
+#pragma unroll
+            for (int y = 0; y < 4; ++y) w[y] = pack_half2(bf16_lo(w[y]) * up, bf16_hi(w[y]) * up);
+            x[k] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
         }
         uint8_t* dst = smem + rt * L::Q_BYTES + (ch / 8) * 128 * 128;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-          uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
-          float amax = 0.f, up, down;
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const float2 f = kv_unpack(w[y], p.is_f16);
-            amax = max_3(amax, fabsf(f.x), fabsf(f.y));
-          }
-#pragma unroll
-          for (int o = LANES / 2; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-          kv_row_factor(amax, up, down);
-          const int row = r0 + k * ROWS;
-          if (ch == 0) tail->row[rt][0][row] = fmaxf(p.sl2 * down, 0x1p-126f);   // not 0: a masked score is -inf
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const float2 f = kv_unpack(w[y], p.is_f16);
-            w[y] = pack_half2(f.x * up, f.y * up);
-          }
-          *reinterpret_cast<uint4*>(dst + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          const int r = q_row + k * ROWS;
+          *reinterpret_cast<uint4*>(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x[k];
         }
         fence_proxy_async_smem();
         tile_bar();
@@ -448,13 +587,13 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
       }
       // of the thread's two rows: factor, the last own key that is seen, maximum (of t) and sum
       const int warp_first = (g.u * WBM + rt * 128 + quad * 32 + half * 16) / p.group;   // token of the warp's first row: it sees least
-      const int warp_last = p.causal ? g.s.len - g.s.n + warp_first : g.s.len - 1;
+      const int warp_last = p.causal ? g.len - g.n + warp_first : g.len - 1;
       uint64_t c2[2];
       float m[2], l[2];
       int e = 0;   // of O as it is
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const float c = tail->row[rt][0][frag_row + 8 * k];
+        const float c = row_of[0][frag_row + 8 * k];
         c2[k] = pk2(c, c);
         m[k] = -INFINITY, l[k] = 0.f;
       }
@@ -482,7 +621,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
             top[k] = -INFINITY;
             sum[k] = pk2(0.f, 0.f);
             if constexpr (decltype(mask)::value)
-              last[k] = cut ? g.s.len - g.s.n + (g.u * WBM + rt * 128 + frag_row + 8 * k) / p.group - key0 - 2 * (lane & 3) : TK;
+              last[k] = cut ? g.len - g.n + (g.u * WBM + rt * 128 + frag_row + 8 * k) / p.group - key0 - 2 * (lane & 3) : TK;
           }
           uint32_t r[2][8];
           float2 key[2][2];   // of the column pairs, fetched 16 columns ahead as S is
@@ -526,12 +665,29 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
             top[k] *= c;
           }
         };
+        if (j == 0) {   // m to begin with: the maximum of the first 16 columns mostly within 2^12 of that of all
+          uint32_t r[8];
+          tmem_ld_frag2(s_frag, r);
+          tmem_ld_wait8(r);
+          const float2 a = *reinterpret_cast<const float2*>(ks), b = *reinterpret_cast<const float2*>(ks + 8);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float c, same;
+            upk2(c2[k], c, same);
+            float t = max_3(__uint_as_float(r[2 * k]) * a.x, __uint_as_float(r[2 * k + 1]) * a.y,
+                            fmaxf(__uint_as_float(r[4 + 2 * k]) * b.x, __uint_as_float(r[5 + 2 * k]) * b.y)) * c;
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+            m[k] = masked || !(fabsf(t) < INFINITY) ? -INFINITY : t;
+          }
+          e = e_new;
+        }
         auto either = [&] {
           if (masked) pass(std::true_type());
           else pass(std::false_type());
         };
         either();
-        bool grew = j == 0 || e_new != e;
+        bool grew = e_new != e;
 #pragma unroll
         for (int k = 0; k < 2; ++k) grew |= top[k] > m[k] + kSlack || (m[k] == -INFINITY && top[k] > m[k]);
         if (__any_sync(0xffffffffu, grew)) {
@@ -577,6 +733,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
         if (lane == 0) mbar_arrive(&tail->p_full[rt]);
       }
       ok = ok && all_ok(mbar_wait(&tail->o_full[rt], no++ & 1, abort_flag, p.status, ST_TIMEOUT_PV_DONE));
+      if (ok) more = segment(seg + 1, ok);
       tc_fence_after();
       // ---- sums and maxima to the threads of the rows ----
 #pragma unroll
@@ -584,24 +741,33 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
         float x = l[k];
         x += __shfl_xor_sync(0xffffffffu, x, 1);
         x += __shfl_xor_sync(0xffffffffu, x, 2);
-        if ((lane & 3) == 0) tail->row[rt][0][frag_row + 8 * k] = x, tail->row[rt][1][frag_row + 8 * k] = m[k];
+        if ((lane & 3) == 0) row_of[0][frag_row + 8 * k] = x, row_of[1][frag_row + 8 * k] = m[k];
       }
       if (bar_sync_or(3 + rt, 256, !ok)) {
         ok = false;
         break;
       }
+      if (more && lane < 16) {   // the next unit's rows of Q are in L2 by then
+        const KvWideSegment& a = tail->seg[(seg + 1) % SEGS];
+        const int next = a.u * WBM + rt * 128 + ((warp - 4) & 7) * 16 + lane, tok = next / p.group;
+        if (tok < a.n) {
+          const uint16_t* q = p.q + static_cast<int64_t>(a.first + tok) * p.q_st + (static_cast<int64_t>(a.h) * p.group + (next - tok * p.group)) * p.q_sh;
+          prefetch_l2(q);
+          if (D == 128) prefetch_l2(q + 64);
+        }
+      }
       const int flat = g.u * WBM + rt * 128 + row, tok = flat / p.group, hh = flat - tok * p.group;
-      const bool there = tok < g.s.n;
-      const int64_t t = g.s.first + tok, head = static_cast<int64_t>(g.h) * p.group + hh;
-      const float l_row = tail->row[rt][0][row], m_row = tail->row[rt][1][row];
+      const bool there = tok < g.n;
+      const int64_t t = g.first + tok, head = static_cast<int64_t>(g.h) * p.group + hh;
+      const float l_row = row_of[0][row], m_row = row_of[1][row];
       const uint32_t o_row = o_base + half * (D / 2);   // this thread's half of the row's channels
-      const bool part = !PREFIX && (g.k0 > 0 || g.k1 < g.s.kt);
+      const bool part = !PREFIX && g.parts > 1;
       if (PREFIX || part) {
         // as the narrow kernel means it: weights 2^(t + log2 vs - m + 15) for the codes, their sum against vs
         const float m_out = m_row + kSlack + static_cast<float>(e), l_out = l_row * kv_ex2(static_cast<float>(-e));
         float* dst;   // of the prefix's rows; a partial result is [D / 4][256 rows] float4, so that lanes write, and a join reads, side by side
         if (PREFIX) {
-          const int64_t at = (static_cast<int64_t>(blockIdx.x - g.x / run.run) * p.c.heads + g.h) * p.r.T * p.group + flat;
+          const int64_t at = (static_cast<int64_t>(blockIdx.x - g.cta) * p.c.heads + g.h) * p.r.T * p.group + flat;
           dst = p.pre_o + at * D + half * (D / 2);
           if (there && half == 0) *reinterpret_cast<float2*>(p.pre_ml + 2 * at) = make_float2(m_out, l_out);
         } else {
@@ -611,34 +777,29 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
         }
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[16];
-          tmem_ld16_async(o_row + c * 16, o);
-          tmem_ld_wait16(o);
+          uint32_t v[16];
+          tmem_ld16_async(o_row + c * 16, v);
+          tmem_ld_wait16(v);
           if (!PREFIX) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              reinterpret_cast<uint4*>(dst)[(c * 4 + k) * WBM] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+              reinterpret_cast<uint4*>(dst)[(c * 4 + k) * WBM] = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
           } else if (there) {
-            st_global_32(dst + c * 16, make_uint4(o[0], o[1], o[2], o[3]), make_uint4(o[4], o[5], o[6], o[7]));
-            st_global_32(dst + c * 16 + 8, make_uint4(o[8], o[9], o[10], o[11]), make_uint4(o[12], o[13], o[14], o[15]));
+            st_global_32(dst + c * 16, make_uint4(v[0], v[1], v[2], v[3]), make_uint4(v[4], v[5], v[6], v[7]));
+            st_global_32(dst + c * 16 + 8, make_uint4(v[8], v[9], v[10], v[11]), make_uint4(v[12], v[13], v[14], v[15]));
           }
         }
-        if (part && warp == 4 && lane == 0) {
-          const int slot = g.k0 > 0 ? 0 : 1;
-          tail->join[slot] = g;
-          tail->first[slot] = g.x / run.run;
-          tail->parts[slot] = (g.x + g.s.kt - 1) / run.run - g.x / run.run + 1;
-        }
+        if (part && warp == 4 && lane == 0) tail->join[g.k0 > 0 ? 0 : 1] = g, tail->parts[g.k0 > 0 ? 0 : 1] = g.parts;
       } else {
         const float inv = l_row == 0.f ? 0.f : __fdiv_rn(kv_ex2(static_cast<float>(e)), l_row);   // no key: 0
         uint16_t* dst = p.out + t * p.o_st + head * p.o_sh + half * (D / 2);
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[16], w[8];
-          tmem_ld16_async(o_row + c * 16, o);
-          tmem_ld_wait16(o);
+          uint32_t v[16], w[8];
+          tmem_ld16_async(o_row + c * 16, v);
+          tmem_ld_wait16(v);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) w[k] = kv_pack(__uint_as_float(o[2 * k]) * inv, __uint_as_float(o[2 * k + 1]) * inv, p.is_f16);
+          for (int k = 0; k < 8; ++k) w[k] = kv_pack(__uint_as_float(v[2 * k]) * inv, __uint_as_float(v[2 * k + 1]) * inv, p.is_f16);
           if (there && (reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
             st_global_32(dst + c * 16, make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7]));
           } else if (there) {
@@ -648,7 +809,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
         }
       }
       tc_fence_before();   // O has been read: the next unit's products may write it behind the next p_full
-      tile_bar();          // and `row` has been
+      release(seg++);
     }
     // ---- the run is done: its parts are counted, and units whose last parts they are joined, a row per thread ----
     if (!PREFIX) {
@@ -656,7 +817,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
       if (!bar_sync_or(1, 512, !ok)) {
         const int tid = threadIdx.x - 128;
         if (tid < 2 && tail->parts[tid]) {
-          const int first = tail->first[tid];
+          const int first = tail->join[tid].cta;
           if (atomicAdd(p.count + first, 1) == tail->parts[tid] - 1) p.count[first] = 0;   // nobody else comes
           else tail->parts[tid] = 0;
           __threadfence();
@@ -664,12 +825,12 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
         asm volatile("bar.sync 2, 512;" ::: "memory");
 #pragma unroll 1
         for (int k = 0; k < 2; ++k) {
-          const int parts = tail->parts[k], first = tail->first[k];
+          const int parts = tail->parts[k], first = tail->join[k].cta;
           if (!parts) continue;
-          const KvSegment& u = tail->join[k];
+          const KvWideSegment& u = tail->join[k];
           const int row = tid & 255, half = tid >> 8;
           const int flat = u.u * WBM + row, tok = flat / p.group, hh = flat - tok * p.group;
-          if (tok >= u.s.n) continue;
+          if (tok >= u.n) continue;
           const int at = WBM * D + row;
           float m = -INFINITY, l = 0.f;
           for (int i2 = 0; i2 < parts; ++i2) m = fmaxf(m, __ldcg(p.part + kv_slot(first, i2) * L::PART + at));
@@ -679,7 +840,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
             l = fmaf(__ldcg(slot + WBM), kv_ex2(__ldcg(slot) - m), l);
           }
           const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
-          uint16_t* dst = p.out + (u.s.first + static_cast<int64_t>(tok)) * p.o_st + (static_cast<int64_t>(u.h) * p.group + hh) * p.o_sh;
+          uint16_t* dst = p.out + (u.first + static_cast<int64_t>(tok)) * p.o_st + (static_cast<int64_t>(u.h) * p.group + hh) * p.o_sh;
 #pragma unroll 1
           for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
             float o[32];
