@@ -416,13 +416,17 @@ typedef struct rh3_kv_attn_args {
   const int32_t* prefix_table; int64_t prefix_pages, prefix;
   float scale; int32_t kind, dtype, causal;
 } rh3_kv_attn_args;
-int rh3_kv_write(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, int dtype, void* kc,
-                 void* vc, float* ks, float* vs, int64_t pages, int64_t heads, int64_t page, int64_t D, int kind,
-                 const int32_t* table, int64_t table_stride, int64_t per_seq, const int32_t* lens, const int32_t* starts,
-                 int64_t B, int64_t T, cudaStream_t stream);
-int rh3_kv_read(const void* kc, const void* vc, const float* ks, const float* vs, int64_t pages, int64_t heads, int64_t page,
-                int64_t D, int kind, const int32_t* table, int64_t table_stride, int64_t per_seq, const int32_t* lens,
-                const int32_t* starts, int64_t B, int64_t T, void* k, void* v, int dtype, cudaStream_t stream);
+typedef struct rh3_kv_rows_args {      /* what rh3_kv_write and rh3_kv_read move */
+  void* k; int64_t k_st, k_sh;         /* [T][heads][D], token and head strides (write only: read puts out contiguous rows) */
+  void* v; int64_t v_st, v_sh;
+  void* kc; void* vc; float* ks; float* vs;
+  int64_t pages, heads, page, D;
+  const int32_t* table; int64_t table_stride, per_seq;
+  const int32_t* lens; const int32_t* starts; int64_t B, T;
+  int32_t kind, dtype;
+} rh3_kv_rows_args;
+int rh3_kv_write(const rh3_kv_rows_args* a, cudaStream_t stream);
+int rh3_kv_read(const rh3_kv_rows_args* a, cudaStream_t stream);
 int64_t rh3_kv_attn_workspace_bytes(int64_t heads, int64_t group, int64_t page, int64_t D, int64_t per_seq, int64_t B, int64_t T,
                                     int64_t prefix);
 int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t workspace_bytes, int32_t* counters, cudaStream_t stream);

@@ -75,8 +75,8 @@ SIGNATURES = {
     "rh3_gn_silu_from_sums": [_P, _P, _D, _D, _P, _P, _I64, _I64, _I64, _P, _P],
     "rh3_block_workspace_bytes": [_P],
     "rh3_block_forward": [_P, _P, _I64, _P],
-    "rh3_kv_write": [_P, _I64, _I64, _P, _I64, _I64, _I, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _I64, _P, _P, _I64, _I64, _P],
-    "rh3_kv_read": [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _I, _P],
+    "rh3_kv_write": [_P, _P],
+    "rh3_kv_read": [_P, _P],
     "rh3_kv_attn_workspace_bytes": [_I64] * 8,
     "rh3_kv_attn": [_P, _P, _I64, _P, _P],
     "rh3_upsample_causal2x": [_P, _P, _I64, _I64, _I64, _I64, _I64, _P],

@@ -643,7 +643,8 @@ template <int D, int FMT, int MODE, int NT>
 int kv_launch(const CUtensorMap& mk, const CUtensorMap& mv, const KvAttnParams& p, int64_t grid, cudaStream_t stream) {
   auto kern = kv_attn_kernel<D, FMT, MODE, NT>;
   const int smem = kv_narrow_smem<D, NT>();
-  if (int e = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "kv_attn smem attribute")) return e;
+  static std::atomic<uint64_t> allowed{0};
+  if (int e = kv_allow_smem(kern, smem, allowed)) return e;
   return check_cuda(launch_chained(kern, dim3(static_cast<unsigned>(grid)), KV_NT, smem, stream, 1, mk, mv, p), "kv_attn launch");
 }
 

@@ -9,6 +9,8 @@
 // factor 2^15 keeps weights down to 2^-29 of the largest at that precision (normal numbers), so that the tail of a long context is not lost;
 // products, sums, m, l and O are fp32. Partial results over parts of the keys carry (O, m, l) with the same m for both.
 #pragma once
+#include <atomic>
+
 #include "kv_cache.cuh"
 #include "rapidh3_b200.h"
 
@@ -98,6 +100,18 @@ __device__ __forceinline__ float2 kv_unpack(uint32_t w, int is_f16) {
   return make_float2(bf16_lo(w), bf16_hi(w));
 }
 __device__ __forceinline__ uint32_t kv_pack(float a, float b, int is_f16) { return is_f16 ? pack_half2(a, b) : pack_bf16x2(a, b); }
+
+// Lets `kern` have `smem` bytes of shared memory, once per device; `done` is the kernel's own word, a bit per device.
+template <class K>
+int kv_allow_smem(K kern, int smem, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (int e = check_cuda(cudaGetDevice(&dev), "kv_attn device")) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return 0;
+  if (int e = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "kv_attn smem attribute")) return e;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return 0;
+}
 
 // kv_attn_wide.cu: the same parameters, units of 256 rows; floats of one of its partial results
 constexpr int KV_WIDE_BM = 256;

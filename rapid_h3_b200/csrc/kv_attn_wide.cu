@@ -886,7 +886,8 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
 template <int D, int FMT, bool PREFIX>
 int kv_wide_start(const KvAttnParams& p, int64_t grid, cudaStream_t stream) {
   auto kern = kv_wide_kernel<D, FMT, PREFIX>;
-  if (int e = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kv_wide_smem<D>()), "kv_attn smem attribute")) return e;
+  static std::atomic<uint64_t> allowed{0};
+  if (int e = kv_allow_smem(kern, kv_wide_smem<D>(), allowed)) return e;
   return check_cuda(launch_chained(kern, dim3(static_cast<unsigned>(grid)), WTHREADS, kv_wide_smem<D>(), stream, 1, p), "kv_attn (wide) launch");
 }
 

@@ -269,46 +269,43 @@ int kv_fill_rows(KvRows* r, const char* what, const int32_t* table, int64_t tabl
 
 using namespace rh3;
 
-extern "C" int rh3_kv_write(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, int dtype, void* kc,
-                            void* vc, float* ks, float* vs, int64_t pages, int64_t heads, int64_t page, int64_t D, int kind,
-                            const int32_t* table, int64_t table_stride, int64_t per_seq, const int32_t* lens, const int32_t* starts,
-                            int64_t B, int64_t T, cudaStream_t stream) {
+extern "C" int rh3_kv_write(const rh3_kv_rows_args* a, cudaStream_t stream) {
+  RH3_CHECK_ARG(a, "kv_write: null arguments");
   KvWriteParams p{};
-  RH3_CHECK_ARG(dtype >= 0 && dtype <= 2, "kv_write: dtype=%d must be 0 (bf16), 1 (fp16) or 2 (fp32)", dtype);
-  if (int e = kv_fill_cache(&p.c, "kv_write", kc, vc, ks, vs, pages, heads, page, D, kind)) return e;
-  if (int e = kv_fill_rows(&p.r, "kv_write", table, table_stride, per_seq, lens, starts, B, T)) return e;
-  if (T == 0) return 0;
-  const int64_t per16 = dtype == KV_F32 ? 4 : 8;
-  RH3_CHECK_ARG(k && v && kv_a16(k) && kv_a16(v) && k_st % per16 == 0 && k_sh % per16 == 0 && v_st % per16 == 0 && v_sh % per16 == 0,
+  RH3_CHECK_ARG(a->dtype >= 0 && a->dtype <= 2, "kv_write: dtype=%d must be 0 (bf16), 1 (fp16) or 2 (fp32)", a->dtype);
+  if (int e = kv_fill_cache(&p.c, "kv_write", a->kc, a->vc, a->ks, a->vs, a->pages, a->heads, a->page, a->D, a->kind)) return e;
+  if (int e = kv_fill_rows(&p.r, "kv_write", a->table, a->table_stride, a->per_seq, a->lens, a->starts, a->B, a->T)) return e;
+  if (a->T == 0) return 0;
+  const int64_t per16 = a->dtype == KV_F32 ? 4 : 8;
+  RH3_CHECK_ARG(a->k && a->v && kv_a16(a->k) && kv_a16(a->v) && a->k_st % per16 == 0 && a->k_sh % per16 == 0 && a->v_st % per16 == 0 && a->v_sh % per16 == 0,
                 "kv_write: every row of k and v must start on a 16-byte boundary");
-  p.k = k, p.v = v, p.k_st = k_st, p.k_sh = k_sh, p.v_st = v_st, p.v_sh = v_sh;
-  p.warps_per_token = kv_warps_per_token(heads, D);
+  p.k = a->k, p.v = a->v, p.k_st = a->k_st, p.k_sh = a->k_sh, p.v_st = a->v_st, p.v_sh = a->v_sh;
+  p.warps_per_token = kv_warps_per_token(a->heads, a->D);
   p.status = device_status_word();
-  const int64_t blocks = (T * p.warps_per_token + KV_THREADS / 32 - 1) / (KV_THREADS / 32);
+  const int64_t blocks = (a->T * p.warps_per_token + KV_THREADS / 32 - 1) / (KV_THREADS / 32);
   RH3_CHECK_ARG(blocks < (1ll << 31), "kv_write: too many rows");
   const bool chained = blocks <= 4 * device_sm_count() && !in_capture(stream);
-  return kv_dispatch(D, kind, dtype, [&](auto d, auto f, auto t) {
+  return kv_dispatch(a->D, a->kind, a->dtype, [&](auto d, auto f, auto t) {
     return check_cuda(launch_kernel(chained, kv_write_kernel<d(), f(), t()>, dim3(static_cast<unsigned>(blocks)), KV_THREADS, 0, stream, 1, p),
                       "kv_write launch");
   });
 }
 
-extern "C" int rh3_kv_read(const void* kc, const void* vc, const float* ks, const float* vs, int64_t pages, int64_t heads, int64_t page,
-                           int64_t D, int kind, const int32_t* table, int64_t table_stride, int64_t per_seq, const int32_t* lens,
-                           const int32_t* starts, int64_t B, int64_t T, void* k, void* v, int dtype, cudaStream_t stream) {
+extern "C" int rh3_kv_read(const rh3_kv_rows_args* a, cudaStream_t stream) {
+  RH3_CHECK_ARG(a, "kv_read: null arguments");
   KvReadParams p{};
-  RH3_CHECK_ARG(dtype >= 0 && dtype <= 2, "kv_read: dtype=%d must be 0 (bf16), 1 (fp16) or 2 (fp32)", dtype);
-  if (int e = kv_fill_cache(&p.c, "kv_read", kc, vc, ks, vs, pages, heads, page, D, kind)) return e;
-  if (int e = kv_fill_rows(&p.r, "kv_read", table, table_stride, per_seq, lens, starts, B, T)) return e;
-  if (T == 0) return 0;
-  RH3_CHECK_ARG(k && v && kv_a16(k) && kv_a16(v), "kv_read: outputs must be set and 16-byte aligned");
-  p.k = k, p.v = v;
-  p.warps_per_token = kv_warps_per_token(heads, D);
+  RH3_CHECK_ARG(a->dtype >= 0 && a->dtype <= 2, "kv_read: dtype=%d must be 0 (bf16), 1 (fp16) or 2 (fp32)", a->dtype);
+  if (int e = kv_fill_cache(&p.c, "kv_read", a->kc, a->vc, a->ks, a->vs, a->pages, a->heads, a->page, a->D, a->kind)) return e;
+  if (int e = kv_fill_rows(&p.r, "kv_read", a->table, a->table_stride, a->per_seq, a->lens, a->starts, a->B, a->T)) return e;
+  if (a->T == 0) return 0;
+  RH3_CHECK_ARG(a->k && a->v && kv_a16(a->k) && kv_a16(a->v), "kv_read: outputs must be set and 16-byte aligned");
+  p.k = a->k, p.v = a->v;
+  p.warps_per_token = kv_warps_per_token(a->heads, a->D);
   p.status = device_status_word();
-  const int64_t blocks = (T * p.warps_per_token + KV_THREADS / 32 - 1) / (KV_THREADS / 32);
+  const int64_t blocks = (a->T * p.warps_per_token + KV_THREADS / 32 - 1) / (KV_THREADS / 32);
   RH3_CHECK_ARG(blocks < (1ll << 31), "kv_read: too many rows");
   const bool chained = blocks <= 4 * device_sm_count() && !in_capture(stream);
-  return kv_dispatch(D, kind, dtype, [&](auto d, auto f, auto t) {
+  return kv_dispatch(a->D, a->kind, a->dtype, [&](auto d, auto f, auto t) {
     return check_cuda(launch_kernel(chained, kv_read_kernel<d(), f(), t()>, dim3(static_cast<unsigned>(blocks)), KV_THREADS, 0, stream, 1, p),
                       "kv_read launch");
   });

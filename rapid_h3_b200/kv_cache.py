@@ -26,15 +26,16 @@ HEAD_DIMS = (64, 128)
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _KINDS = {"int8": (torch.int8, 0), "fp8": (FP8, 1)}
 
-# rh3_kv_attn_args: q, out, the cache and the batch (pointers, strides, sizes), then scale, kind, dtype, causal
-_ARGS = struct.Struct("@PqqPqqPPPPqqqqPqqPPqqqPqqfiii")
+# rh3_kv_attn_args and rh3_kv_rows_args: the two tensors (pointer, token and head stride), the cache, the batch, then what the call adds
+_TENSORS, _CACHE, _BATCH = struct.Struct("@PqqPqq"), struct.Struct("@PPPPqqqq"), struct.Struct("@PqqPPq")
+_ATTN, _ROWS = struct.Struct("@qqPqqfiii"), struct.Struct("@qii")
 
 
 class KVCache:
     """Codes k, v [pages, kv_heads, page, head_dim] (int8, or float8_e4m3fn) and scales k_scale, v_scale fp32 [pages, kv_heads, page],
     contiguous, on one CUDA device. page: 16, 32, 64 or 128 tokens; head_dim: 64 or 128."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page", "head_dim", "kind", "device", "_args")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page", "head_dim", "kind", "device", "_index", "_args")
 
     def __init__(self, k, v, k_scale, v_scale):
         _lib.require_cuda(k, v, k_scale, v_scale)
@@ -54,7 +55,8 @@ class KVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.device = k.device
         self.kind = 0 if k.dtype == torch.int8 else 1
-        self._args = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.pages, self.kv_heads, self.page, self.head_dim)
+        self._index = k.get_device()
+        self._args = _CACHE.pack(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.pages, self.kv_heads, self.page, self.head_dim)
 
 
 def alloc(pages, kv_heads, head_dim=128, page=64, kind="int8", device="cuda"):
@@ -90,68 +92,77 @@ class Rows:
             raise RuntimeError("lens, starts and the rows of table must be contiguous")
         if (table.shape[0] > 1 and table.stride(0) < table.shape[1]) or not table.device == lens.device == starts.device:
             raise RuntimeError("the rows of table must not overlap, and all three must be on one device")
-        object.__setattr__(self, "_args", (table.data_ptr(), max(table.stride(0), table.shape[1]), table.shape[1], lens.data_ptr(),
-                                           starts.data_ptr(), len(lens)))
+        object.__setattr__(self, "_index", table.get_device())
+        object.__setattr__(self, "_sizes", (table.shape[1], len(lens)))
+        object.__setattr__(self, "_args", _BATCH.pack(table.data_ptr(), max(table.stride(0), table.shape[1]), table.shape[1], lens.data_ptr(),
+                                                      starts.data_ptr(), len(lens)))
 
 
-# counters of the attention kernels, per (device, stream): 0 between calls, so only calls that cannot overlap share them
-_COUNTERS = {}
+# What the attention kernels need beside their arguments, per (device, stream), where only calls that cannot overlap share it: the counters,
+# which are 0 between calls, and a workspace for calls that need little (for most, allocating one takes as long as the kernel).
+_SCRATCH = {}
+_KEPT_BYTES = 4 << 20
+_NEED = {}
 
 
-def _counters(device, stream):
-    """Zeros on `device` that no call uses at the same time as one on `stream`. A captured call gets its own, cleared by the graph: a
-    graph may be replayed on any stream."""
+def _scratch(device, index, stream, need):
+    """(counters, workspace of `need` bytes) for a call on `stream`. A captured call gets its own, the counters cleared by the graph: a graph
+    may be replayed on any stream."""
     if torch._C._cuda_isCurrentStreamCapturing():
-        return torch.zeros(1024, device=device, dtype=torch.int32)
-    t = _COUNTERS.get((device.index, stream))
-    if t is None:
-        t = _COUNTERS.setdefault((device.index, stream), torch.zeros(1024, device=device, dtype=torch.int32))
-    return t
+        return torch.zeros(1024, device=device, dtype=torch.int32), torch.empty(need, device=device, dtype=torch.uint8)
+    kept = _SCRATCH.get((index, stream))
+    if kept is None:
+        kept = _SCRATCH.setdefault((index, stream), (torch.zeros(1024, device=device, dtype=torch.int32),
+                                                     torch.empty(_KEPT_BYTES, device=device, dtype=torch.uint8)))
+    return kept if need <= _KEPT_BYTES else (kept[0], torch.empty(need, device=device, dtype=torch.uint8))
 
 
-class _on:
-    """The device a call's work goes to; entering it costs nothing where it is the current one."""
+def _workspace_bytes(*sizes):
+    need = _NEED.get(sizes)
+    if need is None:
+        if len(_NEED) > 4096:
+            _NEED.clear()
+        need = _NEED[sizes] = _lib.lib().rh3_kv_attn_workspace_bytes(*sizes)
+    return need
 
-    __slots__ = ("guard",)
 
-    def __init__(self, device):
-        self.guard = None if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _run(index, fn):
+    """fn() with device `index` current: the library works on the current device and its stream."""
+    if index == torch._C._cuda_getDevice():
+        return fn()
+    with torch.cuda.device(index):
+        return fn()
 
 
 def _check_batch(cache, rows):
-    if rows.table.device != cache.device:
+    if rows._index != cache._index:
         raise RuntimeError("the batch must be on the cache's device")
 
 
 def _check_rows(x, name, cache, heads, types):
-    if not x.is_cuda or x.device != cache.device:
+    """(pointer, token stride, head stride) of x [T, heads, head_dim]."""
+    if x.get_device() != cache._index:
         raise RuntimeError(f"{name} must be a CUDA tensor on the cache's device; there is no CPU path")
-    if x.ndim != 3 or x.dtype not in types or x.shape[2] != cache.head_dim or (heads is not None and x.shape[1] != heads):
-        raise RuntimeError(f"{name}: expected [T, {heads or 'heads'}, {cache.head_dim}] of {', '.join(str(t) for t in types)}, got {tuple(x.shape)} {x.dtype}")
+    shape = x.shape
+    if len(shape) != 3 or x.dtype not in types or shape[2] != cache.head_dim or (heads is not None and shape[1] != heads):
+        raise RuntimeError(f"{name}: expected [T, {heads or 'heads'}, {cache.head_dim}] of {', '.join(str(t) for t in types)}, got {tuple(shape)} {x.dtype}")
+    st, sh, unit = x.stride()
+    ptr = x.data_ptr()
     per16 = 16 // x.element_size()
-    if x.numel() and (x.stride(2) != 1 or x.stride(0) % per16 or x.stride(1) % per16 or x.data_ptr() % 16):
+    if (unit != 1 or st % per16 or sh % per16 or ptr % 16) and x.numel():
         raise RuntimeError(f"{name}: the last dim must be contiguous and every row start on a 16-byte boundary")
+    return ptr, st, sh
 
 
 def write(cache, k, v, rows):
     """Quantize k, v [T, kv_heads, head_dim] (bf16, fp16 or fp32, any token and head strides of whole 16 bytes) into the pages of
     their sequences. A row with a NaN or an infinity reads back as NaN. Sequences that share a page must not write the same token."""
     _check_batch(cache, rows)
-    _check_rows(k, "k", cache, cache.kv_heads, tuple(_DTYPES))
-    _check_rows(v, "v", cache, cache.kv_heads, (k.dtype,))
+    at = (*_check_rows(k, "k", cache, cache.kv_heads, tuple(_DTYPES)), *_check_rows(v, "v", cache, cache.kv_heads, (k.dtype,)))
     if v.shape != k.shape:
         raise RuntimeError("k and v must have the same number of rows")
-    with _on(cache.device):
-        _lib.call("rh3_kv_write", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _DTYPES[k.dtype],
-                  *cache._args, cache.kind, *rows._args, k.shape[0], _lib.stream())
+    args = _TENSORS.pack(*at) + cache._args + rows._args + _ROWS.pack(k.shape[0], cache.kind, _DTYPES[k.dtype])
+    _run(cache._index, lambda: _lib.call("rh3_kv_write", args, _lib.stream()))
 
 
 def read(cache, rows, total, dtype=torch.bfloat16, out=None):
@@ -168,14 +179,14 @@ def read(cache, rows, total, dtype=torch.bfloat16, out=None):
         for t in (k, v):
             if t.shape != shape or t.dtype != dtype or t.device != cache.device or not t.is_contiguous() or t.data_ptr() % 16:
                 raise RuntimeError(f"out: expected two contiguous, 16-byte aligned {dtype} tensors {shape} on the cache's device")
-    with _on(cache.device):
-        _lib.call("rh3_kv_read", *cache._args, cache.kind, *rows._args, total, k.data_ptr(), v.data_ptr(), _DTYPES[dtype], _lib.stream())
+    args = _TENSORS.pack(k.data_ptr(), 0, 0, v.data_ptr(), 0, 0) + cache._args + rows._args + _ROWS.pack(total, cache.kind, _DTYPES[dtype])
+    _run(cache._index, lambda: _lib.call("rh3_kv_read", args, _lib.stream()))
     return k, v
 
 
 def _attend(q, cache, rows, prefix, prefix_len, scale, causal, out):
     _check_batch(cache, rows)
-    _check_rows(q, "q", cache, None, (torch.bfloat16, torch.float16))
+    at = _check_rows(q, "q", cache, None, (torch.bfloat16, torch.float16))
     t, heads, d = q.shape
     if heads == 0 or heads % cache.kv_heads:
         raise RuntimeError(f"{heads} query heads are not a multiple of the cache's {cache.kv_heads}")
@@ -183,23 +194,26 @@ def _attend(q, cache, rows, prefix, prefix_len, scale, causal, out):
     if not 0 < scale < float("inf"):
         raise RuntimeError("the softmax scale must be positive and finite")
     if out is None:
-        out = torch.empty((t, heads, d), device=q.device, dtype=q.dtype)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        to = out.data_ptr(), heads * d, d
     else:
-        _check_rows(out, "out", cache, heads, (q.dtype,))
+        to = _check_rows(out, "out", cache, heads, (q.dtype,))
         if out.shape != q.shape:
             raise RuntimeError("out must have the shape of q")
     if t == 0:
         return out
     group = heads // cache.kv_heads
-    table, stride, per_seq, lens, starts, batch = rows._args
-    with _on(cache.device):
-        need = _lib.lib().rh3_kv_attn_workspace_bytes(cache.kv_heads, group, cache.page, d, per_seq, batch, t, prefix_len)
-        work = torch.empty(need, device=q.device, dtype=torch.uint8)
-        args = _ARGS.pack(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), *cache._args, table, stride,
-                          per_seq, lens, starts, batch, t, group, prefix.data_ptr() if prefix is not None else 0,
-                          prefix.numel() if prefix is not None else 0, prefix_len, scale, cache.kind, _DTYPES[q.dtype], bool(causal))
+    pre, pre_pages = (0, 0) if prefix is None else (prefix.data_ptr(), prefix.numel())
+    args = (_TENSORS.pack(*at, *to) + cache._args + rows._args
+            + _ATTN.pack(t, group, pre, pre_pages, prefix_len, scale, cache.kind, _DTYPES[q.dtype], bool(causal)))
+
+    def launch():
         stream = _lib.stream()
-        _lib.call("rh3_kv_attn", args, work.data_ptr(), need, _counters(q.device, stream).data_ptr(), stream)
+        need = _workspace_bytes(cache.kv_heads, group, cache.page, d, *rows._sizes, t, prefix_len)
+        counters, work = _scratch(q.device, cache._index, stream, need)
+        _lib.call("rh3_kv_attn", args, work.data_ptr(), need, counters.data_ptr(), stream)
+
+    _run(cache._index, launch)
     return out
 
 

@@ -10,25 +10,23 @@ from rapid_h3_b200 import _lib, kv_cache
 P = 4096  # an address that is never touched: the argument checks come first
 
 
-def write_args(**kw):
-    a = dict(k=P, k_st=1024, k_sh=128, v=P, v_st=1024, v_sh=128, dtype=0, kc=P, vc=P, ks=P, vs=P, pages=8, heads=8, page=64, D=128, kind=0, table=P,
-             table_stride=4, per_seq=4, lens=P, starts=P, B=2, T=3, stream=None)
-    a.update(kw)
-    return list(a.values())
+CACHE_ARGS = dict(kc=P, vc=P, ks=P, vs=P, pages=8, heads=8, page=64, D=128)
+BATCH_ARGS = dict(table=P, table_stride=4, per_seq=4, lens=P, starts=P, B=2)
 
 
-def read_args(**kw):
-    a = dict(kc=P, vc=P, ks=P, vs=P, pages=8, heads=8, page=64, D=128, kind=0, table=P, table_stride=4, per_seq=4, lens=P, starts=P, B=2, T=3,
-             k=P, v=P, dtype=0, stream=None)
-    a.update(kw)
-    return list(a.values())
+def pack(a):
+    v = list(a.values())
+    tail = kv_cache._ROWS if len(v) == 23 else kv_cache._ATTN
+    return kv_cache._TENSORS.pack(*v[:6]) + kv_cache._CACHE.pack(*v[6:14]) + kv_cache._BATCH.pack(*v[14:20]) + tail.pack(*v[20:])
+
+
+def rows_args(**kw):
+    return pack(dict(k=P, k_st=1024, k_sh=128, v=P, v_st=1024, v_sh=128, **CACHE_ARGS, **BATCH_ARGS, T=3, kind=0, dtype=0) | kw)
 
 
 def attn_args(**kw):
-    a = dict(q=P, q_st=1024, q_sh=128, out=P, o_st=1024, o_sh=128, k=P, v=P, ks=P, vs=P, pages=8, heads=2, page=64, D=128, table=P, table_stride=4,
-             per_seq=4, lens=P, starts=P, B=2, T=3, group=4, prefix_table=0, prefix_pages=0, prefix=0, scale=0.1, kind=0, dtype=0, causal=1)
-    a.update(kw)
-    return kv_cache._ARGS.pack(*a.values())
+    return pack(dict(q=P, q_st=1024, q_sh=128, out=P, o_st=1024, o_sh=128, **(CACHE_ARGS | dict(heads=2)), **BATCH_ARGS, T=3, group=4, prefix_table=0,
+                     prefix_pages=0, prefix=0, scale=0.1, kind=0, dtype=0, causal=1) | kw)
 
 
 CACHE = [(dict(kind=2), b"kind"), (dict(kind=-1), b"kind"), (dict(D=96), b"head size"), (dict(page=8), b"16, 32, 64 or 128"), (dict(page=48), b"16, 32, 64 or 128"),
@@ -40,12 +38,12 @@ BATCH = [(dict(B=0), b"bad batch"), (dict(B=1 << 20), b"bad batch"), (dict(per_s
 
 @pytest.mark.parametrize("change,said", CACHE + BATCH + [(dict(dtype=3), b"dtype"), (dict(k=P + 2), b"16-byte"), (dict(v_sh=100), b"16-byte"), (dict(k_st=1), b"16-byte")])
 def test_write_refuses(change, said):
-    assert _lib.lib().rh3_kv_write(*write_args(**change)) < 0 and said in _lib.lib().rh3_last_error_string()
+    assert _lib.lib().rh3_kv_write(rows_args(**change), None) < 0 and said in _lib.lib().rh3_last_error_string()
 
 
 @pytest.mark.parametrize("change,said", CACHE + BATCH + [(dict(dtype=-1), b"dtype"), (dict(k=P + 8), b"aligned"), (dict(v=0), b"must be set")])
 def test_read_refuses(change, said):
-    assert _lib.lib().rh3_kv_read(*read_args(**change)) < 0 and said in _lib.lib().rh3_last_error_string()
+    assert _lib.lib().rh3_kv_read(rows_args(**change), None) < 0 and said in _lib.lib().rh3_last_error_string()
 
 
 @pytest.mark.parametrize("change,said", CACHE + BATCH + [
@@ -66,7 +64,8 @@ def test_attention_refuses(change, said):
 
 def test_calls_without_rows_do_nothing():
     lib = _lib.lib()
-    assert lib.rh3_kv_write(*write_args(T=0, k=0, v=0)) == 0 and lib.rh3_kv_read(*read_args(T=0, k=0, v=0)) == 0
+    assert lib.rh3_kv_write(rows_args(T=0, k=0, v=0), None) == 0 and lib.rh3_kv_read(rows_args(T=0, k=0, v=0), None) == 0
+    assert lib.rh3_kv_write(None, None) < 0 and lib.rh3_kv_read(None, None) < 0
     assert lib.rh3_kv_attn(attn_args(T=0, q=0, out=0), None, 0, None, None) == 0
 
 
