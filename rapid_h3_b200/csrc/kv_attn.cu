@@ -26,9 +26,10 @@ namespace rh3 {
 namespace {
 
 constexpr int TK = 128;                 // keys of a tile
-// Rows of a sequence (new tokens x query heads of a KV head), on average, above which the 128-row tiles of kv_attn_wide.cu take a call
-constexpr int64_t KV_WIDE_FROM = 16;
 constexpr int KV_WARPS = 4;             // computing warps
+// What it takes to begin and end a unit, in tiles; with the parts of a prefix pass taken in. (us with 0 / 0, 1 / 3, 2 / 3: 48 ragged sequences of up to
+// 4,096 tokens 56.1, 53.8, 52.3; 64 of up to 700 behind a prefix 103, 88.2, 88.0.) 0 where every tile can have a CTA of its own.
+constexpr int KV_PLAIN_COST = 2, KV_OWN_COST = 3;
 constexpr int KV_NT = KV_WARPS * 32 + 32;
 enum { MODE_PLAIN = 0, MODE_PREFIX = 1, MODE_OWN = 2 };
 
@@ -42,6 +43,8 @@ struct KvNarrow {
   static constexpr int TAIL = SCALES + STAGES * 2 * TK * 4;
   static constexpr int PART = BM * D + 2 * BM;                    // floats of a partial result: NT * D / 16 fragments, m, l
   static constexpr int PER = NT * (D / 16) / KV_WARPS;            // fragments that a warp joins
+  static constexpr int CARRY = STAGE_BYTES / (BM * D * 4);        // parts of the prefix pass that a stage takes
+  static constexpr int CARRY_ML = (BM + 2) * 2;                   // floats of a part's m and l, from an even row on
 };
 struct KvJoin {   // a cut unit that the CTA has a part of; parts = 0: none, or not to be joined here
   KvSegment g;
@@ -192,6 +195,27 @@ __device__ __forceinline__ bool kv_join_parts(const KvAttnParams& p, const KvJoi
   return true;
 }
 
+// What the prefix pass left for the rows of an own unit, which lie in one or two of its units: so many parts at most.
+struct KvCarry {
+  int flat, rows;         // the unit's first row in the prefix pass, its rows
+  int edge, n0, n1;       // rows before `edge` have n0 parts, the others n1
+};
+template <int BM>
+__device__ __forceinline__ KvCarry kv_carry(const KvAttnParams& p, const KvSegment& g) {
+  KvCarry c;
+  c.flat = g.s.first * p.group + g.u * BM;
+  c.rows = min(BM, g.s.n * p.group - g.u * BM);
+  const int units = (p.r.T * p.group + p.pre_bm - 1) / p.pre_bm, u = c.flat / p.pre_bm;
+  auto parts = [&](int unit) {
+    const int x = (g.h * units + unit) * p.pre_unit;
+    return (x + p.pre_last) / p.pre_run - (x + p.pre_first) / p.pre_run + 1;
+  };
+  c.edge = (u + 1) * p.pre_bm - c.flat;
+  c.n0 = parts(u);
+  c.n1 = c.edge < c.rows ? parts(u + 1) : 0;
+  return c;
+}
+
 template <int D, int FMT, int MODE, int NT>
 __global__ void __launch_bounds__(KV_NT, KvNarrow<D, NT>::CTAS)
 kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const KvAttnParams p) {
@@ -216,7 +240,7 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   }
   __syncthreads();
   grid_dependency_begin();
-  const KvRun run = kv_find_run<BM, TK>(p.r, p.c.page_log2, p.c.heads, p.group, p.most, p.status);
+  const KvRun run = kv_find_run<BM, TK>(p.r, p.c.page_log2, p.c.heads, p.group, p.cost, p.most, p.status);
   KvWalk<BM, TK> walk(run);
   KvSegment g;
 
@@ -229,7 +253,28 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
     const int page = 1 << p.c.page_log2, tile_pages = TK >> p.c.page_log2;
     int stage = 0;
     uint32_t ph = 1;
-    while (walk.next(p.r, p.c.page_log2, p.c.heads, p.group, g)) {
+    while (walk.next(p.r, p.c.page_log2, p.c.heads, p.group, p.cost, g)) {
+      if (MODE == MODE_OWN && g.k0 == 0) {   // what the prefix pass left goes through the ring before the keys do
+        const KvCarry c = kv_carry<BM>(p, g);
+        const int64_t rows = static_cast<int64_t>(p.r.T) * p.group;
+        const int parts = max(c.n0, c.n1);
+        for (int s0 = 0; s0 < parts; s0 += L::CARRY) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&tail->empty[stage], ph, abort_flag, p.status, ST_TIMEOUT_STAGE_EMPTY))) {
+            kv_settle();
+            return;
+          }
+          const int n = min(L::CARRY, parts - s0);
+          if (lane == 0) mbar_arrive_expect_tx(&tail->full[stage], n * (c.rows * D * 4 + L::CARRY_ML * 4));
+          __syncwarp();
+          if (lane < n) {
+            const int64_t at = (static_cast<int64_t>(s0 + lane) * p.c.heads + g.h) * rows + c.flat;
+            bulk_load(smem + stage * L::STAGE_BYTES + lane * BM * D * 4, p.pre_o + at * D, c.rows * D * 4, &tail->full[stage]);
+            bulk_load(scales + stage * 2 * TK + lane * L::CARRY_ML, p.pre_ml + 2 * (at & ~1ll), L::CARRY_ML * 4, &tail->full[stage]);
+          }
+          __syncwarp();
+          if (++stage == S) stage = 0, ph ^= 1;
+        }
+      }
       const int kend = kv_last_tile<BM>(p, g);
       for (int kt = g.k0; kt < kend; ++kt) {
         const int at = kt * tile_pages + lane;
@@ -273,7 +318,7 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   bool ok = true;
   int stage = 0, unit = 0;
   uint32_t ph = 0;
-  while (walk.next(p.r, p.c.page_log2, p.c.heads, p.group, g)) {
+  while (walk.next(p.r, p.c.page_log2, p.c.heads, p.group, p.cost, g)) {
     // query rows as B fragments of D / 16 products, row 8 nt + gq, channels 16c .. 16c+15 of each 64; per column: the factor from
     // accumulator to base-2 exponent, and where the accumulator begins
     uint32_t qb[NT][D / 16][2];
@@ -324,9 +369,51 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       for (int j = 0; j < MT; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
     }
 
+    if (MODE == MODE_OWN && g.k0 == 0) {   // what the prefix pass left for the rows: warp w begins with parts w, w + 4, ...
+      const KvCarry cr = kv_carry<BM>(p, g);
+      const int64_t rows = static_cast<int64_t>(p.r.T) * p.group;
+      const int parts = max(cr.n0, cr.n1);
+      for (int s0 = 0; s0 < parts && ok; s0 += L::CARRY) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&tail->full[stage], ph, abort_flag, p.status, ST_TIMEOUT_TMA_FULL));
+        if (!ok) break;
+#pragma unroll 1
+        for (int s = warp; s < min(L::CARRY, parts - s0); s += KV_WARPS) {
+          const int odd = static_cast<int>(((static_cast<int64_t>(s0 + s) * p.c.heads + g.h) * rows + cr.flat) & 1);
+          const float* part = reinterpret_cast<const float*>(smem + stage * L::STAGE_BYTES) + s * BM * D + ch0;
+          const float* ml = scales + stage * 2 * TK + s * L::CARRY_ML + 2 * odd;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int r = 8 * nt + 2 * c + e;
+              const bool is = r < cr.rows && s0 + s < (r < cr.edge ? cr.n0 : cr.n1);
+              const float pm = is ? ml[2 * r] : -INFINITY, pl = is ? ml[2 * r + 1] : 0.f;
+              const float nm = fmaxf(m[nt][e], pm);
+              const float zz = nm == -INFINITY ? 0.f : nm;
+              const float f = kv_ex2(m[nt][e] - zz), fp = kv_ex2(pm - zz);
+              m[nt][e] = nm;
+              l[nt][e] = l[nt][e] * f + (gq == 0 ? pl * fp : 0.f);   // l is a sum over the column's eight lanes
+              if (is) {
+#pragma unroll
+                for (int j = 0; j < MT; j += 2) {
+                  const float4 x = *reinterpret_cast<const float4*>(part + r * D + 2 * j);
+                  o[nt][j][e] = o[nt][j][e] * f + x.x * fp;
+                  o[nt][j][2 + e] = o[nt][j][2 + e] * f + x.y * fp;
+                  o[nt][j + 1][e] = o[nt][j + 1][e] * f + x.z * fp;
+                  o[nt][j + 1][2 + e] = o[nt][j + 1][2 + e] * f + x.w * fp;
+                }
+              }
+            }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tail->empty[stage]);
+        if (++stage == S) stage = 0, ph ^= 1;
+      }
+    }
     const int kend = kv_last_tile<BM>(p, g);
     const int pos_first = p.causal ? g.s.len - g.s.n + g.u * BM / p.group : g.s.len - 1;
-    for (int kt = g.k0; kt < kend; ++kt) {
+    for (int kt = g.k0; kt < kend && ok; ++kt) {
       if (!__all_sync(0xffffffffu, mbar_wait(&tail->full[stage], ph, abort_flag, p.status, ST_TIMEOUT_TMA_FULL))) {
         ok = false;
         break;
@@ -484,40 +571,6 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       if (++stage == S) stage = 0, ph ^= 1;
     }
 
-    // what the prefix pass found for these rows joins in the part that begins the unit; warp w takes splits w, w + 4, ...
-    if (MODE == MODE_OWN && g.k0 == 0) {
-      const long long rows = static_cast<long long>(p.r.T) * p.group;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const KvLaneRow r = kv_lane_row<BM>(p, g, 8 * nt + 2 * c + e);
-          int parts = 0;
-          if (r.q >= 0) {
-            const int x = (g.h * ((static_cast<int>(rows) + p.pre_bm - 1) / p.pre_bm) + r.flat / p.pre_bm) * p.pre_unit;
-            parts = (x + p.pre_last) / p.pre_run - (x + p.pre_first) / p.pre_run + 1;
-          }
-          for (int s = warp; s < parts; s += KV_WARPS) {
-            const long long at = (static_cast<long long>(s) * p.c.heads + g.h) * rows + r.flat;
-            const float pm = p.pre_ml[2 * at], pl = p.pre_ml[2 * at + 1];
-            const float nm = fmaxf(m[nt][e], pm);
-            const float zz = nm == -INFINITY ? 0.f : nm;
-            const float f = kv_ex2(m[nt][e] - zz), fp = kv_ex2(pm - zz);
-            m[nt][e] = nm;
-            l[nt][e] = l[nt][e] * f + (gq == 0 ? pl * fp : 0.f);   // l is a sum over the column's eight lanes
-            const float* src = p.pre_o + at * D + ch0;
-#pragma unroll
-            for (int j = 0; j < MT; j += 2) {
-              const uint4 x = ld_global_16(src + 2 * j);
-              o[nt][j][e] = o[nt][j][e] * f + __uint_as_float(x.x) * fp;
-              o[nt][j][2 + e] = o[nt][j][2 + e] * f + __uint_as_float(x.y) * fp;
-              o[nt][j + 1][e] = o[nt][j + 1][e] * f + __uint_as_float(x.z) * fp;
-              o[nt][j + 1][2 + e] = o[nt][j + 1][2 + e] * f + __uint_as_float(x.w) * fp;
-            }
-          }
-        }
-    }
-
     // ---- join the four warps: each leaves its sums where its own keys of the last tile were ----
     float4* own = reinterpret_cast<float4*>(smem + stage * L::STAGE_BYTES + warp * 32 * D);   // fragments of nt = 0 over its K rows, 1 over V
     float(*ml)[2][16] = tail->ml[unit & 1];
@@ -651,16 +704,26 @@ int kv_launch(const CUtensorMap& mk, const CUtensorMap& mv, const KvAttnParams& 
 // The plan of a call: which kernel and rows per unit, grids and the pieces of its workspace.
 struct KvPass {
   int nt;                       // narrow: units of 8 * nt rows; 0: wide, units of 256
-  int64_t bm, kt, w, grid;      // rows of a unit, key tiles of a unit and tiles of the pass at most, CTAs
+  int64_t bm, kt, w, grid;      // rows of a unit, key tiles of a unit and weight of the pass at most, CTAs
+  int cost;                     // what a unit weighs besides its tiles
 };
-KvPass kv_pass(int64_t heads, int64_t rows, int64_t seqs, int64_t kt) {
+KvPass kv_pass(int64_t heads, int64_t rows, int64_t seqs, int64_t kt, int cost) {
   KvPass x{};
-  x.nt = rows > KV_WIDE_FROM * seqs ? 0 : rows <= 8 * seqs ? 1 : 2;
+  x.cost = cost;
+  x.nt = rows <= 8 * seqs ? 1 : 2;
+  // Which kernel, by what the passes cost per SM: 0.8 us for a tile of 16 rows here; there 10 us to begin with (tensor memory, Q, the first
+  // tile's latency, the output), 2.6 us for a tile of 256 rows and 1.8 for one of up to 128 (measured at 128 channels; with 8 KV heads 24 rows x 700 keys
+  // 17 / 23 us here / there, 512 x 12,000 130 / 40, 8,044 x 18,000 3,029 / 620). Sequences count as equally long.
+  const int64_t each = (rows + seqs - 1) / seqs;
+  const double work = static_cast<double>(heads) * seqs * (kt < 1 ? 1 : kt) / device_sm_count();
+  if (each > 16 && 10.0 + (each > 128 ? 2.6 * ((each + 255) / 256) : 1.8) * work < 0.8 * ((each + 15) / 16) * work) x.nt = 0;
   x.bm = x.nt ? 8 * x.nt : KV_WIDE_BM;
   x.kt = kt < 1 ? 1 : kt;
   const int64_t units = heads * (rows / x.bm + seqs);
-  x.w = units * x.kt;
-  x.grid = kv_grid(units, x.kt, x.nt == 0 ? 1 : x.nt == 1 ? 3 : 2);
+  const int per_sm = x.nt == 0 ? 1 : x.nt == 1 ? 3 : 2;
+  x.grid = kv_grid(units, x.kt, per_sm);
+  if (x.grid < static_cast<int64_t>(per_sm) * device_sm_count()) x.cost = 0;
+  x.w = units * (x.kt + x.cost);
   return x;
 }
 struct KvPlan {
@@ -677,22 +740,22 @@ KvPlan kv_plan(int64_t heads, int64_t group, int64_t page, int64_t D, int64_t pe
     x.bytes += (bytes + 255) / 256 * 256;
     return at;
   };
-  x.own = kv_pass(heads, rows, seqs, own_kt);
-  if (x.own.nt == 0) x.own = kv_pass(heads, rows, seqs, own_kt + pre_kt);
+  x.own = kv_pass(heads, rows, seqs, own_kt, prefix > 0 ? KV_OWN_COST : KV_PLAIN_COST);
+  if (x.own.nt == 0) x.own = kv_pass(heads, rows, seqs, own_kt + pre_kt, KV_PLAIN_COST);
   x.part = take(x.own.grid * 2 * (x.own.nt ? x.own.bm * D + 2 * x.own.bm : kv_wide_part_floats(D)) * sizeof(float));
   if (prefix > 0 && x.own.nt) {
-    x.pre = kv_pass(heads, rows, 1, pre_kt);
+    x.pre = kv_pass(heads, rows, 1, pre_kt, KV_PLAIN_COST);
     const int64_t units = heads * ((rows + x.pre.bm - 1) / x.pre.bm);
-    x.pre_unit = x.pre.nt ? pre_kt : KV_WIDE_UNIT_COST + prefix;   // tiles, or keys and the unit's own cost
-    x.pre_first = x.pre.nt ? 0 : KV_WIDE_UNIT_COST;
-    x.pre_last = x.pre.nt ? pre_kt - 1 : KV_WIDE_UNIT_COST + (pre_kt - 1) * TK;
+    x.pre_unit = x.pre.nt ? x.pre.cost + pre_kt : KV_WIDE_UNIT_COST + prefix;   // in tiles or in keys
+    x.pre_first = x.pre.nt ? x.pre.cost : KV_WIDE_UNIT_COST;
+    x.pre_last = x.pre.nt ? x.pre.cost + pre_kt - 1 : KV_WIDE_UNIT_COST + (pre_kt - 1) * TK;
     x.pre.w = units * x.pre_unit;
     x.pre.grid = kv_grid(units, pre_kt, x.pre.nt == 0 ? 1 : x.pre.nt == 1 ? 3 : 2);
     x.pre_run = (x.pre.w + x.pre.grid - 1) / x.pre.grid;
     if (x.pre.nt == 0 && x.pre_run < TK) x.pre_run = TK;
     x.pre_splits = (x.pre_last - x.pre_first) / x.pre_run + 2;
     if (x.pre_splits > pre_kt) x.pre_splits = pre_kt;
-    x.pre_ml = take(x.pre_splits * heads * rows * 2 * sizeof(float));
+    x.pre_ml = take((x.pre_splits * heads * rows + 32) * 2 * sizeof(float));   // windows of m and l begin at even rows and end behind a unit's
     x.pre_o = take(x.pre_splits * heads * rows * D * sizeof(float));
   }
   return x;
@@ -739,6 +802,7 @@ extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t w
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.count = counters;
   p.most = static_cast<int>(x.own.w);
+  p.cost = x.own.cost;
   p.part = reinterpret_cast<float*>(ws + x.part);
   if (x.own.nt == 0) {
     p.r.pre_tiles = static_cast<int>((a->prefix + TK - 1) / TK);
@@ -773,6 +837,7 @@ extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t w
                static_cast<int>(a->prefix), 0};
   q.causal = 0;
   q.most = static_cast<int>(x.pre.w);
+  q.cost = x.pre.cost;
   if (int e = x.pre.nt == 0 ? kv_wide_launch(q, a->D, a->kind, true, x.pre.grid, stream) : launch(std::integral_constant<int, MODE_PREFIX>(), q, x.pre)) return e;
   return launch(std::integral_constant<int, MODE_OWN>(), p, x.own);
 }

@@ -75,13 +75,14 @@ __device__ __forceinline__ int64_t kv_place(const KvCache& c, const KvRows& r, i
 // ---------------------------------------------------------------------------------------------
 // The rows of a sequence are its new tokens x the query heads of one KV head ("group"): row = token * group + head. A unit is
 // BM such rows of one sequence and KV head against all of its keys, in tiles of TK keys; every unit has at least one tile, so that rows
-// without a key are written too. The tiles of all units, in the order (sequence, head, row tile, key tile), are dealt to the CTAs
-// in runs of `run` = W / grid, rounded up: a CTA's run begins and ends anywhere inside a unit. The entry knows a bound `most` below 2^31
+// without a key are written too. A unit weighs its tiles and `cost` more, for what it takes to begin and end it. All units, in the order
+// (sequence, head, row tile), are dealt to the CTAs in runs of `run` = W / grid, rounded up: a run begins and ends anywhere inside a unit,
+// where position y stands for key tile y - cost (0 up to there). The entry knows a bound `most` below 2^31
 // of W; more than that comes of starts that are not ascending, and nothing is done then.
 struct KvSeq {
   int first, n, len;  // first row token of the call, new tokens, cached tokens
   int qt, kt;         // row tiles, key tiles of a unit
-  __device__ __forceinline__ int tiles(int heads) const { return heads * qt * kt; }
+  __device__ __forceinline__ int weight(int heads, int cost) const { return heads * qt * (kt + cost); }
 };
 template <int BM, int TK>
 __device__ __forceinline__ KvSeq kv_seq(const KvRows& r, int page_log2, int group, int b) {
@@ -96,20 +97,20 @@ __device__ __forceinline__ KvSeq kv_seq(const KvRows& r, int page_log2, int grou
   return s;
 }
 struct KvRun {
-  int x0, x1;   // the CTA's tiles
-  int run;      // tiles of a CTA: x belongs to CTA x / run
-  int b, xb;    // the sequence that x0 lies in and its first tile
+  int x0, x1;   // the CTA's run
+  int run;      // length of a run: x belongs to CTA x / run
+  int b, xb;    // the sequence that x0 lies in and where it begins
 };
 // Every warp scans the sequences by itself (they are in L1 after the first): no barrier, one round of loads up to 32 sequences.
 template <int BM, int TK>
-__device__ __forceinline__ KvRun kv_find_run(const KvRows& r, int page_log2, int heads, int group, int most, int* status) {
+__device__ __forceinline__ KvRun kv_find_run(const KvRows& r, int page_log2, int heads, int group, int cost, int most, int* status) {
   const int lane = threadIdx.x & 31;
   const int per = (r.B + 31) >> 5;
   const int b0 = min(r.B, lane * per), b1 = min(r.B, b0 + per);
   long long sum = 0;
   for (int b = b0; b < b1; ++b) {
     const KvSeq s = kv_seq<BM, TK>(r, page_log2, group, b);
-    sum += static_cast<long long>(heads) * s.qt * s.kt;
+    sum += static_cast<long long>(heads) * s.qt * (s.kt + cost);
   }
   int own = static_cast<int>(min(sum, static_cast<long long>(most) + 1));
   if (__any_sync(0xffffffffu, own > most)) own = lane == 0 ? most + 1 : 0;
@@ -133,7 +134,7 @@ __device__ __forceinline__ KvRun kv_find_run(const KvRows& r, int page_log2, int
   const bool mine = run.x0 < run.x1 && xb <= run.x0 && run.x0 < incl;
   if (mine && per > 1) {
     for (; b < b1; ++b) {
-      const int w = kv_seq<BM, TK>(r, page_log2, group, b).tiles(heads);
+      const int w = kv_seq<BM, TK>(r, page_log2, group, b).weight(heads, cost);
       if (run.x0 - xb < w) break;
       xb += w;
     }
@@ -148,7 +149,7 @@ struct KvSegment {
   KvSeq s;
   int b, h, u;        // sequence, KV head, row tile
   int k0, k1;         // key tiles [k0, k1) of the unit's s.kt
-  int x;              // the unit's first tile
+  int x;              // position of the unit's first tile
 };
 // Steps through a run; next() gives the segment at x and moves on.
 template <int BM, int TK>
@@ -157,24 +158,25 @@ struct KvWalk {
   KvSeq s;
   bool have;
   __device__ __forceinline__ KvWalk(const KvRun& run) : x(run.x0), x1(run.x1), xb(run.xb), b(run.b), have(false) {}
-  __device__ __forceinline__ bool next(const KvRows& r, int page_log2, int heads, int group, KvSegment& g) {
-    if (x >= x1) return false;
+  __device__ __forceinline__ bool next(const KvRows& r, int page_log2, int heads, int group, int cost, KvSegment& g) {
+   while (x < x1) {
     if (!have) s = kv_seq<BM, TK>(r, page_log2, group, b), have = true;
-    while (x - xb >= s.tiles(heads)) {  // ends: the tiles of the sequences from b on reach beyond x < x1 <= W
+    while (x - xb >= s.weight(heads, cost)) {  // ends: the sequences from b on reach beyond x < x1 <= W
       if (b + 1 >= r.B) return false;
-      xb += s.tiles(heads);
+      xb += s.weight(heads, cost);
       s = kv_seq<BM, TK>(r, page_log2, group, ++b);
     }
-    const unsigned rem = x - xb;
-    const unsigned unit = rem / static_cast<unsigned>(s.kt);
+    const unsigned rem = x - xb, w = s.kt + cost, unit = rem / w;
+    const int y = rem - unit * w, end = min(static_cast<int>(w), y + (x1 - x));
     g.s = s, g.b = b;
-    g.k0 = rem - unit * s.kt;
-    g.x = x - g.k0;
+    g.k0 = max(0, y - cost), g.k1 = max(0, end - cost);
+    g.x = x - y + cost;
     g.h = unit / static_cast<unsigned>(s.qt);
     g.u = unit - static_cast<unsigned>(g.h) * s.qt;
-    g.k1 = min(s.kt, g.k0 + (x1 - x));
-    x += g.k1 - g.k0;
-    return true;
+    x += end - y;
+    if (g.k0 < g.k1) return true;
+   }
+   return false;
   }
 };
 // Keys that some row of row tile u sees: the last row's position + 1 (causal) or all of them.
