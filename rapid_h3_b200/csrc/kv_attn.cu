@@ -701,6 +701,9 @@ int kv_launch(const CUtensorMap& mk, const CUtensorMap& mv, const KvAttnParams& 
   return check_cuda(launch_chained(kern, dim3(static_cast<unsigned>(grid)), KV_NT, smem, stream, 1, mk, mv, p), "kv_attn launch");
 }
 
+// rh3_kv_attn_use_wide: -1 by cost, 0 never, 1 always
+std::atomic<int> g_use_wide{-1};
+
 // The plan of a call: which kernel and rows per unit, grids and the pieces of its workspace.
 struct KvPass {
   int nt;                       // narrow: units of 8 * nt rows; 0: wide, units of 256
@@ -716,7 +719,9 @@ KvPass kv_pass(int64_t heads, int64_t rows, int64_t seqs, int64_t kt, int cost) 
   // 17 / 23 us here / there, 512 x 12,000 130 / 40, 8,044 x 18,000 3,029 / 620). Sequences count as equally long.
   const int64_t each = (rows + seqs - 1) / seqs;
   const double work = static_cast<double>(heads) * seqs * (kt < 1 ? 1 : kt) / device_sm_count();
-  if (each > 16 && 10.0 + (each > 128 ? 2.6 * ((each + 255) / 256) : 1.8) * work < 0.8 * ((each + 15) / 16) * work) x.nt = 0;
+  const int use = g_use_wide.load(std::memory_order_relaxed);
+  if (use >= 0) x.nt = use ? 0 : x.nt;
+  else if (each > 16 && 10.0 + (each > 128 ? 2.6 * ((each + 255) / 256) : 1.8) * work < 0.8 * ((each + 15) / 16) * work) x.nt = 0;
   x.bm = x.nt ? 8 * x.nt : KV_WIDE_BM;
   x.kt = kt < 1 ? 1 : kt;
   const int64_t units = heads * (rows / x.bm + seqs);
@@ -771,6 +776,8 @@ extern "C" int64_t rh3_kv_attn_workspace_bytes(int64_t heads, int64_t group, int
   if (heads <= 0 || group <= 0 || page <= 0 || (D != 64 && D != 128) || per_seq < 0 || B <= 0 || T <= 0 || prefix < 0) return 0;
   return kv_plan(heads, group, page, D, per_seq, B, T, prefix).bytes;
 }
+
+extern "C" int rh3_kv_attn_use_wide(int use) { return g_use_wide.exchange(use < 0 ? -1 : use ? 1 : 0); }
 
 extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t workspace_bytes, int32_t* counters, cudaStream_t stream) {
   RH3_CHECK_ARG(a, "kv_attn: null arguments");

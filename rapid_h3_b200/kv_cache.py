@@ -117,6 +117,14 @@ def _scratch(device, index, stream, need):
     return kept if need <= _KEPT_BYTES else (kept[0], torch.empty(need, device=device, dtype=torch.uint8))
 
 
+def use_wide(use):
+    """Which kernel attention runs on: None (the default) the cheaper one for a call's sizes, False the one for few rows per sequence, True the one
+    on 128-row tensor-core tiles. For the whole process; returns the previous setting."""
+    before = _lib.lib().rh3_kv_attn_use_wide(-1 if use is None else int(use))
+    _NEED.clear()
+    return None if before < 0 else bool(before)
+
+
 def _workspace_bytes(*sizes):
     need = _NEED.get(sizes)
     if need is None:

@@ -3,7 +3,9 @@
 Tolerance of attention, derived: the output is rounded once (eps / 2 of its value); every weight is rounded to fp16 (2^-11 of it),
 computed with approximate exp2, log2 and reciprocal (2^-17 together, |log2 vs| <= 40) from a score that D / 16 tensor-core steps
 sum in fp32 (2^-22 of the magnitudes' sum for each, the two products behind it included) and enters numerator and
-denominator. Weights move the output by at most their relative error times sum_j p_j |v_j|."""
+denominator. Weights move the output by at most their relative error times sum_j p_j |v_j|. The kernel for few rows adds K codes as code + 128 <= 255,
+about twice the magnitudes, and the kernel for many rows rounds V to fp16 (2^-11 of a value, and 2^-25 of twice the largest row's magnitude where that
+is more)."""
 import random
 
 import pytest
@@ -21,6 +23,14 @@ def kv():
     _lib.lib()
     _lib.check_status()
     return kv_cache
+
+
+@pytest.fixture(params=[False, True], ids=["few rows", "many rows"])
+def path(kv, request):
+    """Both kernels, whatever a call's sizes would choose."""
+    before = kv.use_wide(request.param)
+    yield
+    kv.use_wide(before)
 
 
 def fill(cache, seed):
@@ -66,7 +76,8 @@ def check_attention(out, q, cache, table, lens, starts, **kw):
     kmax = (k.float() * ks[..., None]).nan_to_num(0, 0, 0).abs().amax()
     s_abs = scale * float(q.double().abs().sum(-1).max() * kmax)
     d = q.shape[2]
-    tol = torch.finfo(q.dtype).eps / 2 * ref.abs() + mag * (2 ** -11 + 2 ** -17 + 2 * (d // 16 + 2) * 2 ** -22 * s_abs) + 1e-7
+    v_max = float((v.float().abs() * vs[..., None]).nan_to_num(0, 0, 0).amax())
+    tol = torch.finfo(q.dtype).eps / 2 * ref.abs() + mag * (2 * 2 ** -11 + 2 ** -17 + 2 * (d // 16 + 2) * 2 ** -22 * 2 * s_abs) + 2 ** -24 * v_max + 1e-7
     rows = starts[-1]
     err = (out.cpu().double() - ref)[:rows].abs()
     assert torch.isfinite(out[:rows]).all()
@@ -88,7 +99,7 @@ SHAPES = [  # kind, dtype, D, page, kv heads, group
     ([1], [1]), ([517], [1]), ([0, 5], [0, 2]), ([64, 1, 130, 257, 16], [1, 1, 1, 1, 1]), ([300, 37, 129], [7, 37, 20]), ([40, 128], [40, 3]),
 ])
 @pytest.mark.parametrize("causal", [True, False])
-def test_attention(kv, kind, dtype, d, page, heads, group, lens, news, causal):
+def test_attention(kv, path, kind, dtype, d, page, heads, group, lens, news, causal):
     pages = sum(-(-n // page) for n in lens) + 2
     cache = kv.alloc(pages, heads, d, page, kind)
     fill(cache, 1)
@@ -141,7 +152,7 @@ def test_write_stores_codes_and_scales_and_read_gives_them_back(kv, kind, dtype,
             assert torch.equal(got[:-2].cpu(), ref) and bool((got[-2:] == 7).all())
 
 
-def test_rows_that_are_not_finite_read_back_as_nan_and_reach_nobody_else(kv):
+def test_rows_that_are_not_finite_read_back_as_nan_and_reach_nobody_else(kv, path):
     """A NaN or an infinity stays in its row's scale, and a masked row of that kind changes nothing."""
     for kind in ("int8", "fp8"):
         cache = kv.alloc(4, 2, 128, 16, kind)
@@ -162,7 +173,7 @@ def test_rows_that_are_not_finite_read_back_as_nan_and_reach_nobody_else(kv):
         assert bool(torch.isnan(out[33]).all())
 
 
-def test_what_lies_in_slots_behind_a_sequence_does_not_matter(kv):
+def test_what_lies_in_slots_behind_a_sequence_does_not_matter(kv, path):
     """Unwritten slots with NaN codes (0x7f of e4m3), NaN and infinite scales."""
     for kind in ("int8", "fp8"):
         cache = kv.alloc(6, 1, 128, 64, kind)
@@ -181,7 +192,7 @@ def test_what_lies_in_slots_behind_a_sequence_does_not_matter(kv):
             assert bool((out[2] == 0).all())              # a row without a key
 
 
-def test_values_without_sense_are_cut_to_what_exists(kv):
+def test_values_without_sense_are_cut_to_what_exists(kv, path):
     """Pages outside the cache, lengths beyond the table, rows beyond the call's, negative lengths."""
     from rapid_h3_b200 import _lib
     i32 = dict(dtype=torch.int32, device="cuda")
@@ -217,7 +228,7 @@ def test_values_without_sense_are_cut_to_what_exists(kv):
     ([0], [1], 1), ([64, 1, 0, 130], [1, 1, 1, 1], 700), ([33, 160, 7], [33, 60, 0], 129), ([5, 300], [2, 9], 0),
 ])
 @pytest.mark.parametrize("causal", [True, False])
-def test_attention_behind_a_shared_prefix(kv, kind, dtype, d, page, heads, group, lens, news, prefix, causal):
+def test_attention_behind_a_shared_prefix(kv, path, kind, dtype, d, page, heads, group, lens, news, prefix, causal):
     pre = -(-prefix // page)
     pages = sum(-(-n // page) for n in lens) + pre + 2
     cache = kv.alloc(pages, heads, d, page, kind)
@@ -233,7 +244,7 @@ def test_attention_behind_a_shared_prefix(kv, kind, dtype, d, page, heads, group
 
 @pytest.mark.parametrize("kind,dtype,d,page,heads,group", SHAPES[:4])
 @pytest.mark.parametrize("lens,news", [([700, 1, 333], [520, 1, 333]), ([2000], [65])])
-def test_attention_of_many_rows(kv, kind, dtype, d, page, heads, group, lens, news):
+def test_attention_of_many_rows(kv, path, kind, dtype, d, page, heads, group, lens, news):
     """Units of 256 rows over several key tiles, cut between CTAs."""
     pages = sum(-(-n // page) for n in lens) + 2
     cache = kv.alloc(pages, heads, d, page, kind)
@@ -243,3 +254,214 @@ def test_attention_of_many_rows(kv, kind, dtype, d, page, heads, group, lens, ne
     q = (torch.randn(starts[-1], heads * group, d, generator=g) * 1.5).to(dtype).cuda()
     out = kv.attention(q, cache, rows)
     check_attention(out, q, cache, table, lens, starts)
+
+
+def test_a_long_context_joined_from_many_parts(kv, path):
+    """One sequence over all of the chip: more parts than a joining CTA takes in at a time, and a tail of tiny weights."""
+    for kind, dtype, d, heads, group in (("int8", torch.bfloat16, 128, 1, 2), ("fp8", torch.float16, 64, 1, 16)):
+        n, page = 20011, 128
+        pages = -(-n // page) + 1
+        cache = kv.alloc(pages, heads, d, page, kind)
+        fill(cache, 31)
+        rows, table, starts = batch(kv, [n], [1], page, pages, 32)
+        g = torch.Generator().manual_seed(33)
+        q = (torch.randn(1, heads * group, d, generator=g) * 1.5).to(dtype).cuda()
+        check_attention(kv.attention(q, cache, rows), q, cache, table, [n], starts)
+
+
+def test_a_prefix_shared_by_many_rows(kv):
+    """Enough rows and tokens that the prefix goes to the tensor-core tiles and the own parts do not; rows of one sequence lie in two units
+    of the prefix pass."""
+    heads, group, d, page, prefix = 4, 5, 128, 32, 1900
+    lens, news = [3, 40, 0, 300, 129, 7] * 9, [1, 2, 1, 1, 3, 1] * 9
+    pre = -(-prefix // page)
+    pages = sum(-(-n // page) for n in lens) + pre + 2
+    cache = kv.alloc(pages, heads, d, page, "int8")
+    fill(cache, 34)
+    rows, table, starts = batch(kv, lens + [prefix], news + [0], page, pages, 35)
+    ids = table[-1][:pre]
+    rows = kv.Rows(rows.table[:-1], rows.lens[:-1], rows.starts[:-1])
+    g = torch.Generator().manual_seed(36)
+    q = torch.randn(starts[-1], heads * group, d, generator=g).to(torch.bfloat16).cuda()
+    before = None
+    for use in (None, True, False):
+        before = kv.use_wide(use) if before is None else (kv.use_wide(use), before)[1]
+        out = kv.attention_shared(q, cache, rows, torch.tensor(ids, dtype=torch.int32, device="cuda"), prefix)
+        check_attention(out, q, cache, table[:-1], lens, starts[:-1], prefix=ids, prefix_len=prefix)
+    kv.use_wide(None)
+
+
+def test_scales_of_very_different_size(kv, path):
+    """V scales over 2^24 and K rows over 2^12: the largest tokens decide what matters, and later tiles bring larger ones."""
+    cache = kv.alloc(8, 1, 128, 64, "int8")
+    fill(cache, 37)
+    rows, table, starts = batch(kv, [500], [40], 64, 8, 38)
+    order = torch.tensor(table[0]).cuda()
+    for i in range(8):
+        cache.v_scale[order[i]] *= 2.0 ** (3 * i - 12)
+        cache.k_scale[order[i]] *= 2.0 ** (i % 3 * 2 - 6)
+    q = torch.randn(40, 4, 128, generator=torch.Generator().manual_seed(39)).to(torch.bfloat16)
+    q[::3] *= 2.0 ** 20
+    q[1::3] *= 2.0 ** -20
+    q = q.cuda()
+    check_attention(kv.attention(q, cache, rows, scale=1e-3), q, cache, table, [500], starts, scale=1e-3)
+    check_attention(kv.attention(q[1::3].contiguous(), cache, kv.Rows(rows.table, rows.lens, torch.tensor([0, 13], dtype=torch.int32, device="cuda"))),
+                    q[1::3], cache, table, [500], [0, 13])
+
+
+def test_rows_behind_the_last_sequence_stay(kv, path):
+    """A padded batch: more rows than starts[B] in q and out, which hold NaN."""
+    cache = kv.alloc(6, 2, 64, 16, "fp8")
+    fill(cache, 40)
+    rows, table, starts = batch(kv, [17, 30], [1, 20], 16, 6, 41)
+    q = torch.full((40, 4, 64), float("nan"), dtype=torch.bfloat16)
+    q[:21] = torch.randn(21, 4, 64, generator=torch.Generator().manual_seed(42)).to(torch.bfloat16)
+    out = torch.full((40, 6, 64), 5.0, dtype=torch.bfloat16, device="cuda")[:, 1:5]
+    q = q.cuda()
+    assert kv.attention(q, cache, rows, out=out) is out
+    check_attention(out[:21], q[:21], cache, table, [17, 30], starts)
+    assert bool((out[21:] == 5).all())
+    pre = torch.tensor([5], dtype=torch.int32, device="cuda")
+    kv.attention_shared(q, cache, rows, pre, 9, out=out)
+    check_attention(out[:21], q[:21], cache, table, [17, 30], starts, prefix=[5], prefix_len=9)
+    assert bool((out[21:] == 5).all())
+
+
+def test_a_captured_step_follows_lengths_and_pages(kv, path):
+    """Write, attention and read of one decoding step in a graph, replayed while sequences grow; an eager call of the same kind in between."""
+    heads, group, d, page = 2, 4, 128, 16
+    cache = kv.alloc(64, heads, d, page, "int8")
+    dev = dict(dtype=torch.int32, device="cuda")
+    table = torch.arange(60, **dev).view(3, 20).contiguous()
+    lens = torch.tensor([300, 1, 95], **dev)
+    rows = kv.Rows(table, lens, torch.arange(4, **dev))
+    fill(cache, 43)
+    k, v = (torch.zeros(3, heads, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    q = torch.zeros(3, heads * group, d, dtype=torch.bfloat16, device="cuda")
+
+    def step():
+        kv.write(cache, k, v, rows)
+        return kv.attention(q, cache, rows), kv.read(cache, rows, 3)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, back = step()
+    g = torch.Generator().manual_seed(44)
+    for i in range(3):
+        for t in (k, v, q):
+            t.copy_(torch.randn(t.shape, generator=g))
+        if i:
+            lens += 3
+            table[1].copy_(table[1].flip(0))
+        graph.replay()
+        first = out.clone()
+        other = kv.attention(q, cache, rows)
+        graph.replay()
+        assert torch.equal(first, out) and torch.equal(first, other)
+        check_attention(out, q, cache, table.tolist(), lens.tolist(), [0, 1, 2, 3])
+        place = [(table[b, (int(lens[b]) - 1) // page], (int(lens[b]) - 1) % page) for b in range(3)]
+        for x, codes, scales in ((back[0], cache.k, cache.k_scale), (back[1], cache.v, cache.v_scale)):
+            ref = torch.stack([codes[p, :, o].float() * scales[p, :, o, None] for p, o in place])
+            assert torch.equal(x, ref.to(torch.bfloat16))
+
+
+def test_calls_on_two_streams_at_once(kv, path):
+    """Each stream has counters and a workspace of its own: results as one after the other."""
+    cache = kv.alloc(80, 2, 128, 64, "fp8")
+    fill(cache, 45)
+    cases = []
+    for i, lens in enumerate(([4000], [300, 800, 64, 1])):
+        rows, _, starts = batch(kv, lens, [1] * len(lens), 64, 80, 46 + i)
+        q = torch.randn(starts[-1], 16, 128, generator=torch.Generator().manual_seed(i)).to(torch.float16).cuda()
+        cases.append((q, rows, kv.attention(q, cache, rows), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):
+        for i, (q, rows, _, stream) in enumerate(cases):
+            with torch.cuda.stream(stream):
+                outs[i].append(kv.attention(q, cache, rows))
+    torch.cuda.synchronize()
+    for got, (_, _, want, _) in zip(outs, cases):
+        assert all(torch.equal(x, want) for x in got)
+
+
+def test_pages_behind_32_bit_offsets(kv, path):
+    """A cache whose codes take more than 2^32 bytes: pages at its end are written, read and attended to."""
+    page, heads, d = 128, 16, 128
+    pages = (1 << 32) // (page * heads * d) + 40
+    codes = [torch.empty(pages, heads, page, d, dtype=torch.int8, device="cuda") for _ in range(2)]
+    cache = kv.KVCache(*codes, *(torch.empty(pages, heads, page, device="cuda") for _ in range(2)))
+    dev = dict(dtype=torch.int32, device="cuda")
+    table = [[pages - 1, pages - 3], [pages - 2, 0]]
+    rows = kv.Rows(torch.tensor(table, **dev), torch.tensor([200, 130], **dev), torch.tensor([0, 200, 330], **dev))
+    g = torch.Generator().manual_seed(48)
+    k, v = (torch.randn(330, heads, d, generator=g).to(torch.bfloat16) for _ in range(2))
+    kv.write(cache, k.cuda(), v.cuda(), rows)
+    q8, s8 = okv.quantize(k, "int8")
+    assert torch.equal(kv.read(cache, rows, 330, torch.float32)[0].cpu(), q8.float() * s8[..., None])
+    q = torch.randn(2, heads, d, generator=g).to(torch.bfloat16).cuda()
+    last = kv.Rows(rows.table, rows.lens, torch.tensor([0, 1, 2], **dev))
+    out = kv.attention(q, cache, last)
+    small = [c[[0, pages - 3, pages - 2, pages - 1]] for c in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    check_attention(out, q, kv.KVCache(*(t.contiguous() for t in small)), [[3, 1], [2, 0]], [200, 130], [0, 1, 2])
+
+
+def test_starts_that_do_not_ascend_are_reported_or_cut(kv, path):
+    from rapid_h3_b200 import _lib
+    cache = kv.alloc(40, 1, 64, 16, "int8")
+    fill(cache, 49)
+    dev = dict(dtype=torch.int32, device="cuda")
+    rows = kv.Rows(torch.arange(40, **dev).view(4, 10), torch.tensor([160, 3, 160, 9], **dev), torch.tensor([0, 9, 2, 9, 1], **dev))
+    q = torch.randn(9, 8, 64).to(torch.bfloat16).cuda()
+    kv.attention(q, cache, rows)
+    kv.read(cache, rows, 9)
+    torch.cuda.synchronize()
+    try:
+        _lib.check_status()
+    except RuntimeError as e:
+        assert "ascending" in str(e)
+
+
+def test_refusals(kv):
+    dev = dict(dtype=torch.int32, device="cuda")
+    cache = kv.alloc(4, 2, 64, 16, "int8")
+    rows = kv.Rows(torch.zeros(1, 4, **dev), torch.ones(1, **dev), torch.tensor([0, 1], **dev))
+    x = torch.zeros(1, 2, 64, dtype=torch.bfloat16, device="cuda")
+    q = torch.zeros(1, 4, 64, dtype=torch.bfloat16, device="cuda")
+    for bad in (x.cpu(), x.double(), x[..., :32], x[:, :1], torch.zeros(1, 2, 68, dtype=torch.bfloat16, device="cuda")[..., 2:66], x.transpose(1, 2).contiguous().transpose(1, 2)):
+        with pytest.raises(RuntimeError):
+            kv.write(cache, bad, x, rows)
+        with pytest.raises(RuntimeError):
+            kv.write(cache, x, bad, rows)
+    with pytest.raises(RuntimeError):
+        kv.write(cache, x, torch.zeros(2, 2, 64, dtype=torch.bfloat16, device="cuda"), rows)
+    for bad in (q[:, :3], q.float(), q.cpu(), torch.zeros(1, 0, 64, dtype=torch.bfloat16, device="cuda")):
+        with pytest.raises(RuntimeError):
+            kv.attention(bad, cache, rows)
+    for kw in (dict(scale=0.0), dict(scale=float("nan")), dict(scale=-1.0), dict(out=q.float()), dict(out=torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="cuda"))):
+        with pytest.raises(RuntimeError):
+            kv.attention(q, cache, rows, **kw)
+    for pre, n in ((torch.zeros(2, **dev), 33), (torch.zeros(2, **dev), -1), (torch.zeros(2, device="cuda"), 3), (torch.zeros(2, 1, **dev), 3)):
+        with pytest.raises(RuntimeError):
+            kv.attention_shared(q, cache, rows, pre, n)
+    for args in ((torch.zeros(1, 4, device="cuda"), rows.lens, rows.starts), (rows.table, torch.ones(2, **dev), rows.starts), (rows.table, rows.lens, rows.lens),
+                 (rows.table[0], rows.lens, rows.starts), (torch.zeros(4, 4, **dev).t()[:1], rows.lens, rows.starts), (rows.table[:0], rows.lens[:0], rows.starts[:1])):
+        with pytest.raises(RuntimeError):
+            kv.Rows(*args)
+    k, ks = cache.k, cache.k_scale
+    for args in ((k, k[:2], ks, ks), (k.float(), k.float(), ks, ks), (k, k, ks.half(), ks), (k, k, ks[:, :1], ks), (k[:, :, ::2], k[:, :, ::2], ks[..., ::2], ks[..., ::2]),
+                 (k.transpose(1, 2), k.transpose(1, 2), ks.transpose(1, 2), ks.transpose(1, 2))):
+        with pytest.raises(RuntimeError):
+            kv.KVCache(*args)
+    with pytest.raises(RuntimeError):
+        kv.read(cache, rows, 1, torch.float64)
+    with pytest.raises(RuntimeError):
+        kv.read(cache, rows, 1, torch.bfloat16, (x[:, :1], x))
+    # calls without rows do nothing
+    kv.write(cache, x[:0], x[:0], rows)
+    assert kv.attention(q[:0], cache, rows).shape == (0, 4, 64) and kv.read(cache, rows, 0)[0].shape == (0, 2, 64)
