@@ -9,9 +9,10 @@
 // holds 8 channels (16-byte accesses on the bf16 side, 8 bytes on the code side), D / 8 lanes a row. A warp has KV_ITER groups of
 // rows of one token, all of K or all of V, issues their loads before it works on the first, and looks up once where they lie
 // (sequence, page); a block's eight warps have eight tokens, whose codes and scales of a head are neighbours in a page. Instructions are
-// what such a warp has to save: its addresses are a pointer and a step, its token and part come from the grid. Measured, 36,436 tokens of 8
-// heads of 128 read as bf16 / three prompts written: 37.5 / 51.9 us, 92 / 85% of a copy's bandwidth (rows of K and V in one warp, an
-// address per row and a division per warp, 471 instructions: 48.5 / 58 us; four tokens a warp besides: 84 / 69 us).
+// what such a warp has to save: its addresses are a pointer and a step, its token and part come from the grid. Measured, 36,436 tokens of
+// 8 heads of 128 read as bf16, and 37 ragged prompts of up to 900 fp32 tokens written: 37.5 and 51.9 us, 92 and 85% of a copy's bandwidth
+// (rows of K and V in one warp, an address per row and a division per warp, 471 instructions: 48.5 and 58 us; four tokens a warp
+// besides: 84 and 69 us).
 #include "kv_cache.cuh"
 #include "rapidh3_b200.h"
 
