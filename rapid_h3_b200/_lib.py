@@ -148,11 +148,16 @@ def call(name, *args, launches=None):
         raise RuntimeError(f"{name} failed ({rc}): {last_error()}")
 
 
+on_failed_status = []   # called before check_status raises: what an abandoned call may have left undone is dropped here
+
+
 def check_status():
     """Synchronise the current stream and raise if a bounded device-side wait gave up."""
     st = ctypes.c_int(0)
     call("rh3_check_status", stream(), ctypes.addressof(st))
     if st.value != 0:
+        for drop in on_failed_status:
+            drop()
         raise RuntimeError(f"device status {st.value}: {last_error()}")
 
 

@@ -785,7 +785,7 @@ extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t w
   if (int e = kv_fill_cache(&p.c, "kv_attn", a->k, a->v, a->ks, a->vs, a->pages, a->heads, a->page, a->D, a->kind)) return e;
   if (int e = kv_fill_rows(&p.r, "kv_attn", a->table, a->table_stride, a->per_seq, a->lens, a->starts, a->B, a->T)) return e;
   RH3_CHECK_ARG(a->dtype == 0 || a->dtype == 1, "kv_attn: dtype=%d must be 0 (bf16) or 1 (fp16)", a->dtype);
-  RH3_CHECK_ARG(a->group >= 1 && a->group * a->heads <= 4096, "kv_attn: %lld query heads per KV head", (long long)a->group);
+  RH3_CHECK_ARG(a->group >= 1 && a->group <= 4096 && a->group * a->heads <= 4096, "kv_attn: %lld query heads per KV head", (long long)a->group);
   RH3_CHECK_ARG(a->scale > 0.f && a->scale < INFINITY, "kv_attn: the softmax scale must be positive and finite");
   RH3_CHECK_ARG(a->prefix >= 0 && a->prefix <= a->prefix_pages * a->page && (a->prefix == 0 || a->prefix_table),
                 "kv_attn: a prefix of %lld tokens needs a table of its pages", (long long)a->prefix);

@@ -159,24 +159,24 @@ struct KvWalk {
   bool have;
   __device__ __forceinline__ KvWalk(const KvRun& run) : x(run.x0), x1(run.x1), xb(run.xb), b(run.b), have(false) {}
   __device__ __forceinline__ bool next(const KvRows& r, int page_log2, int heads, int group, int cost, KvSegment& g) {
-   while (x < x1) {
-    if (!have) s = kv_seq<BM, TK>(r, page_log2, group, b), have = true;
-    while (x - xb >= s.weight(heads, cost)) {  // ends: the sequences from b on reach beyond x < x1 <= W
-      if (b + 1 >= r.B) return false;
-      xb += s.weight(heads, cost);
-      s = kv_seq<BM, TK>(r, page_log2, group, ++b);
+    while (x < x1) {
+      if (!have) s = kv_seq<BM, TK>(r, page_log2, group, b), have = true;
+      while (x - xb >= s.weight(heads, cost)) {  // ends: the sequences from b on reach beyond x < x1 <= W
+        if (b + 1 >= r.B) return false;
+        xb += s.weight(heads, cost);
+        s = kv_seq<BM, TK>(r, page_log2, group, ++b);
+      }
+      const unsigned rem = x - xb, w = s.kt + cost, unit = rem / w;
+      const int y = rem - unit * w, end = min(static_cast<int>(w), y + (x1 - x));
+      g.s = s, g.b = b;
+      g.k0 = max(0, y - cost), g.k1 = max(0, end - cost);
+      g.x = x - y + cost;
+      g.h = unit / static_cast<unsigned>(s.qt);
+      g.u = unit - static_cast<unsigned>(g.h) * s.qt;
+      x += end - y;
+      if (g.k0 < g.k1) return true;
     }
-    const unsigned rem = x - xb, w = s.kt + cost, unit = rem / w;
-    const int y = rem - unit * w, end = min(static_cast<int>(w), y + (x1 - x));
-    g.s = s, g.b = b;
-    g.k0 = max(0, y - cost), g.k1 = max(0, end - cost);
-    g.x = x - y + cost;
-    g.h = unit / static_cast<unsigned>(s.qt);
-    g.u = unit - static_cast<unsigned>(g.h) * s.qt;
-    x += end - y;
-    if (g.k0 < g.k1) return true;
-   }
-   return false;
+    return false;
   }
 };
 // Keys that some row of row tile u sees: the last row's position + 1 (causal) or all of them.

@@ -101,6 +101,7 @@ class Rows:
 # What the attention kernels need beside their arguments, per (device, stream), where only calls that cannot overlap share it: the counters,
 # which are 0 between calls, and a workspace for calls that need little (for most, allocating one takes as long as the kernel).
 _SCRATCH = {}
+_lib.on_failed_status.append(_SCRATCH.clear)   # a call that was given up may leave its counters at anything
 _KEPT_BYTES = 4 << 20
 _NEED = {}
 

@@ -1,5 +1,6 @@
 """Refusals of the cache operators that need no GPU, the descriptors' checks, and the arithmetic that deals tiles to CTAs."""
 import bisect
+import ctypes
 import random
 
 import pytest
@@ -113,6 +114,71 @@ def test_every_tile_has_one_owner_and_every_cut_unit_is_joined_once():
                 assert all(a[2] == b[1] for a, b in zip(parts, parts[1:]))
                 cut.add(u)
         assert cut | whole == set(range(len(units))) and not cut & whole and len(slots) == sum(1 for s in slots)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_units_that_cost_something_to_begin_are_dealt_without_gaps(wide):
+    """The same with what a unit weighs besides its tiles: positions up to the cost stand for tile 0, and (wide: weights are in keys, linear in
+    the row tile, 128 to a key tile) positions behind the last tile for its end. The CTAs with parts are told from two positions."""
+    rng = random.Random(3)
+    cut = 0
+    for _ in range(400):
+        cost = rng.choice([256, 0]) if wide else rng.choice([0, 2, 3])
+        tiles = [rng.choice([1, 1, 2, 5, rng.randint(1, 300)]) for _ in range(rng.randint(1, 60))]
+        grid = rng.choice([1, 2, 7, 148, rng.randint(1, 400)])
+        # wide: keys of a unit as the weight has them, more or fewer than its tiles hold
+        weight = [cost + max(1, kt * 128 - rng.randint(-100, 300)) if wide else kt + cost for kt in tiles]
+        begin = [sum(weight[:i]) for i in range(len(tiles))]
+        w = sum(weight)
+        run = max(128 if wide else 1, -(-w // grid))
+
+        def tile(u, y):
+            if y >= weight[u]:
+                return tiles[u]
+            return 0 if y <= cost else min(tiles[u], -(-(y - cost) // 128) if wide else y - cost)
+
+        slots, whole = {}, set()
+        for c in range(grid):
+            x, x1 = min(w, c * run), min(w, (c + 1) * run)
+            while x < x1:
+                u = bisect.bisect_right(begin, x) - 1
+                y, end = x - begin[u], min(weight[u], x1 - begin[u])
+                k0, k1 = tile(u, y), tile(u, end)
+                x = begin[u] + end
+                if k0 == k1:
+                    continue
+                if k0 == 0 and k1 == tiles[u]:
+                    whole.add(u)
+                else:
+                    assert (c, k0 == 0) not in slots
+                    slots[c, k0 == 0] = u, k0, k1
+        firsts = set()
+        for u, kt in enumerate(tiles):
+            last = min(weight[u], cost + (kt - 1) * 128 + 1) - 1 if wide else cost + kt - 1
+            c = (begin[u] + cost) // run
+            n = (begin[u] + last) // run - c + 1
+            assert (n == 1) == (u in whole)
+            if n > 1:
+                parts = [slots.pop((c, True))] + [slots.pop((c + i, False)) for i in range(1, n)]
+                assert all(q[0] == u for q in parts) and parts[0][1] == 0 and parts[-1][2] == kt
+                assert all(a[2] == b[1] for a, b in zip(parts, parts[1:]))
+                assert c not in firsts   # the word its parts are counted in
+                firsts.add(c)
+                cut += 1
+        assert not slots
+    assert cut > 1000
+
+
+def test_an_abandoned_call_leaves_no_counters_behind(monkeypatch):
+    def failed(name, *args):
+        ctypes.c_int.from_address(args[1]).value = 1
+
+    monkeypatch.setattr(_lib, "call", failed)
+    monkeypatch.setattr(_lib, "stream", lambda: 0)
+    monkeypatch.setitem(kv_cache._SCRATCH, (0, 0), ("counters", "workspace"))
+    with pytest.raises(RuntimeError, match="device status 1"):
+        _lib.check_status()
+    assert not kv_cache._SCRATCH
 
 
 def test_a_prefix_falls_into_as_many_parts_as_the_workspace_holds():
