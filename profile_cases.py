@@ -4,6 +4,7 @@
     python profile_cases.py gemm  --M 8192 --N 12288 --K 4096 [--epi plain|gated|swiglu]
     python profile_cases.py quant --M 36436 --K 4096 [--kind plain|fp8|normmod|rot|normmod_rot]
     python profile_cases.py prepass --L 16384 --H 8
+    python profile_cases.py kv --kind attn|read|write --seqs 48 --new 1 --L 4096 --H 8 --group 8
 
 Each case builds seeded random inputs on the device, runs the kernel `--iters` times and prints the mean time
 from CUDA events, so the same command line serves a plain timing run and a profiler capture.
@@ -30,7 +31,7 @@ def _time(fn, iters):
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("case", choices=["attn", "gemm", "quant", "prepass", "conv", "vae", "mma_rate"])
+    ap.add_argument("case", choices=["attn", "gemm", "quant", "prepass", "conv", "vae", "mma_rate", "kv"])
     ap.add_argument("--L", type=int, default=16384)
     ap.add_argument("--H", type=int, default=8)
     ap.add_argument("--M", type=int, default=8192)
@@ -43,6 +44,10 @@ def main():
     ap.add_argument("--WW", type=int, default=42)
     ap.add_argument("--Cin", type=int, default=512)
     ap.add_argument("--Cout", type=int, default=512)
+    ap.add_argument("--seqs", type=int, default=48, help="kv: sequences, of L down to half of L tokens")
+    ap.add_argument("--new", type=int, default=1, help="kv: rows per sequence")
+    ap.add_argument("--group", type=int, default=8, help="kv: query heads per KV head (H of these)")
+    ap.add_argument("--codes", default="int8", choices=["int8", "fp8"], help="kv: the cache's codes")
     ap.add_argument("--iters", type=int, default=3)
     ap.add_argument("--rotate", action="store_true", help="attn / prepass: the token-scaled numerics")
     ap.add_argument("--rope", action="store_true", help="prepass: with the per-head RMSNorm + RoPE fused in")
@@ -102,6 +107,30 @@ def main():
                 print(f"mma_feed {where}, {fill // 1024} KB per stage: {ms:.3f} ms per launch, {ops.value / ms / 1e9:.0f} TOP/s, "
                       f"{148 * 40000 * fill / ms / 1e9:.1f} TB/s taken in", flush=True)
             del src
+        return
+    if a.case == "kv":
+        from rapid_h3_b200 import kv_cache
+        page = 64
+        width = -(-a.L // page)
+        cache = kv_cache.alloc(a.seqs * width, a.H, 128, page, a.codes)
+        lens = [max(a.new, a.L - i * a.L // (2 * a.seqs)) for i in range(a.seqs)]
+        table = torch.randperm(a.seqs * width, device="cuda", generator=g).int().view(a.seqs, width)
+
+        def batch(news):
+            starts = torch.tensor([0] + news, dtype=torch.int64).cumsum(0)
+            return kv_cache.Rows(table, *(torch.tensor(x).int().cuda() for x in (lens, starts.tolist()))), sum(news)
+
+        rows, total = batch(lens)
+        k, v = (randn(total, a.H, 128).to(torch.bfloat16) for _ in range(2))
+        kv_cache.write(cache, k, v, rows)
+        del k, v
+        rows, total = batch([a.new] * a.seqs)
+        x, y = (randn(total, a.H, 128).to(torch.bfloat16) for _ in range(2))
+        q = randn(total, a.H * a.group, 128).to(torch.bfloat16)
+        fn = {"attn": lambda: kv_cache.attention(q, cache, rows), "write": lambda: kv_cache.write(cache, x, y, rows),
+              "read": lambda: kv_cache.read(cache, rows, total, out=(x, y))}[a.kind]
+        ms = _time(fn, a.iters)
+        print(f"kv {a.kind} {a.codes}, {a.seqs} sequences of up to {a.L}, {a.new} rows each, {a.H} KV heads of {a.group}: {ms * 1e3:.1f} us")
         return
     if a.case == "conv":
         from rapid_h3_b200 import vae

@@ -13,6 +13,8 @@
 // 8 heads of 128 read as bf16, and 37 ragged prompts of up to 900 fp32 tokens written and read: 36.9 and 50.2 us, 94 and 87% of a copy's bandwidth
 // (rows of K and V in one warp, an address per row and a division per warp, 471 instructions: 48.5 and 58 us; four tokens a warp
 // besides: 84 and 69 us).
+#include <cuda_bf16.h>
+
 #include "kv_cache.cuh"
 #include "rapidh3_b200.h"
 
@@ -62,6 +64,50 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
+// largest magnitude of the eight
+template <int DT>
+__device__ __forceinline__ float kv_amax8(const KvRaw<DT>& r) {
+  if constexpr (DT == KV_F32) {
+    float x[8];
+    kv_unpack8<DT>(r, x);
+    float a = fabsf(x[0]);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) a = max_nan(a, fabsf(x[j]));
+    return a;
+  } else {   // two at a time, as they are
+    using T2 = std::conditional_t<DT == KV_F16, __half2, __nv_bfloat162>;
+    const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+    T2 m = __habs2(*reinterpret_cast<const T2*>(&w[0]));
+#pragma unroll
+    for (int j = 1; j < 4; ++j) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const T2*>(&w[j])));
+    return max_nan(__low2float(m), __high2float(m));
+  }
+}
+// quant8_e4m3 (the codes of the row quantizers) with the two tests for values near a tie of the product made once for all eight: of the smallest magnitude
+// and of the smallest distance of the 20 dropped bits from 0x7FFF0, moved to the top of the word
+__device__ __forceinline__ uint2 kv_quant8_e4m3(const float* y, float s, float inv) {
+  float yq[8], least = INFINITY;
+  uint32_t near = 0xFFFFFFFFu;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    yq[j] = __fmul_rn(y[j], inv);
+    least = fminf(least, fabsf(yq[j]));
+    near = min(near, __float_as_uint(yq[j]) * 4096u - 0x7FFF0u * 4096u);
+  }
+  if (least < 0.015625f || near < 0x20u * 4096u) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) yq[j] = __fdiv_rn(y[j], s);
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint16_t h;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(h) : "f"(yq[2 * j]), "f"(yq[2 * j + 1]));
+    w[j] = h;
+  }
+  return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+}
+
 struct KvWriteParams {
   KvCache c;
   KvRows r;
@@ -99,13 +145,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const KvWriteParam
   static_assert(KV_ITER == 4, "a group for each of four neighbouring lanes");
   float a[KV_ITER];
 #pragma unroll
-  for (int i = 0; i < KV_ITER; ++i) {
-    float x[8];
-    kv_unpack8<DT>(raw[i], x);
-    a[i] = fabsf(x[0]);
-#pragma unroll
-    for (int j = 1; j < 8; ++j) a[i] = max_nan(a[i], fabsf(x[j]));
-  }
+  for (int i = 0; i < KV_ITER; ++i) a[i] = kv_amax8<DT>(raw[i]);
   const bool odd = lane & 1, high = lane & 2;
   const float a0 = max_nan(odd ? a[1] : a[0], __shfl_xor_sync(0xffffffffu, odd ? a[0] : a[1], 1));
   const float a1 = max_nan(odd ? a[3] : a[2], __shfl_xor_sync(0xffffffffu, odd ? a[2] : a[3], 1));
@@ -126,7 +166,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const KvWriteParam
     float x[8];
     kv_unpack8<DT>(raw[i], x);
     uint2 q = make_uint2(0, 0);
-    if (s < INFINITY) q = FMT == RH3_KIND_I8 ? quant8_i8(x, s, inv) : quant8_e4m3(x, s, inv);
+    if (s < INFINITY) q = FMT == RH3_KIND_I8 ? quant8_i8(x, s, inv) : kv_quant8_e4m3(x, s, inv);
     if (first + i * ROWS < p.c.heads) *reinterpret_cast<uint2*>(code) = q;
   }
 }
