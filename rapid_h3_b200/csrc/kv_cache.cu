@@ -10,7 +10,7 @@
 // rows of one token, all of K or all of V, issues their loads before it works on the first, and looks up once where they lie
 // (sequence, page); a block's eight warps have eight tokens, whose codes and scales of a head are neighbours in a page. Instructions are
 // what such a warp has to save: its addresses are a pointer and a step, its token and part come from the grid. Measured, 36,436 tokens of
-// 8 heads of 128 read as bf16, and 37 ragged prompts of up to 900 fp32 tokens written and read: 36.9 and 50.2 us, 94 and 87% of a copy's bandwidth
+// 8 heads of 128 read as bf16, and 37 ragged prompts of up to 900 fp32 tokens written and read: 37 and 49 us, 93 and 90% of a copy's bandwidth
 // (rows of K and V in one warp, an address per row and a division per warp, 471 instructions: 48.5 and 58 us; four tokens a warp
 // besides: 84 and 69 us).
 #include <cuda_bf16.h>
@@ -83,29 +83,36 @@ __device__ __forceinline__ float kv_amax8(const KvRaw<DT>& r) {
     return max_nan(__low2float(m), __high2float(m));
   }
 }
-// quant8_e4m3 (the codes of the row quantizers) with the two tests for values near a tie of the product made once for all eight: of the smallest magnitude
-// and of the smallest distance of the 20 dropped bits from 0x7FFF0, moved to the top of the word
-__device__ __forceinline__ uint2 kv_quant8_e4m3(const float* y, float s, float inv) {
-  float yq[8], least = INFINITY;
-  uint32_t near = 0xFFFFFFFFu;
+// The codes of the row quantizers, of the quotients y / s rounded to fp32, without a division and without a branch: with inv = RN(1 / s) and q
+// within an ulp of y / s, r = y - q * s is exact in an FMA and RN(q + r * inv) is the rounded quotient (Markstein, "Computation of elementary
+// functions on the IBM RISC System/6000 processor", 1990). RN(y * inv) may be 1.5 ulp off, one such step brings it within an ulp. Nothing
+// leaves the normal numbers where it matters: s is at least 1e-12 and at most 2^128 / 127, and quotients too small for that give the code 0 either way. (bf16 rows have quotients that lie exactly between two codes: dividing where the product lies near
+// one, as the row quantizers do, sends a third of the warps down that path. 32 ragged prompts of up to 900 bf16 tokens to int8: 50 us that way, 43
+// this.)
+template <int FMT>
+__device__ __forceinline__ uint2 kv_quant8(const float* y, float s, float inv) {
+  float q[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    yq[j] = __fmul_rn(y[j], inv);
-    least = fminf(least, fabsf(yq[j]));
-    near = min(near, __float_as_uint(yq[j]) * 4096u - 0x7FFF0u * 4096u);
+    const float p = __fmul_rn(y[j], inv), near = __fmaf_rn(__fmaf_rn(-p, s, y[j]), inv, p);
+    q[j] = __fmaf_rn(__fmaf_rn(-near, s, y[j]), inv, near);
+    if constexpr (FMT == RH3_KIND_F8) q[j] = copysignf(q[j], y[j]);   // a zero keeps its sign
   }
-  if (least < 0.015625f || near < 0x20u * 4096u) {
+  if constexpr (FMT == RH3_KIND_I8) {
+    uint32_t t[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) yq[j] = __fdiv_rn(y[j], s);
-  }
-  uint32_t w[4];
+    for (int j = 0; j < 8; ++j) t[j] = __float_as_uint(__fadd_rn(q[j], 12582912.f));   // the integer in the low bits
+    return make_uint2(pack_low_bytes(t[0], t[1], t[2], t[3]), pack_low_bytes(t[4], t[5], t[6], t[7]));
+  } else {
+    uint32_t w[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint16_t h;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(h) : "f"(yq[2 * j]), "f"(yq[2 * j + 1]));
-    w[j] = h;
+    for (int j = 0; j < 4; ++j) {
+      uint16_t h;
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(h) : "f"(q[2 * j]), "f"(q[2 * j + 1]));
+      w[j] = h;
+    }
+    return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
   }
-  return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
 }
 
 struct KvWriteParams {
@@ -141,7 +148,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const KvWriteParam
   const int64_t place = kv_place(p.c, p.r, static_cast<int>(t), lane, p.status, &known);
   if (place < 0) return;
   // Largest magnitudes: the lanes of a row halve what they carry while they exchange, so that lane l ends with that of group l % 4, whose scale
-  // and inverse it works out for all (a butterfly and two divisions per group: 51.9 us instead of 50.2 for the prompts above).
+  // and inverse it works out for all (a butterfly and two divisions per group took 1.7 us more for the prompts above).
   static_assert(KV_ITER == 4, "a group for each of four neighbouring lanes");
   float a[KV_ITER];
 #pragma unroll
@@ -166,7 +173,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const KvWriteParam
     float x[8];
     kv_unpack8<DT>(raw[i], x);
     uint2 q = make_uint2(0, 0);
-    if (s < INFINITY) q = FMT == RH3_KIND_I8 ? quant8_i8(x, s, inv) : kv_quant8_e4m3(x, s, inv);
+    if (s < INFINITY) q = kv_quant8<FMT>(x, s, inv);
     if (first + i * ROWS < p.c.heads) *reinterpret_cast<uint2*>(code) = q;
   }
 }

@@ -152,6 +152,31 @@ def test_write_stores_codes_and_scales_and_read_gives_them_back(kv, kind, dtype,
             assert torch.equal(got[:-2].cpu(), ref) and bool((got[-2:] == 7).all())
 
 
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_codes_are_those_of_the_rounded_quotients(kv, kind, dtype):
+    """Rows of every magnitude, many of whose quotients lie at or next to a value between two codes."""
+    n, heads, d, page = 1024, 8, 128, 128
+    g = torch.Generator().manual_seed(7)
+    exponent = torch.randint(-44, 120, (n, heads, 1), generator=g).float()   # scales down to their lower limit
+    x = torch.rand(n, heads, d, generator=g) * 2 - 1
+    top = 1 + torch.rand(n, heads, 1, generator=g)
+    half = torch.randint(-254, 255, (n, heads, d), generator=g).float() / 254 * top.to(dtype).float()   # (k + 1/2) / 127 of the largest
+    wiggle = 1 + torch.randint(-3, 4, (n, heads, d), generator=g).float() * 2.0**-23
+    x = torch.where(torch.rand(n, heads, d, generator=g) < 0.7, half * wiggle, x)
+    x[..., :1] = top
+    x = (x * torch.exp2(exponent)).to(dtype)
+    cache = kv.alloc(n // page, heads, d, page, kind)
+    rows, table, starts = batch(kv, [n], [n], page, n // page, 8)
+    kv.write(cache, x.cuda(), x.flip(0).cuda(), rows)
+    q, s = okv.quantize(x, kind)
+    order = torch.tensor(table[0])
+    for of, want_q, want_s in ((0, q, s), (1, q.flip(0), s.flip(0))):
+        codes, scales = (t.view(torch.uint8)[order] if t.dtype != torch.float32 else t[order] for t in host(cache)[of::2])
+        assert torch.equal(scales.transpose(1, 2).reshape(n, heads), want_s)
+        assert torch.equal(codes.transpose(1, 2).reshape(n, heads, d), want_q.contiguous().view(torch.uint8))
+
+
 def test_rows_that_are_not_finite_read_back_as_nan_and_reach_nobody_else(kv, path):
     """A NaN or an infinity stays in its row's scale, and a masked row of that kind changes nothing."""
     for kind in ("int8", "fp8"):
