@@ -19,6 +19,8 @@
 // The order of channels and keys inside an mma is free, so each lane takes the channels and keys whose bytes it can load
 // 16 at a time: channel order (K) 16c .. 16c+15 of lane c, key order n -> (n >> 1) | ((n & 1) << 2), output channels of
 // lane group g 16g' .. 16g'+15.
+#include <algorithm>
+
 #include "kv_attn.cuh"
 #include "rapidh3_b200.h"
 
@@ -31,7 +33,8 @@ constexpr int KV_WARPS = 4;             // computing warps
 // 4,096 tokens 56.1, 53.8, 52.3; 64 of up to 700 behind a prefix 103, 88.2, 88.0.) 0 where every tile can have a CTA of its own.
 constexpr int KV_PLAIN_COST = 2, KV_OWN_COST = 3;
 constexpr int KV_NT = KV_WARPS * 32 + 32;
-enum { MODE_PLAIN = 0, MODE_PREFIX = 1, MODE_OWN = 2 };
+// no prefix; the prefix's own pass; the pass behind it, which takes its parts in; the prefix's tiles before every unit's own, in one pass
+enum { MODE_PLAIN = 0, MODE_PREFIX = 1, MODE_OWN = 2, MODE_ONE = 3 };
 
 template <int D, int NT>
 struct KvNarrow {
@@ -127,7 +130,7 @@ __device__ __forceinline__ KvLaneRow kv_lane_row(const KvAttnParams& p, const Kv
 // is where the warps' results meet).
 template <int BM>
 __device__ __forceinline__ int kv_last_tile(const KvAttnParams& p, const KvSegment& g) {
-  return max(g.k0 + 1, min(g.k1, (kv_visible<BM>(g.s, p.group, g.u, p.causal) + TK - 1) / TK));
+  return max(g.k0 + 1, min(g.k1, p.r.pre_tiles + (kv_visible<BM>(g.s, p.group, g.u, p.causal) + TK - 1) / TK));
 }
 // Joins the parts of a cut unit: slot 1 of CTA `first`, slot 0 of the ones behind it, in that order. They are
 // brought into the ring (which is done with) by bulk copies, as many as it holds at a time, and every thread sums its own fragments'
@@ -277,9 +280,10 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       }
       const int kend = kv_last_tile<BM>(p, g);
       for (int kt = g.k0; kt < kend; ++kt) {
-        const int at = kt * tile_pages + lane;
-        const bool need = lane < tile_pages && (static_cast<int64_t>(at) << p.c.page_log2) < g.s.len;
-        const int id = need ? p.r.table[g.b * p.r.table_stride + at] : -1;
+        const bool pre = MODE == MODE_ONE && kt < p.r.pre_tiles;
+        const int at = (MODE == MODE_ONE && !pre ? kt - p.r.pre_tiles : kt) * tile_pages + lane;
+        const bool need = lane < tile_pages && (static_cast<int64_t>(at) << p.c.page_log2) < (pre ? p.pre_len : g.s.len);
+        const int id = need ? (pre ? p.pre_table + at : p.r.table + g.b * p.r.table_stride + at)[0] : -1;
         const bool good = need && id >= 0 && id < p.c.pages;
         if (need && !good) kv_report(p.status, ST_KV_BAD_PAGE);
         const uint32_t mask = __ballot_sync(0xffffffffu, good);
@@ -422,10 +426,12 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       uint8_t* sv = sk + TK * D;
       const float* sks = scales + stage * 2 * TK + warp * 32;
       const uint32_t pages = tail->pages[stage];
-      const int key0 = warp * 32, pos0 = kt * TK + key0;
-      const bool whole = pages == (0xffffffffu >> (32 - (TK >> p.c.page_log2))) && kt * TK + TK <= g.s.len;
-      const bool masked = !whole || kt * TK + TK - 1 > pos_first;
-      auto there = [&](int key) { return pos0 + key < g.s.len && ((pages >> ((key0 + key) >> p.c.page_log2)) & 1u); };
+      const bool pre = MODE == MODE_ONE && kt < p.r.pre_tiles;   // of the prefix, which every row sees
+      const int tile0 = (MODE == MODE_ONE && !pre ? kt - p.r.pre_tiles : kt) * TK, len = pre ? p.pre_len : g.s.len;
+      const int key0 = warp * 32, pos0 = tile0 + key0;
+      const bool whole = pages == (0xffffffffu >> (32 - (TK >> p.c.page_log2))) && tile0 + TK <= len;
+      const bool masked = !whole || (!pre && tile0 + TK - 1 > pos_first);
+      auto there = [&](int key) { return pos0 + key < len && ((pages >> ((key0 + key) >> p.c.page_log2)) & 1u); };
       if (!whole) {
         // what was not loaded, or lies behind the sequence's end, may hold anything: a NaN code times a weight of 0 is a NaN
         if (!there(lane)) {
@@ -490,7 +496,7 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                if (!is || pos0 + key > pos[nt][e]) u[nt][kb][r][e] = -INFINITY;
+                if (!is || (!pre && pos0 + key > pos[nt][e])) u[nt][kb][r][e] = -INFINITY;
               }
           }
       }
@@ -710,18 +716,25 @@ struct KvPass {
   int64_t bm, kt, w, grid;      // rows of a unit, key tiles of a unit and weight of the pass at most, CTAs
   int cost;                     // what a unit weighs besides its tiles
 };
+// What a pass costs, by what it costs per SM: here 0.8 us for a tile of 16 rows and 0.5 for one of 8; in the wide kernel 10 us to begin with (tensor
+// memory, Q, the first tile's latency, the output), 2.6 us for a tile of 256 rows and 1.8 for one of up to 128. Measured at 128 channels; with
+// 8 KV heads 24 rows x 700 keys 17 / 23 us here / there, 512 x 12,000 130 / 40, 8,044 x 18,000 3,029 / 620. Sequences count as equally long.
+struct KvCost {
+  double narrow, wide;
+};
+KvCost kv_cost(int64_t heads, int64_t rows, int64_t seqs, int64_t kt) {
+  const int64_t each = (rows + seqs - 1) / seqs;
+  const double work = static_cast<double>(heads) * seqs * (kt < 1 ? 1 : kt) / device_sm_count();
+  return {(rows <= 8 * seqs ? 0.5 : 0.8 * ((each + 15) / 16)) * work, 10.0 + (each > 128 ? 2.6 * ((each + 255) / 256) : 1.8) * work};
+}
 KvPass kv_pass(int64_t heads, int64_t rows, int64_t seqs, int64_t kt, int cost) {
   KvPass x{};
   x.cost = cost;
   x.nt = rows <= 8 * seqs ? 1 : 2;
-  // Which kernel, by what the passes cost per SM: 0.8 us for a tile of 16 rows here; there 10 us to begin with (tensor memory, Q, the first
-  // tile's latency, the output), 2.6 us for a tile of 256 rows and 1.8 for one of up to 128 (measured at 128 channels; with 8 KV heads 24 rows x 700 keys
-  // 17 / 23 us here / there, 512 x 12,000 130 / 40, 8,044 x 18,000 3,029 / 620). Sequences count as equally long.
-  const int64_t each = (rows + seqs - 1) / seqs;
-  const double work = static_cast<double>(heads) * seqs * (kt < 1 ? 1 : kt) / device_sm_count();
   const int use = g_use_wide.load(std::memory_order_relaxed);
-  if (use >= 0) x.nt = use ? 0 : x.nt;
-  else if (each > 16 && 10.0 + (each > 128 ? 2.6 * ((each + 255) / 256) : 1.8) * work < 0.8 * ((each + 15) / 16) * work) x.nt = 0;
+  const KvCost cost_us = kv_cost(heads, rows, seqs, kt);
+  if (use >= 0) x.nt = use == 1 ? 0 : x.nt;
+  else if ((rows + seqs - 1) / seqs > 16 && cost_us.wide < cost_us.narrow) x.nt = 0;
   x.bm = x.nt ? 8 * x.nt : KV_WIDE_BM;
   x.kt = kt < 1 ? 1 : kt;
   const int64_t units = heads * (rows / x.bm + seqs);
@@ -732,7 +745,8 @@ KvPass kv_pass(int64_t heads, int64_t rows, int64_t seqs, int64_t kt, int cost) 
   return x;
 }
 struct KvPlan {
-  KvPass own, pre;              // pre.grid = 0: no pass of its own for the prefix (none, or its tiles are among the wide units' own)
+  KvPass own, pre;              // pre.grid = 0: no pass of its own for the prefix (none, or its tiles come before the units' own)
+  bool one;                     // its tiles come before the units' own
   int64_t pre_run, pre_unit, pre_first, pre_last;   // see KvAttnParams
   int64_t pre_splits;           // into how many parts the prefix pass's units may fall
   int64_t part, pre_ml, pre_o, bytes;   // byte offsets
@@ -746,9 +760,22 @@ KvPlan kv_plan(int64_t heads, int64_t group, int64_t page, int64_t D, int64_t pe
     return at;
   };
   x.own = kv_pass(heads, rows, seqs, own_kt, prefix > 0 ? KV_OWN_COST : KV_PLAIN_COST);
-  if (x.own.nt == 0) x.own = kv_pass(heads, rows, seqs, own_kt + pre_kt, KV_PLAIN_COST);
-  x.part = take(x.own.grid * 2 * (x.own.nt ? x.own.bm * D + 2 * x.own.bm : kv_wide_part_floats(D)) * sizeof(float));
   if (prefix > 0 && x.own.nt) {
+    // A pass of its own for the prefix takes some 7 us besides its work (its launch, its parts written and taken in). Without it every sequence's units
+    // work on the prefix's tiles, from L2 mostly. (us in one pass / in two, 8 KV heads of 4, a row per sequence: 6 sequences behind 700
+    // tokens 11.8 / 15.9, 64 30.5 / 31.8; 6 behind 4,000 17.8 / 25.2, 16 30.7 / 27.7; 64 x 8 rows behind 12,000 222 / 197, with the prefix on
+    // the tensor-core tiles 88.)
+    const double here = kv_cost(heads, rows, seqs, pre_kt).narrow;
+    const KvCost apart = kv_cost(heads, rows, 1, pre_kt);
+    x.one = g_use_wide.load(std::memory_order_relaxed) != 2 && here - std::min(apart.narrow, apart.wide) < 7.0;
+  }
+  if (prefix > 0 && (x.one || x.own.nt == 0)) {
+    const KvPass both = kv_pass(heads, rows, seqs, own_kt + pre_kt, KV_PLAIN_COST);
+    x.one = x.own.nt == 0 || both.nt;   // many rows are worked on with the prefix's tiles, if at all
+    if (x.one) x.own = both;
+  }
+  x.part = take(x.own.grid * 2 * (x.own.nt ? x.own.bm * D + 2 * x.own.bm : kv_wide_part_floats(D)) * sizeof(float));
+  if (prefix > 0 && !x.one) {
     x.pre = kv_pass(heads, rows, 1, pre_kt, KV_PLAIN_COST);
     const int64_t units = heads * ((rows + x.pre.bm - 1) / x.pre.bm);
     x.pre_unit = x.pre.nt ? x.pre.cost + pre_kt : KV_WIDE_UNIT_COST + prefix;   // in tiles or in keys
@@ -777,7 +804,7 @@ extern "C" int64_t rh3_kv_attn_workspace_bytes(int64_t heads, int64_t group, int
   return kv_plan(heads, group, page, D, per_seq, B, T, prefix).bytes;
 }
 
-extern "C" int rh3_kv_attn_use_wide(int use) { return g_use_wide.exchange(use < 0 ? -1 : use ? 1 : 0); }
+extern "C" int rh3_kv_attn_use_wide(int use) { return g_use_wide.exchange(use < 0 || use > 2 ? -1 : use); }
 
 extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t workspace_bytes, int32_t* counters, cudaStream_t stream) {
   RH3_CHECK_ARG(a, "kv_attn: null arguments");
@@ -811,12 +838,12 @@ extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t w
   p.most = static_cast<int>(x.own.w);
   p.cost = x.own.cost;
   p.part = reinterpret_cast<float*>(ws + x.part);
-  if (x.own.nt == 0) {
+  if (x.one) {
     p.r.pre_tiles = static_cast<int>((a->prefix + TK - 1) / TK);
     p.pre_table = a->prefix_table;
     p.pre_len = static_cast<int>(a->prefix);
-    return kv_wide_launch(p, a->D, a->kind, false, x.own.grid, stream);
   }
+  if (x.own.nt == 0) return kv_wide_launch(p, a->D, a->kind, false, x.own.grid, stream);
   CUtensorMap mk, mv;
   if (int e = kv_maps(&mk, &mv, p.c, a->D)) return e;
   auto launch = [&](auto mode, const KvAttnParams& q, const KvPass& pass) {
@@ -831,6 +858,7 @@ extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t w
     return pass.nt == 1 ? by_kind(std::integral_constant<int, 64>(), One()) : by_kind(std::integral_constant<int, 64>(), Two());
   };
   if (a->prefix == 0) return launch(std::integral_constant<int, MODE_PLAIN>(), p, x.own);
+  if (x.one) return launch(std::integral_constant<int, MODE_ONE>(), p, x.own);
   p.pre_ml = reinterpret_cast<float*>(ws + x.pre_ml);
   p.pre_o = reinterpret_cast<float*>(ws + x.pre_o);
   p.pre_unit = static_cast<int>(x.pre_unit);

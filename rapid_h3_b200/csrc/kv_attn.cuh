@@ -40,7 +40,7 @@ struct KvAttnParams {
   // which parts the prefix pass leaves of a unit, in its measure of work: a CTA has pre_run of it, a unit weighs pre_unit; the CTAs that
   // positions pre_first and pre_last of a unit belong to have its first and its last part
   int pre_run, pre_unit, pre_first, pre_last, pre_bm;
-  // shared prefix in the wide kernel's single pass: r.pre_tiles tiles of it before a unit's own
+  // shared prefix in a single pass: r.pre_tiles tiles of it before a unit's own
   const int* pre_table;
   int pre_len;
 };

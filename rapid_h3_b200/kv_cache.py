@@ -118,12 +118,18 @@ def _scratch(device, index, stream, need):
     return kept if need <= _KEPT_BYTES else (kept[0], torch.empty(need, device=device, dtype=torch.uint8))
 
 
+_PATHS = (None, False, True, "apart")
+
+
 def use_wide(use):
     """Which kernel attention runs on: None (the default) the cheaper one for a call's sizes, False the one for few rows per sequence, True the one
-    on 128-row tensor-core tiles. For the whole process; returns the previous setting."""
-    before = _lib.lib().rh3_kv_attn_use_wide(-1 if use is None else int(use))
+    on 128-row tensor-core tiles; "apart": as False, and a shared prefix always has a pass of its own. For the whole process; returns
+    the previous setting."""
+    if not any(use is x for x in _PATHS[:3]) and use != "apart":
+        raise RuntimeError(f"expected one of {_PATHS}, got {use!r}")
+    before = _lib.lib().rh3_kv_attn_use_wide(_PATHS.index(use) - 1)
     _NEED.clear()
-    return None if before < 0 else bool(before)
+    return _PATHS[before + 1]
 
 
 def _workspace_bytes(*sizes):

@@ -33,6 +33,13 @@ def path(kv, request):
     kv.use_wide(before)
 
 
+@pytest.fixture(params=[False, "apart", True], ids=["few rows", "few rows, prefix apart", "many rows"])
+def prefix_path(kv, request):
+    before = kv.use_wide(request.param)
+    yield
+    kv.use_wide(before)
+
+
 def fill(cache, seed):
     """Random codes and scales in every slot of the cache, valid or not."""
     g = torch.Generator().manual_seed(seed)
@@ -253,7 +260,7 @@ def test_values_without_sense_are_cut_to_what_exists(kv, path):
     ([0], [1], 1), ([64, 1, 0, 130], [1, 1, 1, 1], 700), ([33, 160, 7], [33, 60, 0], 129), ([5, 300], [2, 9], 0),
 ])
 @pytest.mark.parametrize("causal", [True, False])
-def test_attention_behind_a_shared_prefix(kv, path, kind, dtype, d, page, heads, group, lens, news, prefix, causal):
+def test_attention_behind_a_shared_prefix(kv, prefix_path, kind, dtype, d, page, heads, group, lens, news, prefix, causal):
     pre = -(-prefix // page)
     pages = sum(-(-n // page) for n in lens) + pre + 2
     cache = kv.alloc(pages, heads, d, page, kind)
