@@ -403,7 +403,8 @@ int rh3_vae_gemm_swiglu(const void* xq, int64_t lda, const void* wq, const float
  *   query heads, head h * group + i reads KV head h. A row without a key gives 0. With prefix > 0 every row sees the first
  *   `prefix` tokens of prefix_table's pages as well, before its own keys; lens, starts and positions then count the own part alone.
  *   workspace: rh3_kv_attn_workspace_bytes() bytes, 256-byte aligned, in use until the call's kernels are done. counters:
- *   RH3_KV_COUNTERS ints on the device, 0 before a call and left 0 by it; calls that may overlap (other streams, graphs) need their own. */
+ *   RH3_KV_COUNTERS ints on the device, 0 before a call and left 0 by it (clear them after a call that gave up: a status other than 0, 120 and 121);
+ *   calls that may overlap (other streams, graphs) need their own. */
 #define RH3_KV_COUNTERS 1024
 typedef struct rh3_kv_attn_args {
   const void* q; int64_t q_st, q_sh;   /* [T][heads * group][D], token and head strides */

@@ -402,6 +402,46 @@ def test_a_captured_step_follows_lengths_and_pages(kv, path):
             assert torch.equal(x, ref.to(torch.bfloat16))
 
 
+def test_a_captured_call_behind_a_prefix_with_rows_that_no_sequence_has(kv, prefix_path):
+    """Rows before the first sequence and behind the last hold NaN and stay; lengths and the prefix's pages change between
+    replays; a second graph of the same call is replayed on another stream meanwhile."""
+    heads, group, d, page, prefix = 2, 3, 64, 16, 150
+    cache = kv.alloc(80, heads, d, page, "int8")
+    fill(cache, 46)
+    dev = dict(dtype=torch.int32, device="cuda")
+    table = torch.arange(40, **dev).view(2, 20).contiguous()
+    pre = torch.arange(40, 50, **dev)
+    lens = torch.tensor([260, 33], **dev)
+    rows = kv.Rows(table, lens, torch.tensor([2, 9, 42], **dev))
+    q = torch.full((50, heads * group, d), float("nan"), dtype=torch.float16, device="cuda")
+    outs = [torch.full_like(q, 3.0) for _ in range(2)]
+    kv.attention_shared(q, cache, rows, pre, prefix, out=outs[0])   # kernels loaded
+    outs[0].fill_(3.0)
+    graphs = []
+    for out in outs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            for _ in range(3):
+                kv.attention_shared(q, cache, rows, pre, prefix, out=out)
+    side = torch.cuda.Stream()
+    g = torch.Generator().manual_seed(47)
+    for i in range(3):
+        q[2:42] = torch.randn(40, heads * group, d, generator=g).to(torch.float16).cuda()
+        if i:
+            lens += 13
+            pre.copy_(pre.flip(0) if i == 1 else pre + 20)
+        side.wait_stream(torch.cuda.current_stream())
+        for _ in range(4):
+            graphs[0].replay()
+            with torch.cuda.stream(side):
+                graphs[1].replay()
+        torch.cuda.current_stream().wait_stream(side)
+        for out in outs:
+            assert bool((out[:2] == 3).all()) and bool((out[42:] == 3).all())
+            check_attention(out[2:42], q[2:42], cache, table.tolist(), lens.tolist(), [0, 7, 40], prefix=pre.tolist(), prefix_len=prefix)
+        assert torch.equal(*outs)
+
+
 def test_calls_on_two_streams_at_once(kv, path):
     """Each stream has counters and a workspace of its own: results as one after the other."""
     cache = kv.alloc(80, 2, 128, 64, "fp8")
