@@ -14,6 +14,7 @@ Keys and values are stored per token and KV head as 8-bit codes with one fp32 sc
 the cache's device, and the work goes to that device's current stream. Everything is CUDA; there is no fallback.
 """
 import struct
+import threading
 from dataclasses import dataclass
 
 import torch
@@ -103,6 +104,7 @@ class Rows:
 _SCRATCH = {}
 _lib.on_failed_status.append(_SCRATCH.clear)   # a call that was given up may leave its counters at anything
 _KEPT_BYTES = 4 << 20
+_LAUNCH = threading.Lock()   # a call's kernels go to the stream together: another thread's would use the same workspace between them
 _NEED = {}
 
 
@@ -188,7 +190,7 @@ def read(cache, rows, total, dtype=torch.bfloat16, out=None):
         raise RuntimeError(f"dtype must be one of {tuple(_DTYPES)}, got {dtype}")
     shape = (total, cache.kv_heads, cache.head_dim)
     if out is None:
-        k, v = torch.empty((2, *shape), device=cache.device, dtype=dtype).unbind(0)
+        k, v = cache.k.new_empty(shape, dtype=dtype), cache.k.new_empty(shape, dtype=dtype)
     else:
         k, v = out
         for t in (k, v):
@@ -226,7 +228,8 @@ def _attend(q, cache, rows, prefix, prefix_len, scale, causal, out):
         stream = _lib.stream()
         need = _workspace_bytes(cache.kv_heads, group, cache.page, d, *rows._sizes, t, prefix_len)
         counters, work = _scratch(q.device, cache._index, stream, need)
-        _lib.call("rh3_kv_attn", args, work.data_ptr(), need, counters.data_ptr(), stream)
+        with _LAUNCH:
+            _lib.call("rh3_kv_attn", args, work.data_ptr(), need, counters.data_ptr(), stream)
 
     _run(cache._index, launch)
     return out

@@ -7,6 +7,7 @@ denominator. Weights move the output by at most their relative error times sum_j
 about twice the magnitudes, and the kernel for many rows rounds V to fp16 (2^-11 of a value, and 2^-25 of twice the largest row's magnitude where that
 is more)."""
 import random
+import threading
 
 import pytest
 import torch
@@ -460,6 +461,35 @@ def test_calls_on_two_streams_at_once(kv, path):
     torch.cuda.synchronize()
     for got, (_, _, want, _) in zip(outs, cases):
         assert all(torch.equal(x, want) for x in got)
+
+
+def test_calls_of_several_threads_on_one_stream(kv, prefix_path):
+    """They share the stream's counters and workspace."""
+    heads, group, d, page, prefix = 2, 4, 128, 64, 1000
+    cache = kv.alloc(60, heads, d, page, "int8")
+    fill(cache, 48)
+    pre = torch.arange(16, dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(49)
+    calls = []
+    for i in range(4):
+        rows, _, _ = batch(kv, [70, 130, 9 + i], [1, 2, 1], page, 40, 50 + i)
+        rows = kv.Rows(rows.table + 16, rows.lens, rows.starts)
+        q = torch.randn(4, heads * group, d, generator=g).to(torch.bfloat16).cuda()
+        calls.append((q, rows, kv.attention_shared(q, cache, rows, pre, prefix)))
+    wrong, stream = [], torch.cuda.current_stream()
+
+    def work(q, rows, want):
+        with torch.cuda.stream(stream):
+            for _ in range(100):
+                if not torch.equal(kv.attention_shared(q, cache, rows, pre, prefix), want):
+                    wrong.append(q)
+
+    threads = [threading.Thread(target=work, args=c) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_pages_behind_32_bit_offsets(kv, path):
