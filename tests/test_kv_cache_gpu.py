@@ -492,6 +492,24 @@ def test_calls_of_several_threads_on_one_stream(kv, prefix_path):
     assert not wrong
 
 
+def test_sequences_without_pages(kv, prefix_path):
+    """A table of no columns: rows see the prefix alone, or nothing; nothing is written, zeros are read."""
+    cache = kv.alloc(4, 2, 64, 32, "fp8")
+    fill(cache, 51)
+    before = host(cache)
+    dev = dict(dtype=torch.int32, device="cuda")
+    rows = kv.Rows(torch.empty(3, 0, **dev), torch.tensor([0, 5, 0], **dev), torch.tensor([0, 1, 1, 4], **dev))
+    q = torch.randn(4, 6, 64, generator=torch.Generator().manual_seed(52)).to(torch.bfloat16).cuda()
+    assert bool((kv.attention(q, cache, rows) == 0).all())
+    out = kv.attention_shared(q, cache, rows, torch.tensor([3, 1], **dev), 33)
+    check_attention(out, q, cache, [[], [], []], [0, 0, 0], [0, 1, 1, 4], prefix=[3, 1], prefix_len=33)
+    kv.write(cache, q[:, :2], q[:, 2:4], rows)
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(host(cache), before))
+    assert all(bool((t == 0).all()) for t in kv.read(cache, rows, 4))
+    none = torch.empty(0, **dev)
+    assert bool((kv.attention_shared(q, cache, rows, none, 0) == 0).all())
+
+
 def test_pages_behind_32_bit_offsets(kv, path):
     """A cache whose codes take more than 2^32 bytes: pages at its end are written, read and attended to."""
     page, heads, d = 128, 16, 128
