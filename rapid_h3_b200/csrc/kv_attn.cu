@@ -6,7 +6,8 @@
 // leaves a partial result, and the one whose is the last joins them, in a fixed order.
 //
 // One CTA = a producer warp and four warps that compute, each on 32 of a tile's 128 keys with its own running maximum, sums and
-// output, joined at the unit's end: no barrier among them per tile. The producer brings pages by TMA into a ring
+// output, joined at the unit's end: no barrier among them per tile. Keys of a shared prefix come before a unit's own, or have been worked on in a pass
+// before, whose parts a unit takes in (kv_plan). The producer brings pages by TMA into a ring
 // (128-byte swizzle over the codes as they lie, so that the accesses below hit 32 banks), their scales by bulk copies.
 //
 // Products are mma.sync m16n8k16 on fp16 with the KEYS (and then the channels) as the 16 rows and the query rows as the 8 columns:
@@ -16,6 +17,7 @@
 // instructions for four of them. K codes enter as code + 128 in the low bits of an fp16 (a subnormal number, (code + 128) * 2^-24,
 // exact): the accumulators begin at -128 * 2^-24 * sum q, the same for every key of a row. V codes are brought to fp16 proper: there the
 // offset would be summed over all keys.
+// Measured: a token of each of 48 sequences of 8,192 to 16,384 tokens, 8 KV heads of 8: 203 us, 6.26 TB/s (0.96 of a copy); of up to 4,096: 52 us.
 // The order of channels and keys inside an mma is free, so each lane takes the channels and keys whose bytes it can load
 // 16 at a time: channel order (K) 16c .. 16c+15 of lane c, key order n -> (n >> 1) | ((n & 1) << 2), output channels of
 // lane group g 16g' .. 16g'+15.
@@ -707,7 +709,7 @@ int kv_launch(const CUtensorMap& mk, const CUtensorMap& mv, const KvAttnParams& 
   return check_cuda(launch_chained(kern, dim3(static_cast<unsigned>(grid)), KV_NT, smem, stream, 1, mk, mv, p), "kv_attn launch");
 }
 
-// rh3_kv_attn_use_wide: -1 by cost, 0 never, 1 always
+// rh3_kv_attn_use_wide: -1 by cost, 0 never, 1 always, 2 never and a prefix has a pass of its own
 std::atomic<int> g_use_wide{-1};
 
 // The plan of a call: which kernel and rows per unit, grids and the pieces of its workspace.

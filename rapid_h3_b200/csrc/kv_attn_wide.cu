@@ -22,7 +22,8 @@
 // The same layout is K-major for K and, with the channels as the product's N, MN-major for V, so nothing is transposed.
 // Shared memory: Q 2 x 32 KB | three fp16 tiles of 32 KB (K and V in turn) | three raw tiles of 16 KB. TMEM: S0 | S1 | O0 | O1.
 // Bound, per step of 128 keys and 256 rows: 2,048 cycles of the tensor pipe, as many of the exponential unit, about 2,800 of shared memory (products'
-// operands 1,536, conversion 768, the keys' scales 512).
+// operands 1,536, conversion 768, the keys' scales 512). Measured: 4,850, as all three wait for one another; 2,011 tokens x 32 heads behind
+// 16,000 take 620 us, 0.90 PFLOP/s (0.55 of the library's bf16 product).
 #include "kv_attn.cuh"
 
 namespace rh3 {
