@@ -116,7 +116,9 @@ int kv_allow_smem(K kern, int smem, std::atomic<uint64_t>& done) {
 
 // kv_attn_wide.cu: the same parameters, units of 256 rows; floats of one of its partial results
 constexpr int KV_WIDE_BM = 256;
-constexpr int KV_WIDE_UNIT_COST = 256;   // what a unit costs besides its keys, in keys
+// What a unit costs besides its keys, in keys: some 12 us of Q, first tile and output. (us with 256 / 512 / 640 / 1,024, 8 KV heads: 10 prompts of up to
+// 512 x 4 rows behind 1,024 tokens 124 / 115 / 116 / 116, 37 fresh ones of up to 900 x 8 710 / 621 / 597 / 606, 4 of 1,500 x 4 183 / 168 / 169 / 178.)
+constexpr int KV_WIDE_UNIT_COST = 640;
 int64_t kv_wide_part_floats(int64_t D);
 int kv_wide_launch(const KvAttnParams& p, int64_t D, int kind, bool prefix, int64_t grid, cudaStream_t stream);
 

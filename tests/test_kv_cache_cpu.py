@@ -123,7 +123,7 @@ def test_units_that_cost_something_to_begin_are_dealt_without_gaps(wide):
     rng = random.Random(3)
     cut = 0
     for _ in range(400):
-        cost = rng.choice([256, 0]) if wide else rng.choice([0, 2, 3])
+        cost = rng.choice([640, 256, 0]) if wide else rng.choice([0, 2, 3])
         tiles = [rng.choice([1, 1, 2, 5, rng.randint(1, 300)]) for _ in range(rng.randint(1, 60))]
         grid = rng.choice([1, 2, 7, 148, rng.randint(1, 400)])
         # wide: keys of a unit as the weight has them, more or fewer than its tiles hold
