@@ -472,7 +472,9 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float ks = sks[kb * 16 + r * 8 + kg], vs = fmaxf(sks[TK + kb * 16 + r * 8 + kg], kVsMin);
+          float ks = sks[kb * 16 + r * 8 + kg];
+          const float v_scale = sks[TK + kb * 16 + r * 8 + kg], vs = fmaxf(v_scale, kVsMin);
+          if (!(v_scale < INFINITY)) ks = kNan;   // a V row that is not finite: its codes are 0, fmaxf would drop a NaN
           const float lv = kv_lg2(vs);
           iv[kb][r] = kv_rcp(vs);
 #pragma unroll

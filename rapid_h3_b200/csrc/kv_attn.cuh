@@ -10,6 +10,7 @@
 // products, sums, m, l and O are fp32. Partial results over parts of the keys carry (O, m, l) with the same m for both.
 #pragma once
 #include <atomic>
+#include <limits>
 
 #include "kv_cache.cuh"
 #include "rapidh3_b200.h"
@@ -78,6 +79,8 @@ constexpr float kWeightLog2 = 15.f;   // the largest weight is 2^15: the most th
 
 // V scales as the kernels use them: a slot that was never written may hold 0
 constexpr float kVsMin = 1e-30f;
+// what makes a key's scores NaN, and so every row that sees it and no other
+constexpr float kNan = std::numeric_limits<float>::quiet_NaN();
 
 // Four codes of a word as two fp16 pairs: (byte 0, byte 1), (byte 2, byte 3), exactly.
 template <int FMT>

@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
         } else {   // the keys' scales
           const bool is = there(tid);
           float ks = tail->scale[s][0][tid], vs = is ? tail->scale[s][1][tid] : 0.f;
-          if (!(vs < INFINITY)) vs = 0.f, ks = __uint_as_float(0x7FC00000u);
+          if (!(vs < INFINITY)) vs = 0.f, ks = kNan;
           const float top = warp_max(vs);
           if (lane == 0) tail->top[parity][warp & 3] = top;
           if (bar_sync_or(5, 128, !ok)) {

@@ -1,0 +1,89 @@
+"""Edges of the cache operators' definitions, both attention kernels on each: rows that are not finite, lengths and row starts that do not fit
+the table or the call, V rows of very different size, outputs that overlap.
+
+Tolerance, derived for each row and head: the output is rounded once (eps / 2 of its value). A weight moves it by its relative error times
+sum_j p_j |v_j|, in numerator and denominator: 2^-11 for its rounding to fp16, 2^-14 for exponents of up to 2^9 (the score's and the V
+scale's, in steps of 2^-15) and approximate exp2, log2 and reciprocal, and 2^-22 of the score's magnitude for each of D / 16 tensor-core steps and two
+products (twice that, as K codes may enter as code + 128). The kernel for many rows rounds V (2^-11 of a value). There weights are fp16 whose
+largest, with its V scale, is at least 2^3: one below 2^-14 is off by up to 2^-25 whatever its size, and its V at most 2^7 times the largest's."""
+import pytest
+import torch
+
+from oracle import kv_cache as okv
+from test_kv_cache_gpu import batch, fill, host, kv, path, prefix_path  # noqa: F401  (the fixtures of both kernels)
+
+pytestmark = pytest.mark.gpu
+I32 = dict(dtype=torch.int32, device="cuda")
+
+
+def reference(q, cache, table, lens, starts, scale=None, causal=True, prefix=(), prefix_len=0):
+    """(out, tolerance) fp64 [T, heads, D] from the definition; rows of no sequence are NaN."""
+    k, v, ks, vs = host(cache)
+    q = q.cpu().double()
+    t, heads, d = q.shape
+    group = heads // k.shape[1]
+    scale = d ** -0.5 if scale is None else scale
+    ref, tol = (torch.full((t, heads, d), float("nan"), dtype=torch.float64) for _ in range(2))
+    pre = [okv.tokens(c, s, prefix, prefix_len) for c, s in ((k, ks), (v, vs))]
+    for b, n in enumerate(lens):
+        room = max(0, min(n, len(table[b]) * k.shape[2]))
+        own = [okv.tokens(c, s, table[b], room) for c, s in ((k, ks), (v, vs))]
+        for r in range(max(0, starts[b]), min(t, starts[b + 1])):
+            seen = own[0][1] & (torch.arange(room) <= n - (starts[b + 1] - r) if causal else True)
+            kk, vv = (torch.cat([p[0][p[1]], o[0][seen]]).repeat_interleave(group, 1) for p, o in zip(pre, own))
+            if len(kk) == 0:
+                ref[r], tol[r] = 0, 0
+                continue
+            p = torch.softmax(scale * torch.einsum("khd,hd->kh", kk, q[r]), 0)
+            ref[r] = torch.einsum("kh,khd->hd", p, vv)
+            mag = torch.einsum("kh,khd->hd", p, vv.abs())
+            size = scale * torch.einsum("khd,hd->kh", kk.abs().amax(2, keepdim=True).expand_as(kk), q[r].abs()).amax(0)
+            peak = (p * vv.abs().amax(2)).amax(0)
+            tol[r] = (mag * (2 * 2**-11 + 2**-14 + 2 * (d // 16 + 2) * 2**-22 * 2 * size[:, None]) + len(kk) * 2**-21 * peak[:, None])
+    return ref, tol
+
+
+def check(out, q, cache, table, lens, starts, **kw):
+    ref, tol = reference(q, cache, table, lens, starts, **kw)
+    has = ~torch.isnan(tol).all(2).all(1)
+    tol = tol + torch.finfo(q.dtype).eps / 2 * ref.abs() + torch.finfo(q.dtype).tiny
+    err = (out.cpu().double() - ref).abs()[has]
+    assert torch.isfinite(out.cpu()[has]).all()
+    assert bool((err <= tol[has]).all()), float((err / tol[has]).max())
+
+
+def randn(seed, *shape, dtype=torch.bfloat16):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_a_v_row_that_is_not_finite_reaches_the_rows_that_see_it(kv, prefix_path, kind, dtype, d, value):
+    """V alone, K clean: every row that sees the key becomes NaN in that KV head, every other row and head stays as it was, bit for bit."""
+    cache = kv.alloc(12, 2, d, 16, kind)
+    rows, table, starts = batch(kv, [60, 9], [40, 9], 16, 8, 1)
+    whole = kv.Rows(rows.table, rows.lens, torch.tensor([0, 60, 69], **I32))
+    pre, pre_rows = torch.tensor([8, 11, 9], **I32), kv.Rows(torch.tensor([[8, 11, 9]], **I32), torch.tensor([37], **I32), torch.tensor([0, 37], **I32))
+    k, v = (randn(s, 69, 2, d, dtype=dtype) for s in (2, 3))
+    pk, pv = (randn(s, 37, 2, d, dtype=dtype) for s in (4, 5))
+    q = randn(6, 49, 16, d, dtype=dtype).cuda()
+
+    def outs():
+        kv.write(cache, k.cuda(), v.cuda(), whole)
+        kv.write(cache, pk.cuda(), pv.cuda(), pre_rows)
+        return [kv.attention(q, cache, rows), kv.attention(q, cache, rows, causal=False), kv.attention_shared(q, cache, rows, pre, 37)]
+
+    clean = outs()
+    v[41, 1, d // 2] = value                    # position 41 of the first sequence, whose rows are positions 20 to 59
+    sees = torch.zeros(49, dtype=torch.bool)
+    sees[21:40] = True
+    every = torch.arange(49) < 40
+    for out, was, who in zip(outs(), clean, (sees, every, sees)):
+        assert bool(torch.isnan(out[who.cuda()][:, 8:]).all())
+        assert torch.equal(out[:, :8], was[:, :8]) and torch.equal(out[~who.cuda()], was[~who.cuda()])
+    v[41, 1, d // 2] = 1
+    pv[5, 0, 0] = value
+    out = outs()[2]
+    assert bool(torch.isnan(out[:, :8]).all()) and torch.isfinite(out[:, 8:]).all()
