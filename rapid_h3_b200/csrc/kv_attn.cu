@@ -474,7 +474,9 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
         for (int r = 0; r < 2; ++r) {
           float ks = sks[kb * 16 + r * 8 + kg];
           const float v_scale = sks[TK + kb * 16 + r * 8 + kg], vs = fmaxf(v_scale, kVsMin);
-          if (!(v_scale < INFINITY)) ks = kNan;   // a V row that is not finite: its codes are 0, fmaxf would drop a NaN
+          // A row of K or V that is not finite has codes 0. fmaxf would drop a NaN of V's, and what the offset of the codes leaves of a sum
+          // that should be 0 times an infinite scale may be -inf, a key left out.
+          if (!(max_nan(ks, v_scale) < INFINITY)) ks = kNan;
           const float lv = kv_lg2(vs);
           iv[kb][r] = kv_rcp(vs);
 #pragma unroll

@@ -12,7 +12,7 @@
 // at most 2^15 and O is hardly ever touched between products (2,011 tokens behind 16,000: 632 us where it might outgrow it by 2^8, 618 by 2^12). e is the exponent of the largest V scale so far: V's one rounding
 // is 2^-11 of a value (2^-25 of the largest row's magnitude for what is smaller than 2^-14 of it), as much as that of the
 // weights. (In the exponent, as in kv_attn.cu, the V scales cost a softmax thread two more floats a key and two more operations a
-// score.) A key whose V scale is not finite has V = 0 and a K scale that is not a number: only the rows that see it become NaN.
+// score.) A key with a scale that is not finite has V = 0 and a K scale that is not a number: only the rows that see it become NaN.
 //
 // 896 threads, one CTA per SM: warp 0 brings pages by bulk copies (codes as they lie), warp 1 issues the products, warp 2 works out the run's segments and tells
 // the others, warps 4-19 are the softmax, eight
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
         } else {   // the keys' scales
           const bool is = there(tid);
           float ks = tail->scale[s][0][tid], vs = is ? tail->scale[s][1][tid] : 0.f;
-          if (!(vs < INFINITY)) vs = 0.f, ks = kNan;
+          if (!(max_nan(ks, vs) < INFINITY)) vs = 0.f, ks = kNan;
           const float top = warp_max(vs);
           if (lane == 0) tail->top[parity][warp & 3] = top;
           if (bar_sync_or(5, 128, !ok)) {

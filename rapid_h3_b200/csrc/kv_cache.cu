@@ -57,13 +57,6 @@ __device__ __forceinline__ void kv_unpack8(const KvRaw<DT>& r, float* x) {
     for (int j = 0; j < 4; ++j) x[2 * j] = bf16_lo(w[j]), x[2 * j + 1] = bf16_hi(w[j]);
   }
 }
-// keeps a NaN, which fmaxf drops
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-
 // largest magnitude of the eight
 template <int DT>
 __device__ __forceinline__ float kv_amax8(const KvRaw<DT>& r) {

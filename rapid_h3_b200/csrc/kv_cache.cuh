@@ -31,6 +31,13 @@ struct KvRows {
   int pre_tiles;   // key tiles of a shared prefix before every unit's own
 };
 
+// keeps a NaN, which fmaxf drops
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 __device__ __forceinline__ void kv_report(int* status, int code) {
   if (status) atomicCAS(status, 0, code);
 }

@@ -87,3 +87,24 @@ def test_a_v_row_that_is_not_finite_reaches_the_rows_that_see_it(kv, prefix_path
     pv[5, 0, 0] = value
     out = outs()[2]
     assert bool(torch.isnan(out[:, :8]).all()) and torch.isfinite(out[:, 8:]).all()
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_a_k_row_that_is_not_finite_reaches_the_rows_that_see_it(kv, prefix_path, kind, dtype, value):
+    """K alone, V clean, over 2,048 rows and heads: what codes of 0 leave of a score must not decide between a NaN and a key left out."""
+    cache = kv.alloc(8, 1, 128, 16, kind)
+    rows, table, starts = batch(kv, [70], [64], 16, 8, 1)
+    whole = kv.Rows(rows.table, rows.lens, torch.tensor([0, 70], **I32))
+    k, v = (randn(s, 70, 1, 128, dtype=dtype) for s in (2, 3))
+    q = randn(4, 64, 32, 128, dtype=dtype).cuda()
+    kv.write(cache, k.cuda(), v.cuda(), whole)
+    clean = kv.attention(q, cache, rows)
+    k[33, 0, 7] = value
+    kv.write(cache, k.cuda(), v.cuda(), whole)
+    assert bool(torch.isnan(kv.attention(q, cache, rows, causal=False)).all())
+    out = kv.attention(q, cache, rows)
+    assert torch.equal(out[:27], clean[:27]) and bool(torch.isnan(out[27:]).all())
+    one = kv.Rows(rows.table, torch.zeros(1, **I32), torch.tensor([0, 64], **I32))
+    assert bool(torch.isnan(kv.attention_shared(q, cache, one, rows.table[0].contiguous(), 70)).all())
