@@ -359,7 +359,8 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      const float f = p.sl2 * down * (FMT == RH3_KIND_I8 ? 16777216.f : 1.f);
+      // a row with an infinity has no softmax, also where all that it sees would be -inf (a NaN among its values does the same by itself)
+      const float f = amax < INFINITY ? p.sl2 * down * (FMT == RH3_KIND_I8 ? 16777216.f : 1.f) : kNan;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         cf[nt][e] = __shfl_sync(0xffffffffu, f, (2 * c + e) * 4);

@@ -153,6 +153,11 @@ __device__ __forceinline__ float max_3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// two fp16, infinities as NaN
+__device__ __forceinline__ uint32_t nan_of_inf(uint32_t w) {
+  const __half2 h = *reinterpret_cast<const __half2*>(&w), y = __hfma2(h, __half2half2(__ushort_as_half(0)), h);
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
 
 // Registers: 72 a thread at launch; service 40, softmax 88, conversion 56
 static_assert(128 * 40 + 512 * 88 + 256 * 56 <= WTHREADS * 72, "the shares must not exceed the pool");
@@ -580,6 +585,8 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
 #pragma unroll
         for (int k = 0; k < N; ++k) {
           const int r = q_row + k * ROWS;
+          // x + 0 * x: an infinity becomes NaN. Its row has no softmax, also where all that it sees would be -inf.
+          x[k] = make_uint4(nan_of_inf(x[k].x), nan_of_inf(x[k].y), nan_of_inf(x[k].z), nan_of_inf(x[k].w));
           *reinterpret_cast<uint4*>(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x[k];
         }
         fence_proxy_async_smem();

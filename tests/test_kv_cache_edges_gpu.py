@@ -108,3 +108,24 @@ def test_a_k_row_that_is_not_finite_reaches_the_rows_that_see_it(kv, prefix_path
     assert torch.equal(out[:27], clean[:27]) and bool(torch.isnan(out[27:]).all())
     one = kv.Rows(rows.table, torch.zeros(1, **I32), torch.tensor([0, 64], **I32))
     assert bool(torch.isnan(kv.attention_shared(q, cache, one, rows.table[0].contiguous(), 70)).all())
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_a_query_that_is_not_finite_gives_nan_where_it_sees_a_key(kv, path, kind, dtype, value):
+    """Its scores are infinite or NaN, and so is their softmax NaN: also where all of them are -inf. Without a key the row is 0."""
+    cache = kv.alloc(6, 1, 64, 16, kind)
+    fill(cache, 1)
+    for page in (0, 1):
+        cache.k[page] = torch.full((1, 16, 64), 1.0 - 2 * page, device="cuda").to(cache.k.dtype)      # scores of one sign
+    rows = kv.Rows(torch.tensor([[0, 2], [1, 2], [2, 3], [4, 5]], **I32), torch.tensor([1, 16, 32, 0], **I32), torch.tensor([0, 1, 3, 23, 24], **I32))
+    q = randn(2, 24, 4, 64, dtype=dtype)
+    clean = kv.attention(q.cuda(), cache, rows)
+    q[::2, 1::2, 9] = value
+    out = kv.attention(q.cuda(), cache, rows)
+    bad = torch.zeros(24, 4, dtype=torch.bool)
+    bad[::2, 1::2] = True
+    assert bool((out[23] == 0).all())
+    bad[23] = False
+    assert bool(torch.isnan(out[bad.cuda()]).all()) and torch.equal(out[~bad.cuda()], clean[~bad.cuda()])
