@@ -391,7 +391,7 @@ int rh3_vae_gemm_swiglu(const void* xq, int64_t lda, const void* wq, const float
  * 128 tokens, D = 64 or 128; all four 16-byte aligned.
  * Batch: table int32 [B] rows of per_seq pages at table_stride, the pages of each sequence in order; lens int32 [B], the tokens each
  * sequence holds, the call's own among them; starts int32 [B + 1], ascending: rows starts[b] .. starts[b + 1] - 1 of the call are the last
- * tokens of sequence b. They are read on the device: a captured call follows them. Rows at or behind starts[B] (T may be larger: a padded
+ * tokens of sequence b, row t at position lens[b] - (starts[b + 1] - t). They are read on the device: a captured call follows them. Rows at or behind starts[B] (T may be larger: a padded
  * batch) are left as they were. Tokens that lie nowhere (before position 0, beyond the table, in a page outside the cache)
  * are not written, read as zeros and are masked; a page outside the cache also leaves status 120 (rh3_check_status).
  * dtype: 0 = bf16, 1 = fp16, 2 = fp32 (write and read only). Every row must start on a 16-byte boundary.

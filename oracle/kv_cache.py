@@ -31,7 +31,8 @@ def tokens(codes, scales, pages, n):
 
 
 def attention(q, cache, table, lens, starts, scale=None, causal=True, prefix=(), prefix_len=0):
-    """out fp64 [T, heads, D] of q [T, heads, D]; cache: (k, v, k_scale, v_scale); rows of no sequence are NaN."""
+    """out fp64 [T, heads, D] of q [T, heads, D]; cache: (k, v, k_scale, v_scale); rows of no sequence are NaN. Row r of sequence b is at
+    position lens[b] - (starts[b + 1] - r), whatever its table and the call have room for."""
     k, v, ks, vs = cache
     t, heads, d = q.shape
     group = heads // k.shape[1]
@@ -44,10 +45,10 @@ def attention(q, cache, table, lens, starts, scale=None, causal=True, prefix=(),
         m = max(0, min(n_all, len(table[b]) * k.shape[2]))
         kk, there = tokens(k, ks, table[b], m)
         vv, _ = tokens(v, vs, table[b], m)
-        for r in range(lo, hi):
+        for r in range(max(lo, 0), min(hi, t)):
             seen = there.clone()
             if causal:
-                seen[max(0, m - (hi - lo) + (r - lo) + 1):] = False
+                seen[max(0, n_all - (hi - r) + 1):] = False
             keys, values = torch.cat([kp[there_p], kk[seen]]), torch.cat([vp[there_p], vv[seen]])
             for h in range(heads):
                 if len(keys) == 0:

@@ -124,7 +124,7 @@ __device__ __forceinline__ KvLaneRow kv_lane_row(const KvAttnParams& p, const Kv
   const int64_t t = g.s.first + i, head = static_cast<int64_t>(g.h) * p.group + hh;
   x.q = there ? t * p.q_st + head * p.q_sh : -1;
   x.o = t * p.o_st + head * p.o_sh;
-  x.pos = p.causal ? g.s.len - g.s.n + i : g.s.len - 1;
+  x.pos = p.causal ? g.s.pos + i : g.s.len - 1;
   x.flat = (g.s.first + i) * p.group + hh;
   return x;
 }
@@ -419,7 +419,7 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
       }
     }
     const int kend = kv_last_tile<BM>(p, g);
-    const int pos_first = p.causal ? g.s.len - g.s.n + g.u * BM / p.group : g.s.len - 1;
+    const int pos_first = p.causal ? g.s.pos + g.u * BM / p.group : g.s.len - 1;
     for (int kt = g.k0; kt < kend && ok; ++kt) {
       if (!__all_sync(0xffffffffu, mbar_wait(&tail->full[stage], ph, abort_flag, p.status, ST_TIMEOUT_TMA_FULL))) {
         ok = false;

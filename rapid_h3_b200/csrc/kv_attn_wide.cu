@@ -45,7 +45,7 @@ struct KvWide {
 };
 // one unit's part of a CTA's run
 struct KvWideSegment {
-  int first, n, len;      // of the sequence
+  int first, n, len, pos; // of the sequence
   int b, h, u;            // sequence, KV head, row tile
   int k0, k1, kt;         // tiles [k0, k1) of the unit's kt
   int cta, parts;         // CTAs cta .. cta + parts - 1 have a part of the unit
@@ -175,23 +175,23 @@ __device__ __forceinline__ void kv_wide_settle() {
 // the last one for kt, so neighbouring runs meet at the same tile. Tiles behind the last visible key are no work and in nobody's run.
 constexpr int UNIT_COST = KV_WIDE_UNIT_COST;
 struct KvWideSeq {
-  int first, n, len, qt;      // first row token of the call, new tokens, cached tokens, row tiles
+  int first, n, len, pos, qt; // first row token of the call, new tokens, cached tokens, position of the first, row tiles
   int step;
   long long base, head;       // of one unit; weight of all units of a head
 };
 __device__ __forceinline__ KvWideSeq kv_wide_seq(const KvAttnParams& p, int b) {
   const KvSeq q = kv_seq<WBM, TK>(p.r, p.c.page_log2, p.group, b);
   KvWideSeq s;
-  s.first = q.first, s.n = q.n, s.len = q.len, s.qt = q.qt;
+  s.first = q.first, s.n = q.n, s.len = q.len, s.pos = q.pos, s.qt = q.qt;
   s.step = p.causal ? WBM / p.group : 0;
-  s.base = UNIT_COST + p.r.pre_tiles * TK + max(1, p.causal ? q.len - q.n + max(1, s.step) : q.len);
+  s.base = UNIT_COST + p.r.pre_tiles * TK + max(1, p.causal ? q.pos + max(1, s.step) : q.len);
   s.head = s.base * s.qt + static_cast<long long>(s.step) * s.qt * (s.qt - 1) / 2;
   return s;
 }
 // tiles that row tile u works on (one at least: rows without a key are written too)
 __device__ __forceinline__ int kv_wide_tiles(const KvAttnParams& p, const KvWideSeq& s, int u) {
   int seen = s.len;
-  if (p.causal) seen = max(0, min(s.len, s.len - s.n + (min((u + 1) * WBM, s.n * p.group) - 1) / p.group + 1));
+  if (p.causal) seen = max(0, min(s.len, s.pos + (min((u + 1) * WBM, s.n * p.group) - 1) / p.group + 1));
   return max(1, p.r.pre_tiles + (seen + TK - 1) / TK);
 }
 struct KvWideWalk {
@@ -250,7 +250,7 @@ struct KvWideWalk {
       g.k0 = tile(x - xu), g.k1 = tile(end);
       x = xu + end;
       if (g.k0 >= g.k1) continue;
-      g.first = s.first, g.n = s.n, g.len = s.len, g.b = b, g.h = h, g.u = u, g.kt = kt;
+      g.first = s.first, g.n = s.n, g.len = s.len, g.pos = s.pos, g.b = b, g.h = h, g.u = u, g.kt = kt;
       const long long full = min(w, static_cast<long long>(UNIT_COST) + static_cast<long long>(kt - 1) * TK + 1);   // from here on all tiles are dealt
       g.cta = static_cast<int>((xu + UNIT_COST) / run);
       g.parts = static_cast<int>((xu + full - 1) / run) - g.cta + 1;
@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
       }
       // of the thread's two rows: factor, the last own key that is seen, maximum (of t) and sum
       const int warp_first = (g.u * WBM + rt * 128 + quad * 32 + half * 16) / p.group;   // token of the warp's first row: it sees least
-      const int warp_last = p.causal ? g.len - g.n + warp_first : g.len - 1;
+      const int warp_last = p.causal ? g.pos + warp_first : g.len - 1;
       uint64_t c2[2];
       float m[2], l[2];
       int e = 0;   // of O as it is
@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
             top[k] = -INFINITY;
             sum[k] = pk2(0.f, 0.f);
             if constexpr (decltype(mask)::value)
-              last[k] = cut ? g.len - g.n + (g.u * WBM + rt * 128 + frag_row + 8 * k) / p.group - key0 - 2 * (lane & 3) : TK;
+              last[k] = cut ? g.pos + (g.u * WBM + rt * 128 + frag_row + 8 * k) / p.group - key0 - 2 * (lane & 3) : TK;
           }
           uint32_t r[2][8];
           float2 key[2][2];   // of the column pairs, fetched 16 columns ahead as S is

@@ -88,17 +88,20 @@ __device__ __forceinline__ int64_t kv_place(const KvCache& c, const KvRows& r, i
 // of W; more than that comes of starts that are not ascending, and nothing is done then.
 struct KvSeq {
   int first, n, len;  // first row token of the call, new tokens, cached tokens
+  int pos;            // position of the first row token, as kv_place has it (at most len: there it sees all of them)
   int qt, kt;         // row tiles, key tiles of a unit
   __device__ __forceinline__ int weight(int heads, int cost) const { return heads * qt * (kt + cost); }
 };
 template <int BM, int TK>
 __device__ __forceinline__ KvSeq kv_seq(const KvRows& r, int page_log2, int group, int b) {
   KvSeq s;
-  const int lo = r.fixed_len ? 0 : min(max(r.starts[b], 0), r.T), hi = r.fixed_len ? r.T : min(max(r.starts[b + 1], lo), r.T);
+  const int lo = r.fixed_len ? 0 : min(max(r.starts[b], 0), r.T), end = r.fixed_len ? r.T : r.starts[b + 1], held = r.fixed_len ? r.fixed_len : r.lens[b];
   s.first = lo;
-  s.n = hi - lo;
+  s.n = min(max(end, lo), r.T) - lo;
   const long long room = static_cast<long long>(r.per_seq) << page_log2;
-  s.len = static_cast<int>(min(static_cast<long long>(r.fixed_len ? r.fixed_len : max(r.lens[b], 0)), room));
+  s.len = static_cast<int>(min(static_cast<long long>(max(held, 0)), room));
+  // from lens and starts as they are, not as far as the table and the call go; below 0 by more than a call has rows is all the same
+  s.pos = static_cast<int>(max(-(1ll << 30), min(static_cast<long long>(s.len), held - (static_cast<long long>(end) - lo))));
   s.qt = (s.n * group + BM - 1) / BM;
   s.kt = max(1, r.pre_tiles + (s.len + TK - 1) / TK);
   return s;
@@ -191,7 +194,7 @@ template <int BM>
 __device__ __forceinline__ int kv_visible(const KvSeq& s, int group, int u, bool causal) {
   if (!causal) return s.len;
   const int last = (min((u + 1) * BM, s.n * group) - 1) / group;
-  return max(0, min(s.len, s.len - s.n + last + 1));
+  return max(0, min(s.len, s.pos + last + 1));
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -73,7 +73,8 @@ def alloc(pages, kv_heads, head_dim=128, page=64, kind="int8", device="cuda"):
 class Rows:
     """Which rows of a call belong to which sequence, int32 on the cache's device:
     table [B, P] the pages of each sequence in order (rows may be strided); lens [B] the tokens each sequence holds, the call's own
-    among them; starts [B + 1], ascending: rows starts[b] .. starts[b + 1] - 1 of the call are the last tokens of sequence b.
+    among them; starts [B + 1], ascending: rows starts[b] .. starts[b + 1] - 1 of the call are the last tokens of sequence b,
+    row t at position lens[b] - (starts[b + 1] - t).
 
     The values are not looked at on the host. Rows at or behind starts[B] (a padded batch) are left as they were; tokens that lie
     nowhere (before position 0, beyond the table, in a page the cache does not have) are not written, read as zeros and are

@@ -129,3 +129,42 @@ def test_a_query_that_is_not_finite_gives_nan_where_it_sees_a_key(kv, path, kind
     assert bool((out[23] == 0).all())
     bad[23] = False
     assert bool(torch.isnan(out[bad.cuda()]).all()) and torch.equal(out[~bad.cuda()], clean[~bad.cuda()])
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("group", [3, 16])
+def test_a_row_is_at_the_position_that_write_gave_it(kv, prefix_path, kind, group):
+    """Lengths beyond the table, more rows named than the call has, rows named before the call's first: positions are lens - (starts[b + 1] - t) for
+    every operator, and causal attention sees what lies up to there."""
+    cache = kv.alloc(26, 2, 64, 16, kind)
+    fill(cache, 1)
+    q = randn(2, 30, 2 * group, 64).cuda()
+    pre = torch.tensor([25, 24], **I32)
+    for table, lens, starts in (
+        ([[3, 7, 1, 9]], [70], [0, 10]),                                   # 64 tokens of room, positions 60 to 69
+        ([[3, 7, 1, 9]], [1 << 30], [0, 30]),                              # all behind the room: a row sees all of it
+        ([[3, 7, 1, 9]], [64], [0, 45]),                                   # the call has 30 rows: positions 19 to 48
+        ([[3, 7, 1, 9], [2, 4, 6, 8]], [64, 50], [-20, 7, 100]),           # 20 rows before the call's first; 70 behind its last
+        ([[3, 7, 1, 9], [2, 4, 6, 8], [10, 11, 12, 13]], [66, 20, 61], [0, 5, 28, 45]),   # the second has more rows than tokens
+        ([[3, 7], [2, 4]], [-2147483648, 2147483647], [0, 15, 2147483647]),               # 32-bit ends
+    ):
+        rows = kv.Rows(torch.tensor(table, **I32), torch.tensor(lens, **I32), torch.tensor(starts, **I32))
+        for causal in (True, False):
+            check(kv.attention(q, cache, rows, causal=causal), q, cache, table, lens, starts, causal=causal)
+        check(kv.attention_shared(q, cache, rows, pre, 19), q, cache, table, lens, starts, prefix=[25, 24], prefix_len=19)
+
+
+def test_a_token_finds_itself(kv, path):
+    """Rows written, and then attended to by queries that single out their own token, where the length is beyond the table."""
+    cache = kv.alloc(4, 1, 64, 16, "int8")
+    rows = kv.Rows(torch.tensor([[2, 0, 3, 1]], **I32), torch.tensor([70], **I32), torch.tensor([0, 26], **I32))
+    at = torch.arange(26) + 44                                             # positions; the last six are beyond the table
+    k = torch.zeros(26, 1, 64, dtype=torch.bfloat16)
+    k[torch.arange(26), 0, torch.arange(26)] = 1
+    v = randn(3, 26, 1, 64)
+    kv.write(cache, k.cuda(), v.cuda(), rows)
+    out = kv.attention((k * 1000).cuda(), cache, rows)
+    back = kv.read(cache, rows, 26)[1]
+    # other tokens' weights are e^-125; out and back are each rounded to bf16 (2^-8 of the value), out from V in fp16 (2^-11), whose sum is below 2^-6
+    assert bool(((out - back).float().abs() <= 2**-6 * back.float().abs())[at < 64].all())
+    assert bool((back[at >= 64] == 0).all())
