@@ -394,6 +394,8 @@ int rh3_vae_gemm_swiglu(const void* xq, int64_t lda, const void* wq, const float
  * tokens of sequence b, row t at position lens[b] - (starts[b + 1] - t). They are read on the device: a captured call follows them. Rows at or behind starts[B] (T may be larger: a padded
  * batch) are left as they were. Tokens that lie nowhere (before position 0, beyond the table, in a page outside the cache)
  * are not written, read as zeros and are masked; a page outside the cache also leaves status 120 (rh3_check_status).
+ * Where starts do not ascend rh3_kv_attn computes nothing and leaves status 121; rh3_kv_write and rh3_kv_read, which look for a row's sequence
+ * by halves, take some rows for those of another sequence, or of none.
  * dtype: 0 = bf16, 1 = fp16, 2 = fp32 (write and read only). Every row must start on a 16-byte boundary.
  *
  * rh3_kv_write: s = max(amax / (127 | 448), 1e-12), codes round-to-nearest-even of x / s. A row with a NaN or an infinity keeps it in its

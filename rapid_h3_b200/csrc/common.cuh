@@ -31,7 +31,7 @@ enum : int {
   ST_TIMEOUT_P_READY = 105,     // attention: MMA issuer waited too long for P
   ST_TIMEOUT_PV_DONE = 106,     // attention: softmax waited too long for P.V
   ST_KV_BAD_PAGE = 120,         // cache operators: the page table named a page that does not exist (its tokens count as masked)
-  ST_KV_BAD_STARTS = 121,       // cache operators: the row starts of a batch are not ascending (nothing is computed)
+  ST_KV_BAD_STARTS = 121,       // cache attention: the row starts of a batch are not ascending (nothing is computed)
   ST_TIMEOUT_SELFTEST = 190,    // rh3_selftest_wait_expiry: the wait that is meant to run out did
 };
 

@@ -245,7 +245,7 @@ kv_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant_
   }
   __syncthreads();
   grid_dependency_begin();
-  const KvRun run = kv_find_run<BM, TK>(p.r, p.c.page_log2, p.c.heads, p.group, p.cost, p.most, p.status);
+  const KvRun run = kv_find_run<BM, TK>(p.r, p.c.page_log2, p.c.heads, p.group, p.cost, p.status);
   KvWalk<BM, TK> walk(run);
   KvSegment g;
 
@@ -842,7 +842,6 @@ extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t w
   p.status = device_status_word();
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.count = counters;
-  p.most = static_cast<int>(x.own.w);
   p.cost = x.own.cost;
   p.part = reinterpret_cast<float*>(ws + x.part);
   if (x.one) {
@@ -878,7 +877,6 @@ extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t w
   q.r = KvRows{a->prefix_table, nullptr, nullptr, a->prefix_pages, 1, static_cast<int>(a->prefix_pages), static_cast<int>(a->T),
                static_cast<int>(a->prefix), 0};
   q.causal = 0;
-  q.most = static_cast<int>(x.pre.w);
   q.cost = x.pre.cost;
   if (int e = x.pre.nt == 0 ? kv_wide_launch(q, a->D, a->kind, true, x.pre.grid, stream) : launch(std::integral_constant<int, MODE_PREFIX>(), q, x.pre)) return e;
   return launch(std::integral_constant<int, MODE_OWN>(), p, x.own);

@@ -27,7 +27,6 @@ struct KvAttnParams {
   int group;          // query heads per KV head
   int causal;
   int cost;           // what a unit weighs besides its tiles
-  int most;           // bound of the weight of the pass
   float sl2;          // softmax scale * log2 e
   int* status;
   // partial results of units that more than one CTA works on: two slots per CTA (0: of the unit its run begins inside of, 1: of the unit

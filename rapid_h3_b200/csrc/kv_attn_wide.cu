@@ -203,7 +203,15 @@ struct KvWideWalk {
     const int lane = threadIdx.x & 31, per = (p.r.B + 31) >> 5;
     const int b0 = min(p.r.B, lane * per), b1 = min(p.r.B, b0 + per);
     long long own = 0;
-    for (int i = b0; i < b1; ++i) own += p.c.heads * kv_wide_seq(p, i).head;
+    bool bad = false;
+    for (int i = b0; i < b1; ++i) {
+      own += p.c.heads * kv_wide_seq(p, i).head;
+      bad |= kv_descends(p.r, i);
+    }
+    if (__any_sync(0xffffffffu, bad)) {   // as kv_find_run
+      own = 0;
+      if (lane == 0) kv_report(p.status, ST_KV_BAD_STARTS);
+    }
     long long incl = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {

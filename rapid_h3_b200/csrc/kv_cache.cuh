@@ -84,13 +84,13 @@ __device__ __forceinline__ int64_t kv_place(const KvCache& c, const KvRows& r, i
 // BM such rows of one sequence and KV head against all of its keys, in tiles of TK keys; every unit has at least one tile, so that rows
 // without a key are written too. A unit weighs its tiles and `cost` more, for what it takes to begin and end it. All units, in the order
 // (sequence, head, row tile), are dealt to the CTAs in runs of `run` = W / grid, rounded up: a run begins and ends anywhere inside a unit,
-// where position y stands for key tile y - cost (0 up to there). The entry knows a bound `most` below 2^31
-// of W; more than that comes of starts that are not ascending, and nothing is done then.
+// where position y stands for key tile y - cost (0 up to there). W is below 2^31 (the entry refuses more) for starts that ascend;
+// where they do not, sequences would claim the same rows: that is reported, and nothing is done.
 struct KvSeq {
   int first, n, len;  // first row token of the call, new tokens, cached tokens
   int pos;            // position of the first row token, as kv_place has it (at most len: there it sees all of them)
   int qt, kt;         // row tiles, key tiles of a unit
-  __device__ __forceinline__ int weight(int heads, int cost) const { return heads * qt * (kt + cost); }
+  __device__ __forceinline__ unsigned weight(int heads, int cost) const { return static_cast<unsigned>(heads) * qt * (kt + cost); }
 };
 template <int BM, int TK>
 __device__ __forceinline__ KvSeq kv_seq(const KvRows& r, int page_log2, int group, int b) {
@@ -106,6 +106,7 @@ __device__ __forceinline__ KvSeq kv_seq(const KvRows& r, int page_log2, int grou
   s.kt = max(1, r.pre_tiles + (s.len + TK - 1) / TK);
   return s;
 }
+__device__ __forceinline__ bool kv_descends(const KvRows& r, int b) { return !r.fixed_len && r.starts[b] > r.starts[b + 1]; }
 struct KvRun {
   int x0, x1;   // the CTA's run
   int run;      // length of a run: x belongs to CTA x / run
@@ -113,38 +114,36 @@ struct KvRun {
 };
 // Every warp scans the sequences by itself (they are in L1 after the first): no barrier, one round of loads up to 32 sequences.
 template <int BM, int TK>
-__device__ __forceinline__ KvRun kv_find_run(const KvRows& r, int page_log2, int heads, int group, int cost, int most, int* status) {
+__device__ __forceinline__ KvRun kv_find_run(const KvRows& r, int page_log2, int heads, int group, int cost, int* status) {
   const int lane = threadIdx.x & 31;
   const int per = (r.B + 31) >> 5;
   const int b0 = min(r.B, lane * per), b1 = min(r.B, b0 + per);
-  long long sum = 0;
+  unsigned own = 0;
+  bool bad = false;
   for (int b = b0; b < b1; ++b) {
-    const KvSeq s = kv_seq<BM, TK>(r, page_log2, group, b);
-    sum += static_cast<long long>(heads) * s.qt * (s.kt + cost);
+    own += kv_seq<BM, TK>(r, page_log2, group, b).weight(heads, cost);
+    bad |= kv_descends(r, b);
   }
-  int own = static_cast<int>(min(sum, static_cast<long long>(most) + 1));
-  if (__any_sync(0xffffffffu, own > most)) own = lane == 0 ? most + 1 : 0;
-  long long total = own;
+  if (__any_sync(0xffffffffu, bad)) {
+    own = 0;
+    if (threadIdx.x == 0) kv_report(status, ST_KV_BAD_STARTS);
+  }
+  unsigned total = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, total, o);
+    const unsigned up = __shfl_up_sync(0xffffffffu, total, o);
     if (lane >= o) total += up;
   }
-  const long long all = __shfl_sync(0xffffffffu, total, 31);
-  if (all > most) {
-    if (threadIdx.x == 0) kv_report(status, ST_KV_BAD_STARTS);
-    own = 0, total = 0;
-  }
-  const int incl = static_cast<int>(total), W = all > most ? 0 : static_cast<int>(all);
+  const int incl = static_cast<int>(total), W = __shfl_sync(0xffffffffu, incl, 31);
   KvRun run;
   run.run = max(1u, (static_cast<unsigned>(W) + gridDim.x - 1) / gridDim.x);
   run.x0 = static_cast<int>(min(static_cast<long long>(W), static_cast<long long>(run.run) * blockIdx.x));
   run.x1 = min(W - run.x0, run.run) + run.x0;
-  int xb = incl - own, b = b0;
+  int xb = incl - static_cast<int>(own), b = b0;
   const bool mine = run.x0 < run.x1 && xb <= run.x0 && run.x0 < incl;
   if (mine && per > 1) {
     for (; b < b1; ++b) {
-      const int w = kv_seq<BM, TK>(r, page_log2, group, b).weight(heads, cost);
+      const int w = static_cast<int>(kv_seq<BM, TK>(r, page_log2, group, b).weight(heads, cost));
       if (run.x0 - xb < w) break;
       xb += w;
     }
@@ -171,7 +170,7 @@ struct KvWalk {
   __device__ __forceinline__ bool next(const KvRows& r, int page_log2, int heads, int group, int cost, KvSegment& g) {
     while (x < x1) {
       if (!have) s = kv_seq<BM, TK>(r, page_log2, group, b), have = true;
-      while (x - xb >= s.weight(heads, cost)) {  // ends: the sequences from b on reach beyond x < x1 <= W
+      while (x - xb >= static_cast<int>(s.weight(heads, cost))) {  // ends: the sequences from b on reach beyond x < x1 <= W
         if (b + 1 >= r.B) return false;
         xb += s.weight(heads, cost);
         s = kv_seq<BM, TK>(r, page_log2, group, ++b);

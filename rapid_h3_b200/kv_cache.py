@@ -78,7 +78,8 @@ class Rows:
 
     The values are not looked at on the host. Rows at or behind starts[B] (a padded batch) are left as they were; tokens that lie
     nowhere (before position 0, beyond the table, in a page the cache does not have) are not written, read as zeros and are
-    masked, and a page the cache does not have is reported by `_lib.check_status()`."""
+    masked, and a page the cache does not have is reported by `_lib.check_status()`. So are starts that do not ascend, by attention, which
+    then computes nothing; which rows write and read take for a sequence's is open then."""
     table: torch.Tensor
     lens: torch.Tensor
     starts: torch.Tensor

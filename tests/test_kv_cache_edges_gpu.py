@@ -168,3 +168,27 @@ def test_a_token_finds_itself(kv, path):
     # other tokens' weights are e^-125; out and back are each rounded to bf16 (2^-8 of the value), out from V in fp16 (2^-11), whose sum is below 2^-6
     assert bool(((out - back).float().abs() <= 2**-6 * back.float().abs())[at < 64].all())
     assert bool((back[at >= 64] == 0).all())
+
+
+@pytest.mark.parametrize("lens,starts", [
+    ([160, 3, 160, 9], [0, 9, 2, 9, 1]), ([160, 3, 160, 9], [0, 5, 5, 4, 9]), ([160, 3, 160, 9], [3, 2, 5, 8, 9]), ([7] * 70, [0] * 60 + [9, 8] + [9] * 9),
+])
+@pytest.mark.parametrize("d", [64, 128])
+def test_starts_that_do_not_ascend_are_reported_and_nothing_is_computed(kv, prefix_path, lens, starts, d):
+    from rapid_h3_b200 import _lib
+    cache = kv.alloc(40, 2, d, 16, "int8")
+    fill(cache, 1)
+    rows = kv.Rows(torch.arange(40, **I32).repeat(18)[:10 * len(lens)].view(len(lens), 10), torch.tensor(lens, **I32), torch.tensor(starts, **I32))
+    q = randn(2, 9, 8, d).cuda()
+    pre = torch.arange(30, **I32)
+    good = kv.Rows(rows.table, rows.lens, torch.tensor([0] * len(lens) + [9], **I32))
+    for call, kw in ((lambda r, out: kv.attention(q, cache, r, out=out), {}),
+                     (lambda r, out: kv.attention_shared(q, cache, r, pre, 470, out=out), dict(prefix=pre.tolist(), prefix_len=470))):
+        out = torch.full_like(q, 5.0)
+        call(rows, out)
+        with pytest.raises(RuntimeError, match="ascending"):
+            _lib.check_status()
+        assert bool((out == 5).all())
+        call(good, out)                                                    # the next call is as any
+        _lib.check_status()
+        check(out, q, cache, rows.table.tolist(), lens, good.starts.tolist(), **kw)
