@@ -6,13 +6,17 @@
 // prefix a unit's keys are the prefix's tiles and then its own (or, in the prefix's own pass, the prefix's alone).
 //
 //   S_g = Q_g . K^T        fp16 x fp16 -> fp32 in TMEM (tcgen05 kind::f16), K the codes as fp16, exactly
-//   t = (s * ks_j) * c_row,  w = 2^(t - m + 3),  l += w
-//   O_g += W_g . V         W fp16 from TMEM (over S), V = fp16(code * vs_j * 2^-e); fp32 in TMEM;  o = O / l * 2^e
-// m is a row's maximum when it was last set: it is set anew, and O and l scaled, only when the maximum outgrows it by 2^12, so W stays
-// at most 2^15 and O is hardly ever touched between products (2,011 tokens behind 16,000: 632 us where it might outgrow it by 2^8, 618 by 2^12). e is the exponent of the largest V scale so far: V's one rounding
-// is 2^-11 of a value (2^-25 of the largest row's magnitude for what is smaller than 2^-14 of it), as much as that of the
-// weights. (In the exponent, as in kv_attn.cu, the V scales cost a softmax thread two more floats a key and two more operations a
-// score.) A key with a scale that is not finite has V = 0 and a K scale that is not a number: only the rows that see it become NaN.
+//   u = (s * ks_j) * c_row + e_j,  w = 2^(u - m + 3),  l += w * 2^-e_j
+//   O_g += W_g . V         W fp16 from TMEM (over S), V = fp16(code * vs_j * 2^-e_j); fp32 in TMEM;  o = O / l
+// m is a row's maximum of u, rounded down, when it was last set: it is set anew, and O and l scaled, only when the maximum outgrows it by 2^12, so W
+// stays at most 2^15 and O is hardly ever touched between products (2,011 tokens behind 16,000: 632 us where it might outgrow it by 2^8, 618 by 2^12).
+// e_j is an exponent of the key's V scale. The keys of a tile share it where their scales lie within 2^7 of one another: it is then added to m once.
+// Else each has its own (as in kv_attn.cu, where the whole scale goes into the exponent), so a large V row takes no bits from others, least of
+// all where it is not seen. That costs a softmax thread four more floats a key and two more operations a score: the 2,011 tokens behind 16,000
+// take 870 us where every tile is such a one, 654 with one in eight or so, 610 with none. V's one rounding
+// is 2^-11 of a value, as much as that of the weights. Weights below 2^-14 lose bits, 2^-25 at most: that is 2^-28 of the row's largest
+// weight times the 2^7 that V scales may differ by. l holds what keys of small V scales weigh: scales of a row may differ by 2^120.
+// A key with a scale that is not finite has V = 0 and a K scale that is not a number: only the rows that see it become NaN.
 //
 // 896 threads, one CTA per SM: warp 0 brings pages by bulk copies (codes as they lie), warp 1 issues the products, warp 2 works out the run's segments and tells
 // the others, warps 4-19 are the softmax, eight
@@ -52,14 +56,16 @@ struct KvWideSegment {
 };
 struct __align__(16) KvWideTail {
   float scale[RAW][2][TK];        // as loaded with a K tile: of K, of V
-  float key[2][TK];               // per key of a tile, by the tile's parity: K scale (-inf: no such key)
-  float value[2][TK];             // and V scale * 2^-e
+  float key[2][TK];               // per key of a tile, by the tile's parity: K scale (-inf: no such key),
+  float value[2][TK];             // V scale * 2^-e,
+  float shift[2][TK];             // and where keys have exponents of their own, e
+  float down[2][TK];              // and 2^-e
   float row[2][2][2][128];        // per row of a row tile: factor c, then l; m; two units' in turn
   uint64_t raw_full[2 * RAW];     // two for a raw tile: for when it holds K, and V, each waited for by its own warps alone
   uint64_t raw_empty[RAW], full[SLOTS], empty[SLOTS], value_full[2];
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2], seg_full[SEGS], seg_empty[SEGS];
-  float top[2][4];                // largest V scale of a warp's keys
-  int exponent[2], whole[2];      // e, and whether all of the tile's keys are there, by the tile's parity
+  alignas(16) uint32_t top[2][4], low[2][4];  // largest and smallest V scale above 0 of a warp's keys (bits)
+  float4 tile[2];                 // by the tile's parity: e, 2^-e, not 0 where all of its keys are there, not 0 where they share e
   uint32_t pages[RAW];
   uint32_t tmem_base;
   int abort_flag;
@@ -163,6 +169,10 @@ __device__ __forceinline__ uint32_t nan_of_inf(uint32_t w) {
 static_assert(128 * 40 + 512 * 88 + 256 * 56 <= WTHREADS * 72, "the shares must not exceed the pool");
 
 constexpr float kSlack = 12.f;   // log2 of how far a row's maximum may outgrow m
+constexpr int kAlike = 7;        // V scales of a tile within 2^7 of one another share an exponent: scale * 2^-e is then in [1, 2^7)
+// e of a V scale above 0, from its bits: 2^(e + 6) <= scale < 2^(e + 7). Below 2^-61 it is held at -67: V's precision falls then, and below 2^-91 it is 0
+// (a scale that was written is at least 2^-40).
+__device__ __forceinline__ int value_exponent(uint32_t bits) { return max(-67, static_cast<int>(bits >> 23) - 133); }
 
 // after an abandoned wait: copies that are still on their way land before the CTA gives its shared memory back
 __device__ __forceinline__ void kv_wide_settle() {
@@ -456,7 +466,6 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
       if (!more) break;
       const KvWideSegment g = tail->seg[seg % SEGS];
       release(seg);
-      int e = -60;   // exponent of the unit's V; scales below 2^-60 count as 0
       for (int kt = g.k0; kt < g.k1; ++kt, i += 2, ++tiles) {
         const KvTile t = kv_wide_tile(p, g, kt);
         const int parity = tiles & 1;
@@ -474,17 +483,23 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
           const bool is = there(tid);
           float ks = tail->scale[s][0][tid], vs = is ? tail->scale[s][1][tid] : 0.f;
           if (!(max_nan(ks, vs) < INFINITY)) vs = 0.f, ks = kNan;
-          const float top = warp_max(vs);
-          if (lane == 0) tail->top[parity][warp & 3] = top;
+          if (!(vs > 0.f)) vs = 0.f;
+          const uint32_t bits = __float_as_uint(vs), most = __reduce_max_sync(0xffffffffu, bits), least = __reduce_min_sync(0xffffffffu, vs > 0.f ? bits : 0x7F7FFFFFu);
+          if (lane == 0) tail->top[parity][warp & 3] = most, tail->low[parity][warp & 3] = least;
           if (bar_sync_or(5, 128, !ok)) {
             ok = false;
             break;
           }
-          const float most = fmaxf(fmaxf(tail->top[parity][0], tail->top[parity][1]), fmaxf(tail->top[parity][2], tail->top[parity][3]));
-          e = min(126, max(e, static_cast<int>(__float_as_uint(most) >> 23) - 126));   // most < 2^e (4 at the very top)
+          const uint4 top = *reinterpret_cast<const uint4*>(tail->top[parity]), low = *reinterpret_cast<const uint4*>(tail->low[parity]);
+          const int e_top = value_exponent(max(max(top.x, top.y), max(top.z, top.w))), e_low = value_exponent(min(min(low.x, low.y), min(low.z, low.w)));
+          const bool alike = e_top - e_low < kAlike;
+          const int e = alike ? e_top : value_exponent(bits);
+          const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
           tail->key[parity][tid] = is ? ks : -INFINITY;
-          tail->value[parity][tid] = vs * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-          if (tid == 0) tail->exponent[parity] = e, tail->whole[parity] = whole;
+          tail->value[parity][tid] = vs * down;
+          const float shift = static_cast<float>(e);
+          if (!alike) tail->shift[parity][tid] = shift, tail->down[parity][tid] = down;
+          if (tid == 0) tail->tile[parity] = make_float4(shift, down, whole, alike);
           __syncwarp();
           if (lane == 0) mbar_arrive(&tail->value_full[parity]);
         }
@@ -606,7 +621,6 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
       const int warp_last = p.causal ? g.pos + warp_first : g.len - 1;
       uint64_t c2[2];
       float m[2], l[2];
-      int e = 0;   // of O as it is
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const float c = row_of[0][frag_row + 8 * k];
@@ -619,21 +633,25 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
         if (!ok) break;
         tc_fence_after();
         const float* ks = &tail->key[parity][2 * (lane & 3)];
-        const int e_new = tail->exponent[parity];
+        const float4 tile = tail->tile[parity];
+        const float e = tile.x;
         const int key0 = (g.k0 + j - p.r.pre_tiles) * TK;
         const bool cut = !PREFIX && p.causal && key0 >= 0 && key0 + TK - 1 > warp_last;   // the prefix is seen by all
-        const bool masked = cut || !tail->whole[parity];
+        const bool alike = tile.w != 0.f, masked = cut || tile.z == 0.f || !alike;
         uint32_t w[32];
         uint64_t sum[2];
         float top[2];
-        // One pass over the rows, 16 columns at a time: s * ks, its maximum, weights against the maximum as it was set before, their sum.
-        auto pass = [&](auto mask) {
+        // One pass over the rows, 16 columns at a time: s * ks, its maximum, weights against the maximum as it was set before, their sum
+        // (without V's exponent).
+        auto pass = [&](auto mask, auto own) {
           uint64_t z2[2];
+          float z[2];
           int last[2] = {0, 0};
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const float z = (kWeightLog2 - kSlack) - (m[k] == -INFINITY ? 0.f : m[k]);
-            z2[k] = pk2(z, z);
+            z[k] = (kWeightLog2 - kSlack) - (m[k] == -INFINITY ? 0.f : m[k]);
+            if constexpr (!decltype(own)::value) z[k] += e;
+            z2[k] = pk2(z[k], z[k]);
             top[k] = -INFINITY;
             sum[k] = pk2(0.f, 0.f);
             if constexpr (decltype(mask)::value)
@@ -655,6 +673,11 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
             for (int b = 0; b < 2; ++b) {
               const int col = c * 16 + b * 8;
               const float2 a = key[c & 1][b];
+              float2 shift, down;
+              if constexpr (decltype(own)::value) {
+                shift = *reinterpret_cast<const float2*>(&tail->shift[parity][2 * (lane & 3) + col]);
+                down = *reinterpret_cast<const float2*>(&tail->down[parity][2 * (lane & 3) + col]);
+              }
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
                 const uint32_t* s = r[c & 1] + 4 * b + 2 * k;
@@ -666,10 +689,17 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
                   if (a.y == -INFINITY || col + 1 > last[k]) u1 = -INFINITY;
                   x = pk2(u0, u1);
                 }
-                top[k] = max_3(top[k], u0, u1);
-                upk2(fma_2(x, c2[k], z2[k]), u0, u1);
-                u0 = kv_ex2(u0), u1 = kv_ex2(u1);
-                sum[k] = add_2(sum[k], pk2(u0, u1));
+                if constexpr (decltype(own)::value) {
+                  upk2(add_2(fma_2(x, c2[k], z2[k]), pk2(shift.x, shift.y)), u0, u1);
+                  top[k] = max_3(top[k], u0, u1);
+                  u0 = kv_ex2(u0), u1 = kv_ex2(u1);
+                  sum[k] = fma_2(pk2(u0, u1), pk2(down.x, down.y), sum[k]);
+                } else {
+                  top[k] = max_3(top[k], u0, u1);
+                  upk2(fma_2(x, c2[k], z2[k]), u0, u1);
+                  u0 = kv_ex2(u0), u1 = kv_ex2(u1);
+                  sum[k] = add_2(sum[k], pk2(u0, u1));
+                }
                 w[(c * 2 + b) * 2 + k] = pack_half2(u0, u1);
               }
             }
@@ -678,7 +708,8 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
           for (int k = 0; k < 2; ++k) {
             float c, same;
             upk2(c2[k], c, same);
-            top[k] *= c;
+            if constexpr (decltype(own)::value) top[k] -= z[k];
+            else top[k] = fmaf(top[k], c, e);
           }
         };
         if (j == 0) {   // m to begin with: the maximum of the first 16 columns mostly within 2^12 of that of all
@@ -694,35 +725,34 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
                             fmaxf(__uint_as_float(r[4 + 2 * k]) * b.x, __uint_as_float(r[5 + 2 * k]) * b.y)) * c;
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-            m[k] = masked || !(fabsf(t) < INFINITY) ? -INFINITY : t;
+            m[k] = masked || !(fabsf(t) < INFINITY) ? -INFINITY : floorf(t) + e;
           }
-          e = e_new;
         }
         auto either = [&] {
-          if (masked) pass(std::true_type());
-          else pass(std::false_type());
+          if (!masked) pass(std::false_type(), std::false_type());
+          else if (alike) pass(std::true_type(), std::false_type());
+          else pass(std::true_type(), std::true_type());
         };
         either();
-        bool grew = e_new != e;
+        bool grew = false;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) grew |= top[k] > m[k] + kSlack || (m[k] == -INFINITY && top[k] > m[k]);
+        for (int k = 0; k < 2; ++k) grew |= top[k] > m[k] + kSlack;
         if (__any_sync(0xffffffffu, grew)) {
-          // a maximum outgrew m, or V's exponent changed: m is set anew, O and l are scaled (the product before is done: its commit lies
-          // before s_full's), and the weights made again
+          // a maximum outgrew m: m is set anew, O and l are scaled (the product before is done: its commit lies before s_full's), and the
+          // weights made again
           float f[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             float x = top[k];
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-            const bool set = x > m[k] + kSlack || (m[k] == -INFINITY && x > m[k]);
+            const bool set = x > m[k] + kSlack;
+            x = floorf(x);
             f[k] = set ? kv_ex2(m[k] - x) : 1.f;
             l[k] *= f[k];
             if (set) m[k] = x;
           }
           if (j > 0) {
-            const float down = kv_ex2(static_cast<float>(e - e_new));
-            f[0] *= down, f[1] *= down;
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
               uint32_t o[8];
@@ -733,14 +763,13 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
               tmem_st_frag2(o_base + half_off + c * 16, o);
             }
           }
-          e = e_new;
           either();
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           float even, odd;
           upk2(sum[k], even, odd);
-          l[k] += even + odd;
+          l[k] = fmaf(even + odd, alike ? tile.y : 1.f, l[k]);
         }
         tmem_st_frag16(s_frag, w);
         tmem_st_wait();
@@ -780,7 +809,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
       const bool part = !PREFIX && g.parts > 1;
       if (PREFIX || part) {
         // as the narrow kernel means it: weights 2^(t + log2 vs - m + 15) for the codes, their sum against vs
-        const float m_out = m_row + kSlack + static_cast<float>(e), l_out = l_row * kv_ex2(static_cast<float>(-e));
+        const float m_out = m_row + kSlack, l_out = l_row;
         float* dst;   // of the prefix's rows; a partial result is [D / 4][256 rows] float4, so that lanes write, and a join reads, side by side
         if (PREFIX) {
           const int64_t at = (static_cast<int64_t>(blockIdx.x - g.cta) * p.c.heads + g.h) * p.r.T * p.group + flat;
@@ -807,7 +836,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv_wide_kernel(const KvAttnParams
         }
         if (part && warp == 4 && lane == 0) tail->join[g.k0 > 0 ? 0 : 1] = g, tail->parts[g.k0 > 0 ? 0 : 1] = g.parts;
       } else {
-        const float inv = l_row == 0.f ? 0.f : __fdiv_rn(kv_ex2(static_cast<float>(e)), l_row);   // no key: 0
+        const float inv = l_row == 0.f ? 0.f : __fdiv_rn(1.f, l_row);   // no key: 0
         uint16_t* dst = p.out + t * p.o_st + head * p.o_sh + half * (D / 2);
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {

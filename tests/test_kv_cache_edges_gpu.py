@@ -192,3 +192,58 @@ def test_starts_that_do_not_ascend_are_reported_and_nothing_is_computed(kv, pref
         call(good, out)                                                    # the next call is as any
         _lib.check_status()
         check(out, q, cache, rows.table.tolist(), lens, good.starts.tolist(), **kw)
+
+
+@pytest.mark.parametrize("kind,dtype,d", [("int8", torch.bfloat16, 128), ("fp8", torch.bfloat16, 64), ("fp8", torch.float16, 128), ("int8", torch.float16, 64)])
+@pytest.mark.parametrize("size", [12, 40, 90])
+def test_a_large_v_row_costs_other_rows_nothing(kv, prefix_path, kind, dtype, d, size):
+    """V rows 2^size times the others, at the beginning, inside and at the end of key tiles: rows that come before them, and rows that give
+    them next to no weight, are as exact as without."""
+    n, page = 420, 64
+    cache = kv.alloc(10, 1, d, page, kind)
+    rows, table, starts = batch(kv, [n], [n], page, 8, 1)
+    k, v = (randn(s, n, 1, d).float() for s in (2, 3))
+    k[:, :, :2] = 0
+    big = [70, 127, 128, 200, 201, 419]
+    v[big] *= 2.0 ** size
+    k[big, :, 0] = 4.0                                    # found through two channels of q
+    kv.write(cache, k.cuda(), v.cuda(), rows)
+    q = randn(4, n, 4, d).float() * 0.3
+    # the large rows' weights: 2^-(size + 20) and more (all that they add stays below fp16's largest)
+    q[..., 0] = -0.7 * d ** 0.5 * (size + 20) / 4 * torch.tensor([1.0, 1.0, 0.9, 0.5 if dtype == torch.bfloat16 else 0.9])
+    q = q.to(dtype).cuda()
+    check(kv.attention(q, cache, rows), q, cache, table, [n], starts)
+    pick = torch.tensor([0, 69, 70, 130, 300, 419])
+    for r in pick.tolist():                               # single rows, and behind a prefix that holds large rows
+        one = kv.Rows(rows.table, torch.tensor([r + 1], **I32), torch.tensor([0, 1], **I32))
+        x = q[r:r + 1].contiguous()
+        check(kv.attention(x, cache, one), x, cache, table, [r + 1], [0, 1])
+    own = kv.Rows(torch.tensor([[8, 9]], **I32), torch.tensor([90], **I32), torch.tensor([0, 60], **I32))
+    kv.write(cache, k[100:190].cuda(), (v[100:190] * 2.0**-5).cuda(), kv.Rows(own.table, own.lens, torch.tensor([0, 90], **I32)))
+    x = q[-60:].contiguous()
+    check(kv.attention_shared(x, cache, own, rows.table[0].contiguous(), n), x, cache, [[8, 9]], [90], [0, 60], prefix=table[0], prefix_len=n)
+
+
+def test_v_scales_that_grow_and_fall_from_tile_to_tile(kv, path):
+    """Every V row has a size of its own, over 2^60; and tiles whose rows are alike within 2^8, each tile of another size."""
+    for seed, per_row in ((1, True), (2, False)):
+        cache = kv.alloc(12, 2, 128, 64, "int8")
+        fill(cache, seed)
+        rows, table, starts = batch(kv, [700, 50], [90, 50], 64, 12, seed)
+        g = torch.Generator().manual_seed(seed)
+        e = torch.randint(-30, 31, (12, 2, 64), generator=g) if per_row else torch.randint(-30, 31, (12, 1, 1), generator=g) + torch.randint(-4, 5, (12, 2, 64), generator=g)
+        cache.v_scale *= torch.exp2(e.float()).cuda()
+        q = randn(seed + 2, 140, 6, 128).cuda()
+        check(kv.attention(q, cache, rows), q, cache, table, [700, 50], starts)
+
+
+@pytest.mark.parametrize("step", [20, 0, -20])
+def test_k_scales_and_queries_of_very_different_size(kv, path, step):
+    """Queries of 2^step with K rows over 2^12, the softmax scale such that the scores are some tens: held to a tolerance by each row's own scores."""
+    cache = kv.alloc(8, 1, 128, 64, "int8")
+    fill(cache, 1)
+    rows, table, starts = batch(kv, [500], [40], 64, 8, 2)
+    for i, p in enumerate(table[0]):
+        cache.k_scale[p] *= 2.0 ** (i % 4 * 4 - 12)
+    q = (randn(3, 40, 4, 128) * 2.0 ** step).cuda()
+    check(kv.attention(q, cache, rows, scale=2.0 ** -step), q, cache, table, [500], starts, scale=2.0 ** -step)
