@@ -173,6 +173,18 @@ def _check_rows(x, name, cache, heads, types):
     return ptr, st, sh
 
 
+def _rows_overlap(t, heads, d, st, sh):
+    """Whether two rows of d elements of a [t, heads] grid with these strides (not negative) share an element."""
+    if t == 1 or heads == 1:
+        return t * heads > 1 and (st if heads == 1 else sh) < d
+    if sh >= d and st >= (heads - 1) * sh + d or st >= d and sh >= (t - 1) * st + d:   # rows of a token, or of a head, lie together
+        return False
+    if st < d or sh < d:
+        return True
+    # the token nearest to `far` is the one before it or the one behind
+    return any(abs(i * st - far) < d for far in range(sh, heads * sh, sh) for i in (far // st, far // st + 1) if i < t)
+
+
 def write(cache, k, v, rows):
     """Quantize k, v [T, kv_heads, head_dim] (bf16, fp16 or fp32, any token and head strides of whole 16 bytes) into the pages of
     their sequences. A row with a NaN or an infinity reads back as NaN. Sequences that share a page must not write the same token."""
@@ -219,6 +231,8 @@ def _attend(q, cache, rows, prefix, prefix_len, scale, causal, out):
         to = _check_rows(out, "out", cache, heads, (q.dtype,))
         if out.shape != q.shape:
             raise RuntimeError("out must have the shape of q")
+        if t and _rows_overlap(t, heads, d, to[1], to[2]):
+            raise RuntimeError(f"out: rows must not overlap, got strides {out.stride()}")
     if t == 0:
         return out
     group = heads // cache.kv_heads
@@ -242,7 +256,7 @@ def attention(q, cache, rows, scale=None, causal=True, out=None):
 
     heads: a multiple of the cache's kv_heads (head h reads KV head h // group). causal: a token sees the tokens up to itself (the
     last one of its sequence sees all), else every token sees all of its sequence. A token that sees nothing gives 0. The call's own
-    tokens are among what is seen: write them first. scale: 1 / sqrt(head_dim) unless given; out: a tensor like q to write to."""
+    tokens are among what is seen: write them first. scale: 1 / sqrt(head_dim) unless given; out: a tensor like q to write to, whose rows do not overlap (q itself will do)."""
     return _attend(q, cache, rows, None, 0, scale, causal, out)
 
 

@@ -247,3 +247,36 @@ def test_k_scales_and_queries_of_very_different_size(kv, path, step):
         cache.k_scale[p] *= 2.0 ** (i % 4 * 4 - 12)
     q = (randn(3, 40, 4, 128) * 2.0 ** step).cuda()
     check(kv.attention(q, cache, rows, scale=2.0 ** -step), q, cache, table, [500], starts, scale=2.0 ** -step)
+
+
+def test_an_output_whose_rows_overlap_is_refused(kv):
+    cache = kv.alloc(4, 2, 64, 16, "int8")
+    fill(cache, 1)
+    rows = kv.Rows(torch.arange(4, **I32).view(1, 4), torch.tensor([40], **I32), torch.tensor([0, 3], **I32))
+    q = randn(2, 3, 4, 64).cuda()
+    want = kv.attention(q, cache, rows)
+    flat = torch.zeros(4096, dtype=torch.bfloat16, device="cuda")
+    for strides in ((0, 64), (64, 0), (256, 32), (64, 64), (128, 64), (200, 64), (64, 128), (0, 0), (192, 384)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            kv.attention(q, cache, rows, out=flat.as_strided((3, 4, 64), (*strides, 1)))
+    for strides in ((256, 64), (64, 192), (1024, 136), (72, 216), (96, 384), (192, 256), (192, 640)):     # token or head first, gaps, woven into one another
+        out = flat.as_strided((3, 4, 64), (*strides, 1))
+        kv.attention(q, cache, rows, out=out)
+        assert torch.equal(out, want)
+    one = kv.Rows(rows.table, rows.lens, torch.tensor([0, 1], **I32))
+    kv.attention(q[:1], cache, one, out=flat.as_strided((1, 4, 64), (0, 64, 1)))       # one row only: its stride is nobody's
+
+
+def test_the_output_may_be_the_query(kv, prefix_path):
+    """Units in one CTA and cut between several, with and without a prefix."""
+    for d, lens, news in ((128, [900, 70, 3000], [40, 1, 90]), (64, [20000], [2])):
+        pages = sum(-(-n // 64) for n in lens) + 8
+        cache = kv.alloc(pages, 2, d, 64, "int8")
+        fill(cache, 1)
+        rows, table, starts = batch(kv, lens, news, 64, pages - 8, 2)
+        pre = torch.arange(pages - 8, pages, **I32)
+        q = randn(3, starts[-1], 12, d).cuda()
+        for call in (kv.attention, lambda *a, **kw: kv.attention_shared(*a, pre, 500, **kw)):
+            x = q.clone()
+            want = call(q, cache, rows)
+            assert call(x, cache, rows, out=x) is x and torch.equal(x, want)
