@@ -106,6 +106,7 @@ class Rows:
 _SCRATCH = {}
 _lib.on_failed_status.append(_SCRATCH.clear)   # a call that was given up may leave its counters at anything
 _KEPT_BYTES = 4 << 20
+_KEPT_STREAMS = 64   # so many streams have them; behind these, the ones kept for longest are dropped (their memory goes back to their stream's)
 _LAUNCH = threading.Lock()   # a call's kernels go to the stream together: another thread's would use the same workspace between them
 _NEED = {}
 
@@ -117,8 +118,11 @@ def _scratch(device, index, stream, need):
         return torch.zeros(1024, device=device, dtype=torch.int32), torch.empty(need, device=device, dtype=torch.uint8)
     kept = _SCRATCH.get((index, stream))
     if kept is None:
-        kept = _SCRATCH.setdefault((index, stream), (torch.zeros(1024, device=device, dtype=torch.int32),
-                                                     torch.empty(_KEPT_BYTES, device=device, dtype=torch.uint8)))
+        kept = torch.zeros(1024, device=device, dtype=torch.int32), torch.empty(_KEPT_BYTES, device=device, dtype=torch.uint8)
+        with _LAUNCH:
+            kept = _SCRATCH.setdefault((index, stream), kept)
+            while len(_SCRATCH) > _KEPT_STREAMS:
+                _SCRATCH.pop(next(iter(_SCRATCH), None), None)
     return kept if need <= _KEPT_BYTES else (kept[0], torch.empty(need, device=device, dtype=torch.uint8))
 
 

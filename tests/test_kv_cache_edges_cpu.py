@@ -2,6 +2,7 @@
 import itertools
 
 import pytest
+import torch
 
 from rapid_h3_b200 import kv_cache
 
@@ -15,3 +16,13 @@ def test_overlapping_rows_are_found(t, heads):
         assert kv_cache._rows_overlap(t, heads, d, st, sh) == overlap, (st, sh)
         found.add(overlap)
     assert found == ({False} if t == heads == 1 else {False, True})
+
+
+def test_scratch_of_many_streams_is_not_kept_for_ever(monkeypatch):
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: False, raising=False)
+    monkeypatch.setattr(kv_cache, "_SCRATCH", {})
+    made = [kv_cache._scratch("cpu", 0, stream, 100) for stream in range(200)]
+    assert len(kv_cache._SCRATCH) == kv_cache._KEPT_STREAMS
+    assert kv_cache._scratch("cpu", 0, 199, 100)[0] is made[199][0] and kv_cache._scratch("cpu", 0, 0, 100)[0] is not made[0][0]
+    big = kv_cache._scratch("cpu", 0, 199, kv_cache._KEPT_BYTES + 1)
+    assert big[0] is made[199][0] and big[1].numel() == kv_cache._KEPT_BYTES + 1
