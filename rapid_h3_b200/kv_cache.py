@@ -10,6 +10,7 @@ Keys and values are stored per token and KV head as 8-bit codes with one fp32 sc
     out = kv_cache.attention_shared(q, cache, rows, prefix, n)   # behind one prefix that all sequences share
     k, v = kv_cache.read(cache, rows, total)              # back as bf16 rows
 
+Nothing here has a backward pass: what `read` and the attentions return carries no gradient, whatever their inputs require.
 `lens`, `starts` and the page table stay on the device and are read there, so a captured call follows them. The tensors of a call are on
 the cache's device, and the work goes to that device's current stream. Everything is CUDA; there is no fallback.
 """

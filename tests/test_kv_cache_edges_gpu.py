@@ -280,3 +280,13 @@ def test_the_output_may_be_the_query(kv, prefix_path):
             x = q.clone()
             want = call(q, cache, rows)
             assert call(x, cache, rows, out=x) is x and torch.equal(x, want)
+
+
+def test_no_gradient_passes(kv):
+    """As documented: inputs may require one, outputs have none."""
+    cache = kv.alloc(2, 2, 64, 16, "int8")
+    rows = kv.Rows(torch.tensor([[0, 1]], **I32), torch.tensor([3], **I32), torch.tensor([0, 3], **I32))
+    x = randn(1, 3, 2, 64).cuda().requires_grad_()
+    kv.write(cache, x, x, rows)
+    outs = [*kv.read(cache, rows, 3), kv.attention(x, cache, rows), kv.attention_shared(x, cache, rows, rows.table[0], 2)]
+    assert not any(o.requires_grad or o.grad_fn is not None for o in outs)
