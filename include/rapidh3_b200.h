@@ -432,6 +432,8 @@ int rh3_kv_write(const rh3_kv_rows_args* a, cudaStream_t stream);
 int rh3_kv_read(const rh3_kv_rows_args* a, cudaStream_t stream);
 int64_t rh3_kv_attn_workspace_bytes(int64_t heads, int64_t group, int64_t page, int64_t D, int64_t per_seq, int64_t B, int64_t T,
                                     int64_t prefix);
+int rh3_kv_attn_launches(int64_t heads, int64_t group, int64_t page, int64_t D, int64_t per_seq, int64_t B, int64_t T,
+                         int64_t prefix);   /* kernels that a call of these sizes launches */
 /* Which kernel rh3_kv_attn takes: -1 (the default) the cheaper one for the call's sizes, 0 the one for few rows, 1 the one on 128-row
  * tensor-core tiles, 2 as 0 with a pass of its own for a shared prefix. For the whole process; returns the previous setting. Workspace sizes are asked for under the setting of the call. */
 int rh3_kv_attn_use_wide(int use);

@@ -78,6 +78,7 @@ SIGNATURES = {
     "rh3_kv_write": [_P, _P],
     "rh3_kv_read": [_P, _P],
     "rh3_kv_attn_workspace_bytes": [_I64] * 8,
+    "rh3_kv_attn_launches": [_I64] * 8,
     "rh3_kv_attn_use_wide": [_I],
     "rh3_kv_attn": [_P, _P, _I64, _P, _P],
     "rh3_upsample_causal2x": [_P, _P, _I64, _I64, _I64, _I64, _I64, _P],
@@ -93,7 +94,7 @@ _lib = None
 # kernels launched per entry point (for launch accounting in benchmarks)
 LAUNCHES = {"rh3_attn_kv_stats": 2, "rh3_attn_kv_stats_noalloc": 2, "rh3_attn_prepass": 3, "rh3_attn_tok_prepass": 5, "rh3_quant_tensor_fp8": 2, "rh3_te_gemm": 2, "rh3_version": 0, "rh3_gemm_use_pairs": 0, "rh3_gemm_tile": 0, "rh3_sm_count": 0, "rh3_check_status": 0,
             "rh3_attn_kv_stats_scratch_bytes": 0, "rh3_conv3d_gn_part_rows": 0, "rh3_block_workspace_bytes": 0,
-            "rh3_kv_attn_workspace_bytes": 0, "rh3_kv_attn_use_wide": 0}
+            "rh3_kv_attn_workspace_bytes": 0, "rh3_kv_attn_launches": 0, "rh3_kv_attn_use_wide": 0}
 launch_count = 0
 
 

@@ -811,6 +811,11 @@ extern "C" int64_t rh3_kv_attn_workspace_bytes(int64_t heads, int64_t group, int
   return kv_plan(heads, group, page, D, per_seq, B, T, prefix).bytes;
 }
 
+extern "C" int rh3_kv_attn_launches(int64_t heads, int64_t group, int64_t page, int64_t D, int64_t per_seq, int64_t B, int64_t T, int64_t prefix) {
+  if (heads <= 0 || group <= 0 || page <= 0 || (D != 64 && D != 128) || per_seq < 0 || B <= 0 || T <= 0 || prefix < 0) return 0;
+  return kv_plan(heads, group, page, D, per_seq, B, T, prefix).pre.grid ? 2 : 1;
+}
+
 extern "C" int rh3_kv_attn_use_wide(int use) { return g_use_wide.exchange(use < 0 || use > 2 ? -1 : use); }
 
 extern "C" int rh3_kv_attn(const rh3_kv_attn_args* a, void* workspace, int64_t workspace_bytes, int32_t* counters, cudaStream_t stream) {

@@ -141,12 +141,13 @@ def use_wide(use):
     return _PATHS[before + 1]
 
 
-def _workspace_bytes(*sizes):
+def _plan(*sizes):
+    """(workspace bytes, kernels) of an attention call."""
     need = _NEED.get(sizes)
     if need is None:
         if len(_NEED) > 4096:
             _NEED.clear()
-        need = _NEED[sizes] = _lib.lib().rh3_kv_attn_workspace_bytes(*sizes)
+        need = _NEED[sizes] = _lib.lib().rh3_kv_attn_workspace_bytes(*sizes), _lib.lib().rh3_kv_attn_launches(*sizes)
     return need
 
 
@@ -198,7 +199,7 @@ def write(cache, k, v, rows):
     if v.shape != k.shape:
         raise RuntimeError("k and v must have the same number of rows")
     args = _TENSORS.pack(*at) + cache._args + rows._args + _ROWS.pack(k.shape[0], cache.kind, _DTYPES[k.dtype])
-    _run(cache._index, lambda: _lib.call("rh3_kv_write", args, _lib.stream()))
+    _run(cache._index, lambda: _lib.call("rh3_kv_write", args, _lib.stream(), launches=min(1, k.shape[0])))
 
 
 def read(cache, rows, total, dtype=torch.bfloat16, out=None):
@@ -216,7 +217,7 @@ def read(cache, rows, total, dtype=torch.bfloat16, out=None):
             if t.shape != shape or t.dtype != dtype or t.device != cache.device or not t.is_contiguous() or t.data_ptr() % 16:
                 raise RuntimeError(f"out: expected two contiguous, 16-byte aligned {dtype} tensors {shape} on the cache's device")
     args = _TENSORS.pack(k.data_ptr(), 0, 0, v.data_ptr(), 0, 0) + cache._args + rows._args + _ROWS.pack(total, cache.kind, _DTYPES[dtype])
-    _run(cache._index, lambda: _lib.call("rh3_kv_read", args, _lib.stream()))
+    _run(cache._index, lambda: _lib.call("rh3_kv_read", args, _lib.stream(), launches=min(1, total)))
     return k, v
 
 
@@ -247,10 +248,10 @@ def _attend(q, cache, rows, prefix, prefix_len, scale, causal, out):
 
     def launch():
         stream = _lib.stream()
-        need = _workspace_bytes(cache.kv_heads, group, cache.page, d, *rows._sizes, t, prefix_len)
+        need, kernels = _plan(cache.kv_heads, group, cache.page, d, *rows._sizes, t, prefix_len)
         counters, work = _scratch(q.device, cache._index, stream, need)
         with _LAUNCH:
-            _lib.call("rh3_kv_attn", args, work.data_ptr(), need, counters.data_ptr(), stream)
+            _lib.call("rh3_kv_attn", args, work.data_ptr(), need, counters.data_ptr(), stream, launches=kernels)
 
     _run(cache._index, launch)
     return out

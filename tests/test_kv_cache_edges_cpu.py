@@ -4,7 +4,7 @@ import itertools
 import pytest
 import torch
 
-from rapid_h3_b200 import kv_cache
+from rapid_h3_b200 import _lib, kv_cache
 
 
 @pytest.mark.parametrize("t,heads", [(1, 1), (1, 4), (5, 1), (2, 2), (3, 4), (4, 3), (7, 5)])
@@ -26,3 +26,18 @@ def test_scratch_of_many_streams_is_not_kept_for_ever(monkeypatch):
     assert kv_cache._scratch("cpu", 0, 199, 100)[0] is made[199][0] and kv_cache._scratch("cpu", 0, 0, 100)[0] is not made[0][0]
     big = kv_cache._scratch("cpu", 0, 199, kv_cache._KEPT_BYTES + 1)
     assert big[0] is made[199][0] and big[1].numel() == kv_cache._KEPT_BYTES + 1
+
+
+def test_launches_of_a_call_are_counted():
+    """A prefix with a pass of its own takes two."""
+    lib, before = _lib.lib(), kv_cache.use_wide(None)
+    sizes = lambda rows, prefix: (8, 4, 64, 128, 11, 64, rows, prefix)
+    try:
+        for use, want in ((False, 1), ("apart", 2), (True, 1)):
+            kv_cache.use_wide(use)
+            assert lib.rh3_kv_attn_launches(*sizes(64, 700)) == want and lib.rh3_kv_attn_launches(*sizes(64, 0)) == 1
+        kv_cache.use_wide(None)
+        assert lib.rh3_kv_attn_launches(*sizes(64, 12000)) == 2 and lib.rh3_kv_attn_launches(*sizes(64, 64)) == 1
+        assert lib.rh3_kv_attn_launches(*sizes(0, 64)) == 0
+    finally:
+        kv_cache.use_wide(before)

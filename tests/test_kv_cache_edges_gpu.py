@@ -290,3 +290,20 @@ def test_no_gradient_passes(kv):
     kv.write(cache, x, x, rows)
     outs = [*kv.read(cache, rows, 3), kv.attention(x, cache, rows), kv.attention_shared(x, cache, rows, rows.table[0], 2)]
     assert not any(o.requires_grad or o.grad_fn is not None for o in outs)
+
+
+def test_launches_are_counted(kv):
+    from rapid_h3_b200 import _lib
+    cache = kv.alloc(20, 2, 64, 16, "int8")
+    fill(cache, 1)
+    rows = kv.Rows(torch.tensor([[0, 1]], **I32), torch.tensor([3], **I32), torch.tensor([0, 3], **I32))
+    x, pre = randn(1, 3, 2, 64).cuda(), torch.arange(2, 20, **I32)
+    before = kv.use_wide(None)
+    for use, call, want in ((None, lambda: kv.write(cache, x, x, rows), 1), (None, lambda: kv.write(cache, x[:0], x[:0], rows), 0), (None, lambda: kv.read(cache, rows, 3), 1),
+                            (None, lambda: kv.read(cache, rows, 0), 0), (None, lambda: kv.attention(x, cache, rows), 1), (None, lambda: kv.attention(x[:0], cache, rows), 0),
+                            ("apart", lambda: kv.attention_shared(x, cache, rows, pre, 280), 2), (True, lambda: kv.attention_shared(x, cache, rows, pre, 280), 1)):
+        kv.use_wide(use)
+        count = _lib.launch_count
+        call()
+        assert _lib.launch_count - count == want
+    kv.use_wide(before)
