@@ -1,5 +1,6 @@
 """What the cache operators decide on the host, against brute force."""
 import itertools
+import random
 
 import pytest
 import torch
@@ -41,3 +42,43 @@ def test_launches_of_a_call_are_counted():
         assert lib.rh3_kv_attn_launches(*sizes(0, 64)) == 0
     finally:
         kv_cache.use_wide(before)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_parts_of_a_prefix_fit_the_room_made_for_them(wide):
+    """kv_plan's arithmetic, restated: what a unit weighs in the prefix pass, in tiles, or in keys with what it costs to begin; the CTAs with parts of a
+    unit are those of its first and last tile's positions and all between, as the pass behind counts them; room is made for pre_splits."""
+    rng = random.Random(1)
+    full = 0
+    for _ in range(4000):
+        heads, tiles = rng.choice([1, 2, 8, 30]), rng.choice([1, 2, 7, rng.randint(1, 200)])
+        prefix = rng.choice([1, 127, 128, 129, rng.randint(1, 40000)])
+        kt, units = -(-prefix // 128), heads * tiles
+        most = rng.choice([1, 2, 3]) * rng.choice([132, 148]) if not wide else rng.choice([132, 148])
+        grid = min(units * kt, most)
+        cost = 640 if wide else rng.choice([0, 2])
+        unit = cost + (prefix if wide else kt)
+        first, last = cost, cost + (kt - 1) * (128 if wide else 1)
+        run = -(-units * unit // grid)
+        if wide:
+            run = max(run, 128)
+        splits = min((last - first) // run + 2, kt)
+
+        def tile(y):   # the first tile behind position y
+            return kt if y >= unit else 0 if y <= cost else min(kt, -(-(y - cost) // 128) if wide else y - cost)
+
+        parts = {}     # unit -> the CTAs that write a part of it
+        for c in range(grid):
+            x, x1 = min(units * unit, c * run), min(units * unit, (c + 1) * run)
+            while x < x1:
+                u, y = divmod(x, unit)
+                end = min(unit, x1 - u * unit)
+                if tile(y) < tile(end):
+                    parts.setdefault(u, []).append(c)
+                x = u * unit + end
+        assert len(parts) == units
+        for u, ctas in parts.items():
+            x = u * unit
+            assert ctas == list(range((x + first) // run, (x + last) // run + 1)) and len(ctas) <= splits
+            full += len(ctas) == splits > 1
+    assert full > 1000
