@@ -388,7 +388,7 @@ int rh3_vae_gemm_swiglu(const void* xq, int64_t lda, const void* wq, const float
  * row quantizers (custom_nodes/rapid_h3/kernels.py:75-82).
  *
  * Cache: codes kc, vc [pages][heads][page][D] bytes (kind 0: int8, 1: e4m3), scales ks, vs fp32 [pages][heads][page]; page = 16, 32, 64 or
- * 128 tokens, D = 64 or 128; all four 16-byte aligned.
+ * 128 tokens, D = 64 or 128; all four 16-byte aligned. Codes are numbers (rh3_kv_write stores no NaN of e4m3).
  * Batch: table int32 [B] rows of per_seq pages at table_stride, the pages of each sequence in order; lens int32 [B], the tokens each
  * sequence holds, the call's own among them; starts int32 [B + 1], ascending: rows starts[b] .. starts[b + 1] - 1 of the call are the last
  * tokens of sequence b, row t at position lens[b] - (starts[b + 1] - t). They are read on the device: a captured call follows them. Rows at or behind starts[B] (T may be larger: a padded

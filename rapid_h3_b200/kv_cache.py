@@ -35,7 +35,8 @@ _ATTN, _ROWS = struct.Struct("@qqPqqfiii"), struct.Struct("@qii")
 
 class KVCache:
     """Codes k, v [pages, kv_heads, page, head_dim] (int8, or float8_e4m3fn) and scales k_scale, v_scale fp32 [pages, kv_heads, page],
-    contiguous, on one CUDA device. page: 16, 32, 64 or 128 tokens; head_dim: 64 or 128."""
+    contiguous, on one CUDA device. page: 16, 32, 64 or 128 tokens; head_dim: 64 or 128. Codes are numbers (`write` stores no NaN of e4m3: rows that
+    are not finite have codes 0). The tensors' contents may change, the tensors of an object may not: calls go by their addresses."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page", "head_dim", "kind", "device", "_index", "_args")
 
@@ -45,8 +46,8 @@ class KVCache:
             raise RuntimeError(f"k: expected int8 or e4m3 codes [pages, kv_heads, page, head_dim], got {tuple(k.shape)} {k.dtype}")
         if v.shape != k.shape or v.dtype != k.dtype:
             raise RuntimeError("v must have the shape and type of k")
-        self.pages, self.kv_heads, self.page, self.head_dim = k.shape
-        if self.page not in PAGES or self.head_dim not in HEAD_DIMS or self.pages < 1 or not 1 <= self.kv_heads <= 1024:
+        pages, kv_heads, page, head_dim = k.shape
+        if page not in PAGES or head_dim not in HEAD_DIMS or pages < 1 or not 1 <= kv_heads <= 1024:
             raise RuntimeError(f"page must be one of {PAGES}, head_dim one of {HEAD_DIMS}: got a cache of {tuple(k.shape)}")
         for t in (k_scale, v_scale):
             if t.dtype != torch.float32 or t.shape != k.shape[:3]:
@@ -54,11 +55,16 @@ class KVCache:
         for t in (k, v, k_scale, v_scale):
             if not t.is_contiguous() or t.data_ptr() % 16 or t.device != k.device:
                 raise RuntimeError("the cache's tensors must be contiguous, 16-byte aligned and on one device")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.device = k.device
-        self.kind = 0 if k.dtype == torch.int8 else 1
-        self._index = k.get_device()
-        self._args = _CACHE.pack(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.pages, self.kv_heads, self.page, self.head_dim)
+        args = _CACHE.pack(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k.shape)
+        for name, x in zip(self.__slots__, (k, v, k_scale, v_scale, *k.shape, 0 if k.dtype == torch.int8 else 1, k.device, k.get_device(), args)):
+            object.__setattr__(self, name, x)
+
+    def __setattr__(self, name, value):
+        if value is not getattr(self, name, None):   # it is for `cache.v_scale *= 2`
+            raise AttributeError(f"cannot assign {name}: calls go by the addresses of the tensors that the cache was made of")
+
+    def __reduce__(self):   # a copy has its own tensors' addresses
+        return KVCache, (self.k, self.v, self.k_scale, self.v_scale)
 
 
 def alloc(pages, kv_heads, head_dim=128, page=64, kind="int8", device="cuda"):
@@ -100,6 +106,9 @@ class Rows:
         object.__setattr__(self, "_sizes", (table.shape[1], len(lens)))
         object.__setattr__(self, "_args", _BATCH.pack(table.data_ptr(), max(table.stride(0), table.shape[1]), table.shape[1], lens.data_ptr(),
                                                       starts.data_ptr(), len(lens)))
+
+    def __reduce__(self):   # as KVCache
+        return Rows, (self.table, self.lens, self.starts)
 
 
 # What the attention kernels need beside their arguments, per (device, stream), where only calls that cannot overlap share it: the counters,

@@ -1,5 +1,7 @@
 """What the cache operators decide on the host, against brute force."""
+import copy
 import itertools
+import pickle
 import random
 
 import pytest
@@ -82,3 +84,22 @@ def test_parts_of_a_prefix_fit_the_room_made_for_them(wide):
             assert ctas == list(range((x + first) // run, (x + last) // run + 1)) and len(ctas) <= splits
             full += len(ctas) == splits > 1
     assert full > 1000
+
+
+def test_a_descriptor_that_is_copied_or_stored_describes_its_own_tensors(monkeypatch):
+    """The addresses that calls take are those of the tensors that the object shows."""
+    monkeypatch.setattr(_lib, "require_cuda", lambda *t: None)
+    codes, scales = (torch.zeros(2, 1, 16, 64, dtype=torch.int8) for _ in range(2)), (torch.zeros(2, 1, 16) for _ in range(2))
+    cache = kv_cache.KVCache(*codes, *scales)
+    rows = kv_cache.Rows(torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32))
+    for again in (copy.copy, copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))):
+        c, r = again(cache), again(rows)
+        assert c._args == kv_cache.KVCache(c.k, c.v, c.k_scale, c.v_scale)._args
+        assert r._args == kv_cache.Rows(r.table, r.lens, r.starts)._args
+        assert (c.k.data_ptr() == cache.k.data_ptr()) == (r.lens.data_ptr() == rows.lens.data_ptr()) == (again is copy.copy)
+    cache.v_scale += 1
+    assert float(cache.v_scale.min()) == 1
+    with pytest.raises(AttributeError):
+        cache.v_scale = torch.zeros(2, 1, 16)
+    with pytest.raises(AttributeError):
+        rows.lens = torch.zeros(1, dtype=torch.int32)
