@@ -402,7 +402,8 @@ int rh3_vae_gemm_swiglu(const void* xq, int64_t lda, const void* wq, const float
  *   scale and reads back as NaN. Sequences that share pages write them in no particular order: they must not write the same token.
  * rh3_kv_read: k, v [T][heads][D] contiguous = codes * scale in fp32, rounded once to dtype.
  * rh3_kv_attn: out[t, head] = softmax(scale * q . k) v over the keys of the row's sequence, at most its own position if causal; heads * group
- *   query heads, head h * group + i reads KV head h. A row without a key gives 0. With prefix > 0 every row sees the first
+ *   query heads, head h * group + i reads KV head h. A row without a key gives 0; a key
+ *   or query that is not finite gives NaN in the rows that see it, and in no others. V scales that a row sees may differ by up to 2^120. With prefix > 0 every row sees the first
  *   `prefix` tokens of prefix_table's pages as well, before its own keys; lens, starts and positions then count the own part alone.
  *   workspace: rh3_kv_attn_workspace_bytes() bytes, 256-byte aligned, in use until the call's kernels are done. counters:
  *   RH3_KV_COUNTERS ints on the device, 0 before a call and left 0 by it (clear them after a call that gave up: a status other than 0, 120 and 121);

@@ -17,7 +17,8 @@
 // instructions for four of them. K codes enter as code + 128 in the low bits of an fp16 (a subnormal number, (code + 128) * 2^-24,
 // exact): the accumulators begin at -128 * 2^-24 * sum q, the same for every key of a row. V codes are brought to fp16 proper: there the
 // offset would be summed over all keys.
-// Measured: a token of each of 48 sequences of 8,192 to 16,384 tokens, 8 KV heads of 8: 203 us, 6.26 TB/s (0.96 of a copy); of up to 4,096: 52 us.
+// Measured, CUDA events around 50 calls: a token of each of 48 sequences of 8,192 to 16,384 tokens, 8 KV heads of 8: 203 us, 6.2 TB/s of codes and scales
+// (0.94 of a copy; 217 us in a row of 2,000 calls); of up to 4,096: 53 us, 52 replayed from a graph.
 // The order of channels and keys inside an mma is free, so each lane takes the channels and keys whose bytes it can load
 // 16 at a time: channel order (K) 16c .. 16c+15 of lane c, key order n -> (n >> 1) | ((n & 1) << 2), output channels of
 // lane group g 16g' .. 16g'+15.

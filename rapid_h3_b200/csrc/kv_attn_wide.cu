@@ -27,7 +27,8 @@
 // Shared memory: Q 2 x 32 KB | three fp16 tiles of 32 KB (K and V in turn) | three raw tiles of 16 KB. TMEM: S0 | S1 | O0 | O1.
 // Bound, per step of 128 keys and 256 rows: 2,048 cycles of the tensor pipe, as many of the exponential unit, about 2,800 of shared memory (products'
 // operands 1,536, conversion 768, the keys' scales 512). Measured: 4,850, as all three wait for one another; 2,011 tokens x 32 heads behind
-// 16,000 take 620 us, 0.90 PFLOP/s (0.55 of the library's bf16 product).
+// 16,000 take 610 us at 1,965 MHz, 0.92 PFLOP/s (0.56 of the library's bf16 product), and 670 us call behind call for a second or more, when
+// the power cap holds the SMs at 1,790 MHz (0.60 of the library's product under that cap).
 #include "kv_attn.cuh"
 
 namespace rh3 {
