@@ -60,11 +60,12 @@ class KVCache:
             object.__setattr__(self, name, x)
 
     def __setattr__(self, name, value):
-        if value is not getattr(self, name, None):   # it is for `cache.v_scale *= 2`
+        if name in KVCache.__slots__ and value is not getattr(self, name):   # it is for `cache.v_scale *= 2`
             raise AttributeError(f"cannot assign {name}: calls go by the addresses of the tensors that the cache was made of")
+        object.__setattr__(self, name, value)
 
     def __reduce__(self):   # a copy has its own tensors' addresses
-        return KVCache, (self.k, self.v, self.k_scale, self.v_scale)
+        return type(self), (self.k, self.v, self.k_scale, self.v_scale)
 
 
 def alloc(pages, kv_heads, head_dim=128, page=64, kind="int8", device="cuda"):
@@ -108,7 +109,7 @@ class Rows:
                                                       starts.data_ptr(), len(lens)))
 
     def __reduce__(self):   # as KVCache
-        return Rows, (self.table, self.lens, self.starts)
+        return type(self), (self.table, self.lens, self.starts)
 
 
 # What the attention kernels need beside their arguments, per (device, stream), where only calls that cannot overlap share it: the counters,

@@ -89,7 +89,7 @@ def test_parts_of_a_prefix_fit_the_room_made_for_them(wide):
 def test_a_descriptor_that_is_copied_or_stored_describes_its_own_tensors(monkeypatch):
     """The addresses that calls take are those of the tensors that the object shows."""
     monkeypatch.setattr(_lib, "require_cuda", lambda *t: None)
-    codes, scales = (torch.zeros(2, 1, 16, 64, dtype=torch.int8) for _ in range(2)), (torch.zeros(2, 1, 16) for _ in range(2))
+    codes, scales = [torch.zeros(2, 1, 16, 64, dtype=torch.int8) for _ in range(2)], [torch.zeros(2, 1, 16) for _ in range(2)]
     cache = kv_cache.KVCache(*codes, *scales)
     rows = kv_cache.Rows(torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32))
     for again in (copy.copy, copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))):
@@ -101,5 +101,13 @@ def test_a_descriptor_that_is_copied_or_stored_describes_its_own_tensors(monkeyp
     assert float(cache.v_scale.min()) == 1
     with pytest.raises(AttributeError):
         cache.v_scale = torch.zeros(2, 1, 16)
+    class Named(kv_cache.KVCache):
+        pass
+
+    named = Named(*codes, *scales)
+    named.name = "text"
+    assert named.name == "text" and type(copy.copy(named)) is Named
+    with pytest.raises(AttributeError):
+        named.k = codes[0] + 1
     with pytest.raises(AttributeError):
         rows.lens = torch.zeros(1, dtype=torch.int32)
