@@ -206,10 +206,14 @@ def write(cache, k, v, rows):
     their sequences. A row with a NaN or an infinity reads back as NaN. Sequences that share a page must not write the same token."""
     _check_batch(cache, rows)
     at = (*_check_rows(k, "k", cache, cache.kv_heads, tuple(_DTYPES)), *_check_rows(v, "v", cache, cache.kv_heads, (k.dtype,)))
-    if v.shape != k.shape:
+    shape = k.shape
+    if v.shape != shape:
         raise RuntimeError("k and v must have the same number of rows")
-    args = _TENSORS.pack(*at) + cache._args + rows._args + _ROWS.pack(k.shape[0], cache.kind, _DTYPES[k.dtype])
-    _run(cache._index, lambda: _lib.call("rh3_kv_write", args, _lib.stream(), launches=min(1, k.shape[0])))
+    t = shape[0]
+    if t == 0:
+        return
+    args = _TENSORS.pack(*at) + cache._args + rows._args + _ROWS.pack(t, cache.kind, _DTYPES[k.dtype])
+    _run(cache._index, lambda: _lib.call("rh3_kv_write", args, _lib.stream()))
 
 
 def read(cache, rows, total, dtype=torch.bfloat16, out=None):
@@ -226,8 +230,10 @@ def read(cache, rows, total, dtype=torch.bfloat16, out=None):
         for t in (k, v):
             if t.shape != shape or t.dtype != dtype or t.device != cache.device or not t.is_contiguous() or t.data_ptr() % 16:
                 raise RuntimeError(f"out: expected two contiguous, 16-byte aligned {dtype} tensors {shape} on the cache's device")
+    if total == 0:
+        return k, v
     args = _TENSORS.pack(k.data_ptr(), 0, 0, v.data_ptr(), 0, 0) + cache._args + rows._args + _ROWS.pack(total, cache.kind, _DTYPES[dtype])
-    _run(cache._index, lambda: _lib.call("rh3_kv_read", args, _lib.stream(), launches=min(1, total)))
+    _run(cache._index, lambda: _lib.call("rh3_kv_read", args, _lib.stream()))
     return k, v
 
 
